@@ -334,6 +334,58 @@ int lk_hip_f16_elementwise(const void* a, const void* b, void* out, int64_t n, i
 /* weight packing: W f16[K, N] -> W^T f16[N, K] */
 int lk_hip_f16_transpose(const void* w, void* wt, int64_t k, int64_t n, void* stream);
 
+/* ---- 4-bit weights (MI355X backend). A value is s (c - 8): a code c of 0 .. 15 and the scale s of its group of 32, 64 or
+ *      128 consecutive k, an f16 >= 0 of at most 8 significant bits. A weight f16[K, N] is laid out once: q,
+ *      lk_hip_w4_codes_bytes, codes in tiles of 16 columns x 128 k; s, lk_hip_w4_scales_bytes, f16 [ceil(N / 16),
+ *      ceil(K / 128), 16, 128 / group]; both 16-byte aligned. ---- */
+int64_t lk_hip_w4_codes_bytes(int64_t n, int64_t k);
+int64_t lk_hip_w4_scales_bytes(int64_t n, int64_t k, int group);
+/* w f16[K, N] (nt: [N, K]) -> q, s: the smallest scale with 7 s >= the group's largest and 8 s >= minus its smallest value
+ * (at most 8128), codes rounded to nearest, halves up. A group with a value that is not finite becomes NaN. */
+int lk_hip_w4_quantize(const void* w, void* q, void* s, int64_t n, int64_t k, int group, int nt, void* stream);
+/* codes u8[K, N] (low 4 bits), scales f16[ceil(K / group), N] -> q, s */
+int lk_hip_w4_pack(const void* codes, const void* scales, void* q, void* s, int64_t n, int64_t k, int group, void* stream);
+/* q, s -> w f16[K, N], exact */
+int lk_hip_w4_unpack(const void* q, const void* s, void* w, int64_t n, int64_t k, int group, void* stream);
+/* out [M, N] = x f16[M, K] @ W (f32 sums): f16, + bias f16[N], + res f16[M, N]; silu(x @ W) * (x @ W2) with q2, s2; f32
+ * with f32_out. gamma f16[K] (M = 1, else null): x is rmsnorm(x, gamma, eps) first. K % 8 == 0; x, gamma 16-byte aligned. */
+int lk_hip_w4_gemm(const void* x, const void* gamma, const void* q, const void* s, const void* q2, const void* s2,
+                   const void* bias, const void* res, void* out, int64_t m, int64_t n, int64_t k, int group, int f32_out,
+                   float eps, void* stream);
+
+/* ---- key / value caches in 4 bits (MI355X backend): u8 [B, 2, kvh, 72 P], P rows (a multiple of 32) per (sequence, keys
+ *      or values, kv head): first 64 bytes of codes a row, then 4 f16 scales a row (groups of 32 of the head's 128 values);
+ *      16-byte aligned. pos: a device i64[B], the position of each sequence's first row of the call. ---- */
+/* k, v f16[B T, kvh 128] -> rows pos[b] .. of sequence b; rows outside the cache are dropped. A row whose key or value is not
+ * finite is held so that a query that sees it gets NaN. */
+int lk_hip_kv4_write(void* kv, const void* k, const void* v, const int64_t* pos, int64_t b, int64_t t, int kvh, int64_t cap,
+                     void* stream);
+/* qkv f16[B T, (qh + 2 kvh) 128]: q = rope(rmsnorm_heads(q, qg)) f16[B T, qh 128]; k = rope(rmsnorm_heads(k, kg)) and v
+ * written as lk_hip_kv4_write does */
+int lk_hip_kv4_qknorm_rope(const void* qkv, const void* qg, const void* kg, const int64_t* pos, void* kv, void* q, int64_t b,
+                           int64_t t, int qh, int kvh, int64_t cap, float eps, float theta, void* stream);
+/* blocks of 72 cap bytes -> f16 [blocks, cap, 128] */
+int lk_hip_kv4_read(const void* kv, void* out, int64_t blocks, int64_t cap, void* stream);
+/* q f16[B T, qh 128]: query i of sequence b (position pos[b] + i) attends to rows 0 .. pos[b] + i of its kv head; scale
+ * 1 / sqrt(128). A query whose position is outside the cache (a negative pos[b]: all of its sequence) gives NaN and
+ * records LK_DEVERR_POSITION. Returns 3 when the workspace is short. */
+int64_t lk_hip_kv4_attention_workspace_bytes(int64_t b, int64_t t, int qh, int kvh, int64_t cap);
+int lk_hip_kv4_attention(const void* q, const void* kv, const int64_t* pos, void* out, int64_t b, int64_t t, int qh, int kvh,
+                         int64_t cap, void* workspace, int64_t workspace_bytes, void* stream);
+/* kv u8 [L, B, 2, kvh, 72 P], B <= 32, L kvh <= 32767: rows 0 .. n[0] - 1 of sequence b become those of sequence parents[b],
+ * in place; a parent out of range gives NaN rows and records LK_DEVERR_INDEX. parents, n: device i64[B], i64[1] */
+int lk_hip_kv4_reorder(void* kv, const int64_t* parents, const int64_t* n, int64_t layers, int64_t b, int kvh, int64_t cap,
+                       void* stream);
+
+/* ---- beam search (MI355X backend): candidate (b, t) = scores[b] + logits[b, t] - log sum exp logits[b], a finished beam's
+ *      (done[b] != 0) its score at eos[0] alone; the k best, ties to the lowest b V + t. B, k <= 32, V <= 262144, 1 to 4
+ *      eos ids. What has no value (NaN; a row or score that is not finite) counts as -inf. out_done: the parent's, or the
+ *      token is an eos. Returns 3 when the workspace (16-byte aligned) is short. ---- */
+int64_t lk_hip_beam_select_workspace_bytes(int64_t b, int64_t v, int k);
+int lk_hip_beam_select_f32(const float* logits, const float* scores, const int64_t* done, float* out_scores,
+                           int64_t* out_parents, int64_t* out_tokens, int64_t* out_done, int64_t b, int64_t v, int k,
+                           const int* eos, int num_eos, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

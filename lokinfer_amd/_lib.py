@@ -44,6 +44,10 @@ def lib():
     L.lk_take_device_error.restype = i32
     L.lk_device_error_message.argtypes = [i32]
     L.lk_device_error_message.restype = C.c_char_p
+    L.lk_hip_kv4_attention_workspace_bytes.argtypes = [i64, i64, i32, i32, i64]
+    L.lk_hip_kv4_attention_workspace_bytes.restype = i64
+    L.lk_hip_beam_select_workspace_bytes.argtypes = [i64, i64, i32]
+    L.lk_hip_beam_select_workspace_bytes.restype = i64
     L.lk_init()
     _lib = L
     return L

@@ -77,6 +77,9 @@ void registerDecodeFusedKernels();
 void registerWinogradKernels();
 void registerF16Kernels();
 void registerGemmSplitKernels();
+void registerQ4Kernels();
+void registerKv4Kernels();
+void registerBeamKernels();
 
 inline unsigned ceilDiv(int64_t a, int64_t b) { return static_cast<unsigned>((a + b - 1) / b); }
 

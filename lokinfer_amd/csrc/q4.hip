@@ -1,0 +1,398 @@
+// Products with 4-bit weights (lk.ops.q4_gpu; no counterpart in the reference, whose weights are f16 or f32).
+//
+//   y[m, n] = sum_k x[m, k] s[k / G, n] (c[k, n] - 8),  x f16, codes c and scales s as in q4.h, G = 32, 64 or 128
+//
+//   lk_hip_w4_quantize   w f16[K, N] (or [N, K]) -> codes and scales in the layout below
+//   lk_hip_w4_pack       given codes u8[K, N] and scales f16[ceil(K / G), N] -> the same layout
+//   lk_hip_w4_unpack     -> f16[K, N], exact
+//   lk_hip_w4_gemm       x @ W, + bias, + residual, SwiGLU of two weights, f32 logits; RMSNorm in front of one row
+//
+// Layout: tiles of 16 columns x 128 k, q [ceil(N / 16), ceil(K / 128), 64, 4] words: word i of lane l holds the codes of column
+// l % 16, k = 32 i + 8 (l / 16) + 0 .. 7 of the tile, so a wave's 16-byte load is one contiguous KiB and its word i is the B
+// operand of a 16x16x32 MFMA (two tiles' words are those of 32x32x16 ones). Scales f16 [ceil(N / 16), ceil(K / 128), 16, 128 / G].
+// Columns and k past the weight's hold zeros (code 8, scale 0).
+#include <algorithm>
+
+#include "common.h"
+#include "lokinfer_hip.h"
+#include "q4.h"
+
+namespace lkd {
+
+struct W4Layout {
+  int64_t n, k, kb;  // logical sizes; kb = ceil(K / 128)
+  int group;
+};
+
+// one thread per (column of a tile, group): MODE 0 from w f16[K, N], 1 from w f16[N, K], 2 from codes u8[K, N] and scales
+template <int MODE>
+__global__ __launch_bounds__(256) void w4PackKernel(const void* __restrict__ src, const h16* __restrict__ scales,
+                                                    unsigned* __restrict__ q, h16* __restrict__ s, W4Layout p) {
+  const int per = 128 / p.group;
+  const int64_t cols = (p.n + 15) / 16 * 16, total = cols * p.kb * per;
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
+       id += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t n = id % cols, gi = id / cols, kb = gi / per;  // neighbouring threads on neighbouring columns
+    const int gb = static_cast<int>(gi - kb * per);
+    const int64_t k0 = gi * p.group;
+    const int live = n < p.n ? static_cast<int>(max<int64_t>(0, min<int64_t>(p.group, p.k - k0))) : 0;
+    const h16* w = static_cast<const h16*>(src);
+    float sc = 0.0f;
+    if (MODE == 2) {
+      if (live) sc = static_cast<float>(scales[gi * p.n + n]);
+    } else {
+      float hi = 0.0f, lo = 0.0f;
+      bool bad = false;
+      for (int j = 0; j < live; ++j) {
+        const float v = static_cast<float>(MODE == 0 ? w[(k0 + j) * p.n + n] : w[n * p.k + k0 + j]);
+        hi = fmaxf(hi, v);
+        lo = fminf(lo, v);
+        bad = bad || !(fabsf(v) < INFINITY);
+      }
+      sc = bad ? __builtin_nanf("") : q4Scale(hi, lo);
+    }
+    const int64_t tile = (n >> 4) * p.kb + kb;
+    s[(tile * 16 + (n & 15)) * per + gb] = static_cast<h16>(sc);
+    for (int o = 0; o < p.group / 8; ++o) {
+      unsigned word = 0;
+      for (int j = 0; j < 8; ++j) {
+        const int at = 8 * o + j;
+        unsigned c = 8u;
+        if (at < live) {
+          const int64_t k = k0 + at;
+          if (MODE == 2) c = static_cast<const uint8_t*>(src)[k * p.n + n] & 15u;
+          else c = q4Code(static_cast<float>(MODE == 0 ? w[k * p.n + n] : w[n * p.k + k]), sc);
+        }
+        word |= c << q4Shift(j);
+      }
+      const int in = gb * p.group + 8 * o;  // k within the tile
+      q[(tile * 64 + (n & 15) + 16 * ((in >> 3) & 3)) * 4 + (in >> 5)] = word;
+    }
+  }
+}
+
+// one thread per (8 k, column): out f16[K, N]
+__global__ __launch_bounds__(256) void w4UnpackKernel(const unsigned* __restrict__ q, const h16* __restrict__ s,
+                                                      h16* __restrict__ out, W4Layout p) {
+  const int per = 128 / p.group;
+  const int64_t total = (p.k + 7) / 8 * p.n;
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
+       id += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t k8 = id / p.n, n = id - k8 * p.n, k = 8 * k8, tile = (n >> 4) * p.kb + k / 128;
+    const int in = static_cast<int>(k & 127);
+    const h16 sc = s[(tile * 16 + (n & 15)) * per + in / p.group];
+    const half8 v = q4Ints(q[(tile * 64 + (n & 15) + 16 * ((in >> 3) & 3)) * 4 + (in >> 5)]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k + j < p.k) out[(k + j) * p.n + n] = v[j] * sc;
+  }
+}
+
+struct W4Params {
+  const h16* x;       // [M, K]
+  const h16* gamma;   // RMSNorm gain [K] (M = 1) or null
+  const uint4* q[2];  // gate, up for SwiGLU
+  const h16* s[2];
+  const h16* bias;  // [N] or null
+  const h16* res;   // [M, N] or null
+  void* out;        // f16 (or f32) [M, N]
+  int64_t m, n, k, kb;
+  float eps;
+};
+
+// Up to 16 MT rows: WAVES waves of a workgroup share one tile of 16 columns (SwiGLU: one of each weight), wave w taking the
+// k blocks w, w + WAVES, ...; their sums meet in LDS. x row j of a 16-row block is the A operand's row 4 (j % 4) + j / 4, so
+// that its sums are accumulator j / 4 of lanes 16 (j % 4) ..: a few rows need only RU = ceil(rows / 4) of the 4
+// accumulators scaled. A group's products are summed on its integers and scaled once, in f32.
+template <int MT, int RU, int G, int W, bool F32, bool RMS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void w4SkinnyKernel(W4Params p) {
+  __shared__ float red[WAVES][W][MT][RU][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int a = lane & 15, kq = lane >> 4;
+  const int64_t tile = blockIdx.x, m0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
+  constexpr int PER = 128 / G, STEPS = G / 32;
+  float rf = 1.0f;
+  if constexpr (RMS) rf = rmsFactor(rowSumSq(p.x, p.k, lane), p.k, p.eps);
+  float acc[W][MT][RU];
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < RU; ++r) acc[w][t][r] = 0.0f;
+  for (int64_t kb = wave; kb < p.kb; kb += WAVES) {
+    uint4 q[W];
+    h16 sc[W][PER];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const int64_t at = tile * p.kb + kb;
+      q[w] = p.q[w][at * 64 + lane];
+#pragma unroll
+      for (int g = 0; g < PER; ++g) sc[w][g] = p.s[w][(at * 16 + a) * PER + g];
+    }
+    half8 xa[4][MT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const int64_t row = m0 + 16 * t + 4 * (a & 3) + (a >> 2), k = kb * 128 + 32 * i + 8 * kq;
+        xa[i][t] = half8{};
+        if (row < p.m && k < p.k) {
+          xa[i][t] = ld8(p.x + row * p.k + k);
+          if constexpr (RMS) {
+            const half8 gv = ld8(p.gamma + k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) xa[i][t][e] = rmsElem(xa[i][t][e], gv[e], rf);
+          }
+        }
+      }
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const unsigned word[4] = {q[w].x, q[w].y, q[w].z, q[w].w};
+#pragma unroll
+      for (int g = 0; g < PER; ++g) {
+        f32x4 d[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) d[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = g * STEPS; i < (g + 1) * STEPS; ++i) {
+          const half8 b = q4Ints(word[i]);
+#pragma unroll
+          for (int t = 0; t < MT; ++t) d[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[i][t], b, d[t], 0, 0, 0);
+        }
+        const float s = static_cast<float>(sc[w][g]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int r = 0; r < RU; ++r) acc[w][t][r] = fmaf(s, d[t][r], acc[w][t][r]);
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < RU; ++r) red[wave][w][t][r][lane] = acc[w][t][r];
+  __syncthreads();
+  for (int o = threadIdx.x; o < MT * RU * 64; o += 64 * WAVES) {
+    const int l = o & 63, r = (o >> 6) % RU, t = (o >> 6) / RU;
+    const int64_t row = m0 + 16 * t + 4 * r + (l >> 4), col = tile * 16 + (l & 15);
+    if (row >= p.m || col >= p.n) continue;
+    float y[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      y[w] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v) y[w] += red[v][w][t][r][l];
+    }
+    if constexpr (F32) {
+      static_cast<float*>(p.out)[row * p.n + col] = y[0];
+    } else {
+      float v = y[0];
+      if constexpr (W == 2) v = siluMul(y[0], y[W - 1]);
+      if (p.bias) v += static_cast<float>(p.bias[col]);
+      if (p.res) v = static_cast<float>(p.res[row * p.n + col]) + v;
+      static_cast<h16*>(p.out)[row * p.n + col] = toH16(v);
+    }
+  }
+}
+
+}  // namespace lkd
+
+namespace {
+
+bool al16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
+bool groupOk(int g) { return g == 32 || g == 64 || g == 128; }
+int launched() { return hipGetLastError() == hipSuccess ? 0 : 2; }
+unsigned gridFor(int64_t threads) { return static_cast<unsigned>(std::min<int64_t>((threads + 255) / 256, 65536)); }
+
+template <int MT, int RU, int G, int W, bool F32, bool RMS>
+void launchSkinny(const lkd::W4Params& p, hipStream_t s) {
+  constexpr int WAVES = 4;
+  const dim3 grid(static_cast<unsigned>((p.n + 15) / 16), static_cast<unsigned>((p.m + 16 * MT - 1) / (16 * MT)));
+  hipLaunchKernelGGL((lkd::w4SkinnyKernel<MT, RU, G, W, F32, RMS, WAVES>), grid, dim3(64 * WAVES), 0, s, p);
+}
+
+template <int G, int W, bool F32>
+void launchW4(const lkd::W4Params& p, hipStream_t s) {
+  if (p.gamma) launchSkinny<1, 1, G, W, F32, true>(p, s);
+  else if (p.m <= 4) launchSkinny<1, 1, G, W, F32, false>(p, s);
+  else if (p.m <= 16) launchSkinny<1, 4, G, W, F32, false>(p, s);
+  else launchSkinny<2, 4, G, W, F32, false>(p, s);
+}
+
+template <int G>
+void launchW4(const lkd::W4Params& p, bool two, bool f32, hipStream_t s) {
+  if (two) launchW4<G, 2, false>(p, s);
+  else if (f32) launchW4<G, 1, true>(p, s);
+  else launchW4<G, 1, false>(p, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t lk_hip_w4_codes_bytes(int64_t n, int64_t k) { return (n + 15) / 16 * ((k + 127) / 128) * 1024; }
+int64_t lk_hip_w4_scales_bytes(int64_t n, int64_t k, int group) {
+  return groupOk(group) ? (n + 15) / 16 * ((k + 127) / 128) * 16 * (128 / group) * 2 : 0;
+}
+
+int lk_hip_w4_quantize(const void* w, void* q, void* s, int64_t n, int64_t k, int group, int nt, void* stream) {
+  if (n <= 0 || k <= 0 || !groupOk(group) || !al16(q) || !al16(s)) return 1;
+  const lkd::W4Layout p{n, k, (k + 127) / 128, group};
+  const unsigned grid = gridFor((n + 15) / 16 * 16 * p.kb * (128 / group));
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (nt)
+    hipLaunchKernelGGL(lkd::w4PackKernel<1>, dim3(grid), dim3(256), 0, st, w, nullptr, static_cast<unsigned*>(q),
+                       static_cast<lkd::h16*>(s), p);
+  else
+    hipLaunchKernelGGL(lkd::w4PackKernel<0>, dim3(grid), dim3(256), 0, st, w, nullptr, static_cast<unsigned*>(q),
+                       static_cast<lkd::h16*>(s), p);
+  return launched();
+}
+
+int lk_hip_w4_pack(const void* codes, const void* scales, void* q, void* s, int64_t n, int64_t k, int group, void* stream) {
+  if (n <= 0 || k <= 0 || !groupOk(group) || !al16(q) || !al16(s)) return 1;
+  const lkd::W4Layout p{n, k, (k + 127) / 128, group};
+  hipLaunchKernelGGL(lkd::w4PackKernel<2>, dim3(gridFor((n + 15) / 16 * 16 * p.kb * (128 / group))), dim3(256), 0,
+                     static_cast<hipStream_t>(stream), codes, static_cast<const lkd::h16*>(scales),
+                     static_cast<unsigned*>(q), static_cast<lkd::h16*>(s), p);
+  return launched();
+}
+
+int lk_hip_w4_unpack(const void* q, const void* s, void* w, int64_t n, int64_t k, int group, void* stream) {
+  if (n <= 0 || k <= 0 || !groupOk(group) || !al16(q) || !al16(s)) return 1;
+  const lkd::W4Layout p{n, k, (k + 127) / 128, group};
+  hipLaunchKernelGGL(lkd::w4UnpackKernel, dim3(gridFor((k + 7) / 8 * n)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const unsigned*>(q), static_cast<const lkd::h16*>(s), static_cast<lkd::h16*>(w), p);
+  return launched();
+}
+
+int lk_hip_w4_gemm(const void* x, const void* gamma, const void* q, const void* s, const void* q2, const void* s2,
+                   const void* bias, const void* res, void* out, int64_t m, int64_t n, int64_t k, int group, int f32_out,
+                   float eps, void* stream) {
+  using namespace lkd;
+  if (m < 0 || n <= 0 || k <= 0 || k % 8 != 0 || !groupOk(group) || !al16(x) || !al16(q) || !al16(s)) return 1;
+  if ((q2 == nullptr) != (s2 == nullptr) || (q2 && (bias || res || f32_out || !al16(q2) || !al16(s2)))) return 1;
+  if (f32_out && (bias || res)) return 1;
+  if (gamma && (m > 1 || !al16(gamma))) return 1;
+  if (m == 0) return 0;
+  if (m > 16 * 2 * 65535) return 1;
+  const W4Params p{static_cast<const h16*>(x), static_cast<const h16*>(gamma),
+                   {static_cast<const uint4*>(q), static_cast<const uint4*>(q2)},
+                   {static_cast<const h16*>(s), static_cast<const h16*>(s2)},
+                   static_cast<const h16*>(bias), static_cast<const h16*>(res), out, m, n, k, (k + 127) / 128, eps};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (group == 32) launchW4<32>(p, q2 != nullptr, f32_out != 0, st);
+  else if (group == 64) launchW4<64>(p, q2 != nullptr, f32_out != 0, st);
+  else launchW4<128>(p, q2 != nullptr, f32_out != 0, st);
+  return launched();
+}
+
+}  // extern "C"
+
+// ---- registry -----------------------------------------------------------------------------------------------------
+namespace lkh {
+
+namespace {
+
+bool w4Shapes(int64_t nt, int64_t kb, int64_t per, int64_t n, int64_t k, int64_t group) {
+  return groupOk(static_cast<int>(group)) && nt == (n + 15) / 16 && kb == (k + 127) / 128 && per == 128 / group;
+}
+
+// quantize_w4_f16_gpu: w[K, N] (nt: [N, K]) -> q i32[NT, KB, 256], s f16[NT, KB, 16, 128 / G]; attrs group, nt
+void runQuantizeW4(ExecCtx& ctx, const KernelArgs& a) {
+  const int64_t group = a.ints[9], nt = a.ints[10];
+  const int64_t k = a.ints[nt ? 1 : 0], n = a.ints[nt ? 0 : 1];
+  LK_REQUIRE(ctx, w4Shapes(a.ints[2], a.ints[3], a.ints[8], n, k, group) && a.ints[4] == 256 && a.ints[7] == 16 &&
+                      a.ints[5] == a.ints[2] && a.ints[6] == a.ints[3],
+             "quantize_w4: q i32[ceil(N / 16), ceil(K / 128), 256], s f16[.., .., 16, 128 / group], group 32, 64 or 128");
+  status(ctx, lk_hip_w4_quantize(a.ptrs[0], a.ptrs[1], a.ptrs[2], n, k, static_cast<int>(group), nt != 0, ctx.stream),
+         "quantize_w4: launch failed");
+}
+
+// pack_w4_u8_gpu: codes u8[K, N], scales f16[ceil(K / G), N] -> q, s; attr group
+void runPackW4(ExecCtx& ctx, const KernelArgs& a) {
+  const int64_t k = a.ints[0], n = a.ints[1], group = a.ints[11];
+  LK_REQUIRE(ctx, w4Shapes(a.ints[4], a.ints[5], a.ints[10], n, k, group) && a.ints[6] == 256 && a.ints[9] == 16 &&
+                      a.ints[3] == n && a.ints[2] == (k + group - 1) / group && a.ints[7] == a.ints[4] &&
+                      a.ints[8] == a.ints[5],
+             "pack_w4: codes u8[K, N], scales f16[ceil(K / group), N], group 32, 64 or 128");
+  status(ctx, lk_hip_w4_pack(a.ptrs[0], a.ptrs[1], a.ptrs[2], a.ptrs[3], n, k, static_cast<int>(group), ctx.stream),
+         "pack_w4: launch failed");
+}
+
+// unpack_w4_f16_gpu: q, s -> w f16[K, N]; attr group
+void runUnpackW4(ExecCtx& ctx, const KernelArgs& a) {
+  const int64_t k = a.ints[7], n = a.ints[8], group = a.ints[9];
+  LK_REQUIRE(ctx, n > 0 && k > 0 && w4Shapes(a.ints[0], a.ints[1], a.ints[6], n, k, group) && a.ints[2] == 256,
+             "unpack_w4: the weight's q and s, out f16[K, N]");
+  status(ctx, lk_hip_w4_unpack(a.ptrs[0], a.ptrs[1], a.ptrs[2], n, k, static_cast<int>(group), ctx.stream),
+         "unpack_w4: launch failed");
+}
+
+// gemm_w4[_bias|_add|_swiglu]_f16_gpu, rmsnorm_gemm_w4[_swiglu]_f16_gpu (one row), lm_head_w4_f16_gpu:
+// x[M, K] [, g[K]], q, s [, q2, s2] [, bias[N] | res[M, N]] -> [M, N]; attr group; float eps with g
+enum : int { W4_PLAIN, W4_BIAS, W4_ADD, W4_SWIGLU, W4_LOGITS };
+template <int EPI, bool RMS>
+void runGemmW4(ExecCtx& ctx, const KernelArgs& a) {
+  Ints it(a);
+  int ptr = 0;
+  const int64_t m = it.next(), k = it.next();
+  const void* x = a.ptrs[ptr++];
+  const void* g = nullptr;
+  if (RMS) {
+    g = a.ptrs[ptr++];
+    LK_REQUIRE(ctx, it.next() == k, "rmsnorm_gemm_w4: g must be f16[K]");
+    LK_REQUIRE(ctx, m == 1, "rmsnorm_gemm_w4: one row (normalize more rows first)");
+  }
+  const int wts = EPI == W4_SWIGLU ? 2 : 1;
+  int64_t dims[2][7];
+  const void* q[2] = {nullptr, nullptr};
+  const void* s[2] = {nullptr, nullptr};
+  for (int w = 0; w < wts; ++w) {
+    q[w] = a.ptrs[ptr++];
+    s[w] = a.ptrs[ptr++];
+    for (int i = 0; i < 7; ++i) dims[w][i] = it.next();
+  }
+  const void *bias = nullptr, *res = nullptr;
+  int64_t e0 = 0, e1 = 0;
+  if (EPI == W4_BIAS) {
+    bias = a.ptrs[ptr++];
+    e0 = it.next();
+  } else if (EPI == W4_ADD) {
+    res = a.ptrs[ptr++];
+    e0 = it.next();
+    e1 = it.next();
+  }
+  const int64_t om = it.next(), n = it.next(), group = it.next();
+  for (int w = 0; w < wts; ++w)
+    LK_REQUIRE(ctx, w4Shapes(dims[w][0], dims[w][1], dims[w][6], n, k, group) && dims[w][2] == 256 &&
+                        dims[w][3] == dims[w][0] && dims[w][4] == dims[w][1] && dims[w][5] == 16,
+               "gemm_w4: x f16[M, K], a weight f16[K, N] in 4 bits, group 32, 64 or 128");
+  LK_REQUIRE(ctx, om == m && (EPI != W4_BIAS || e0 == n) && (EPI != W4_ADD || (e0 == m && e1 == n)),
+             "gemm_w4: out [M, N], bias f16[N], res f16[M, N]");
+  status(ctx, lk_hip_w4_gemm(x, g, q[0], s[0], q[1], s[1], bias, res, a.ptrs[ptr], m, n, k, static_cast<int>(group),
+                             EPI == W4_LOGITS, F(a, 0, 1e-6f), ctx.stream),
+         "gemm_w4: K must be a multiple of 8 and the operands 16-byte aligned");
+}
+
+}  // namespace
+
+void registerQ4Kernels() {
+  const Device G = Device::Gpu;
+  registerKernel({"quantize_w4_f16_gpu", G, runQuantizeW4, 1, 2});
+  registerKernel({"pack_w4_u8_gpu", G, runPackW4, 2, 2});
+  registerKernel({"unpack_w4_f16_gpu", G, runUnpackW4, 2, 1});
+  registerKernel({"gemm_w4_f16_gpu", G, runGemmW4<W4_PLAIN, false>, 3, 1});
+  registerKernel({"gemm_w4_bias_f16_gpu", G, runGemmW4<W4_BIAS, false>, 4, 1});
+  registerKernel({"gemm_w4_add_f16_gpu", G, runGemmW4<W4_ADD, false>, 4, 1});
+  registerKernel({"gemm_w4_swiglu_f16_gpu", G, runGemmW4<W4_SWIGLU, false>, 5, 1});
+  registerKernel({"lm_head_w4_f16_gpu", G, runGemmW4<W4_LOGITS, false>, 3, 1});
+  registerKernel({"rmsnorm_gemm_w4_f16_gpu", G, runGemmW4<W4_PLAIN, true>, 4, 1});
+  registerKernel({"rmsnorm_gemm_w4_swiglu_f16_gpu", G, runGemmW4<W4_SWIGLU, true>, 6, 1});
+  registerKernel({"rmsnorm_lm_head_w4_f16_gpu", G, runGemmW4<W4_LOGITS, true>, 4, 1});
+}
+
+}  // namespace lkh

@@ -586,6 +586,9 @@ static void registerAll() {
     registerWinogradKernels();
     registerF16Kernels();
     registerGemmSplitKernels();
+    registerQ4Kernels();
+    registerKv4Kernels();
+    registerBeamKernels();
     std::sort(names().begin(), names().end());
   });
 }

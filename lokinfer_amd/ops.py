@@ -921,6 +921,29 @@ def argmax_f32_gpu(x):
     return _launch("argmax_f32_gpu", [x], [(x.shape[0],)], out_dtypes=[i64])
 
 
+def beam_select_f32_gpu(logits, scores, done, k, eos):
+    """(MI355X backend) A beam search's step over logits f32[B, V], the beams' scores f32[B] and done i64[B]: the k best of
+    the candidates scores[b] + logits[b, t] - log sum exp logits[b] (a beam with done[b] != 0 has one, its score at eos[0]),
+    ties to the lowest b V + t -> (scores f32[k], parents i64[k], tokens i64[k], done i64[k]), best first; done: the parent's,
+    or the token is one of `eos` (1 to 4 ids). What has no value (a NaN, a row or a score that is not finite) counts as
+    -inf. B, k <= 32, V <= 262144. Not traceable."""
+    check(current_graph() is None, "beam_select runs eagerly or in a stream-captured function, not in a traced one")
+    _gpu(logits, scores, done)
+    _f32(logits, rank=2)
+    _f32(scores, rank=1)
+    b, v = logits.shape
+    k, eos = int(k), [int(e) for e in eos]
+    dev = GpuContext.shared().device
+    check(all(x.t.device == dev for x in (logits, scores, done)), f"operands must be on {dev}")
+    check(1 <= b <= 32 and 1 <= k <= 32 and 1 <= v <= 262144 and k <= b * v, "B and k at most 32, V at most 262144, k <= B V")
+    check(scores.shape[0] == b and done.dtype == i64 and tuple(done.shape) == (b,), "scores must be f32[B], done i64[B]")
+    check(1 <= len(eos) <= 4 and all(0 <= e < v for e in eos), "eos must be 1 to 4 ids below V")
+    need = GpuContext.shared().lib.lk_hip_beam_select_workspace_bytes(b, v, k)
+    return _launch("beam_select_f32_gpu", [logits, scores, done], [(k,), (k,), (k,), (k,), (need // 4,)], dict(eos=eos),
+                   out_dtypes=[f32, i64, i64, i64, f32])[:4]
+
+
+
 # ---- Kokoro token-rate sequence + signal kernels (MI355X backend: the reference runs these on the host) ------
 
 def lstm_bidir_t_f32_gpu(x, w_ih, w_hh_t, b):

@@ -1,0 +1,103 @@
+"""TEST INFRASTRUCTURE ONLY. Values held in 4 bits, attention over caches of them and a beam search's step in float64 numpy,
+from their definitions (lokinfer_amd/q4_gpu.py, ops.beam_select_f32_gpu)."""
+from __future__ import annotations
+
+import numpy as np
+
+
+def scale_of(hi: float, lo: float) -> float:
+    """The smallest f16 of at most 8 significant bits with 7 s >= hi and 8 s >= -lo, at most 8128 (hi >= 0 >= lo), found by
+    search from the exact conditions."""
+    if hi == 0 and lo == 0:
+        return 0.0
+    a = max(hi / 7, -lo / 8)
+    e = max(int(np.floor(np.log2(a))) - 8, -24)  # one bit lower than needed: the search walks up
+    m = max(int(np.floor(a / 2.0 ** e)) - 2, 0)
+    while True:
+        s = m * 2.0 ** e
+        odd = m
+        while odd and odd % 2 == 0:
+            odd //= 2
+        if odd < 256 and 7 * s >= hi and 8 * s >= -lo:
+            return min(s, 8128.0)
+        m += 1
+
+
+def quantize(x: np.ndarray):
+    """x f16[..., G] -> (codes int[..., G], scales f64[...]); a group that is not finite: scale NaN, codes 8."""
+    flat = np.asarray(x, np.float64).reshape(-1, x.shape[-1])
+    codes = np.full(flat.shape, 8, np.int64)
+    scales = np.zeros(len(flat))
+    for i, g in enumerate(flat):
+        if not np.isfinite(g).all():
+            scales[i] = np.nan
+            continue
+        s = scales[i] = scale_of(max(g.max(), 0.0), min(g.min(), 0.0))
+        if s > 0:
+            codes[i] = 8 + np.clip(np.floor(g / s + 0.5), -8, 7).astype(np.int64)
+    return codes.reshape(x.shape), scales.reshape(x.shape[:-1])
+
+
+def weight_values(w: np.ndarray, group: int) -> np.ndarray:
+    """w f16[K, N] -> the values f64[K, N] that its 4-bit form holds (groups along K)."""
+    k, n = w.shape
+    out = np.empty((k, n))
+    for k0 in range(0, k, group):
+        codes, s = quantize(w[k0:k0 + group].T)
+        out[k0:k0 + group] = ((codes - 8) * s[:, None]).T
+    return out
+
+
+def cache_values(k: np.ndarray, v: np.ndarray, kvh: int):
+    """Keys and values f64[rows, kvh, 128] that rows f16[rows, kvh 128] are held as; a row (of one head) whose key or value
+    is not finite: NaN keys, zero values."""
+    rows = k.shape[0]
+    out = []
+    ok = np.isfinite(k.astype(np.float64)).reshape(rows, kvh, 128).all(-1) & \
+        np.isfinite(v.astype(np.float64)).reshape(rows, kvh, 128).all(-1)
+    for x, bad in ((k, np.nan), (v, 0.0)):
+        x = np.where(ok[..., None], x.reshape(rows, kvh, 128), 0).astype(np.float16)
+        codes, s = quantize(x.reshape(rows, kvh, 4, 32))
+        y = ((codes - 8) * s[..., None]).reshape(rows, kvh, 128)
+        out.append(np.where(ok[..., None], y, bad))
+    return out
+
+
+def attention(q: np.ndarray, key: np.ndarray, val: np.ndarray, pos: int):
+    """q f16[T, qh, 128] at positions pos + i over key, val f64[P, kvh, 128] -> (f64[T, qh, 128], the largest score error
+    term: sqrt(sum (q k)^2) / sqrt(128) and |score|, over the keys seen)."""
+    t, qh, _ = q.shape
+    kvh = key.shape[1]
+    q = q.astype(np.float64)
+    out = np.empty(q.shape)
+    term = np.zeros((t, qh))
+    for h in range(qh):
+        kk, vv = key[:, h // (qh // kvh)], val[:, h // (qh // kvh)]
+        for i in range(t):
+            n = pos + i + 1
+            s = kk[:n] @ q[i, h] / np.sqrt(128)
+            e = np.exp(s - s.max())
+            out[i, h] = (e / e.sum()) @ vv[:n]
+            norm = np.sqrt((kk[:n] ** 2) @ (q[i, h] ** 2)) / np.sqrt(128)
+            term[i, h] = (np.sqrt(128) * norm + np.abs(s)).max()
+    return out, term
+
+
+def beam_select(logits, scores, done, k, eos):
+    """-> (scores f64[k], parents, tokens, done)."""
+    x = np.asarray(logits, np.float64)
+    b, v = x.shape
+    cand = np.full((b, v), -np.inf)
+    for i in range(b):
+        if not np.isfinite(scores[i]):
+            continue
+        if done[i]:
+            cand[i, eos[0]] = scores[i]
+            continue
+        m = x[i].max()
+        if np.isfinite(m):
+            cand[i] = float(scores[i]) + (x[i] - (m + np.log(np.exp(x[i] - m).sum())))
+    cand = np.where(np.isnan(cand), -np.inf, cand).reshape(-1)
+    at = np.argsort(-cand, kind="stable")[:k]
+    parent, token = at // v, at % v
+    return cand[at], parent, token, np.array([int(bool(done[p]) or t in eos) for p, t in zip(parent, token)])
