@@ -17,6 +17,11 @@ Per layer (variant "opt", the reference's _lm_layer_opt; at T = 1 two fusions of
 then logits = lm_head_last(rmsnorm(h, norm), embed). Variant "basic" is the reference's op-per-op graph
 (:275-287). Weights are the reference's folded layout (`fold_weights`, :19-66: linear weights [in, out], the tied
 embedding stored once as "embed"), packed on upload as W^T for the kernels.
+
+Variant "q4" (MI355X backend) holds the projections and the LM head in 4 bits (lk.ops.q4_gpu; the embedding's rows are
+looked up in f16) and takes a 4-bit cache of B sequences, kv u8[L, B, 2, kvh, 72 P]. A call runs the first S of them, S the
+length of pos: ids i64[S T], logits f32[S, V]. The layer is "opt"'s with its products, QK-norm / RoPE / cache write and
+attention in their 4-bit forms. `beam_search` decodes with it.
 """
 from __future__ import annotations
 
@@ -27,6 +32,7 @@ import torch
 
 from . import ops
 from . import f16_gpu as F
+from . import q4_gpu as Q4
 from .compiler import capture as lk_capture
 from .runtime import GpuContext
 from .tensor import Tensor, f16
@@ -95,12 +101,13 @@ def config5_inputs(cfg: Qwen3Config = CONFIG5, n_audio: int = 400, n_prompt: int
 
 
 class Qwen3Lm:
-    """Weights uploaded and packed once; call(ids, audio, pos, kv) -> logits (reference build_generate)."""
+    """Weights uploaded and packed once; call(ids, audio, pos, kv) -> logits (reference build_generate). `group`: the k
+    that share a scale in the 4-bit weights of variant "q4"."""
 
     def __init__(self, sd: dict[str, np.ndarray], cfg: Qwen3Config = CONFIG5, variant: str = "opt",
-                 graph: bool = True):
-        if variant not in ("basic", "opt"):
-            raise ValueError(f"variant {variant!r}: expected 'basic' or 'opt'")
+                 graph: bool = True, group: int = 64):
+        if variant not in ("basic", "opt", "q4"):
+            raise ValueError(f"variant {variant!r}: expected 'basic', 'opt' or 'q4'")
         self.cfg, self.variant = cfg, variant
         dev = GpuContext.shared().device
         self.device = dev
@@ -114,6 +121,12 @@ class Qwen3Lm:
         for i in range(cfg.layers):
             p = f"lm.{i}."
             L = {k: up(sd[p + k]) for k in ("ln1.g", "ln2.g", "qn.g", "kn.g")}
+            if variant == "q4":
+                L["qkv"] = Q4.pack_w4(np.concatenate([sd[p + "q.w"], sd[p + "k.w"], sd[p + "v.w"]], axis=1), group=group)
+                for k in ("gate", "up", "o", "down"):
+                    L[k] = Q4.pack_w4(sd[p + k + ".w"], group=group)
+                self.layers.append(L)
+                continue
             if variant == "opt":  # the reference's fold_opt concatenations (model.py:349-368)
                 L["qkv"] = F.pack(np.concatenate([sd[p + "q.w"], sd[p + "k.w"], sd[p + "v.w"]], axis=1))
                 L["gateup"] = F.pack(np.concatenate([sd[p + "gate.w"], sd[p + "up.w"]], axis=1))
@@ -123,14 +136,21 @@ class Qwen3Lm:
             L["o"] = F.pack(sd[p + "o.w"])
             L["down"] = F.pack(sd[p + "down.w"])
             self.layers.append(L)
+        if variant == "q4":
+            self.head = Q4.pack_w4(self.embed, group=group, nt=True)
         self.positions = torch.arange(1 << 16, dtype=torch.int64, device=dev)  # device pos views, no host copies
         self.counters = Tensor(torch.zeros(cfg.qh, dtype=torch.int32, device=dev))  # decode attention merge counters
         self.model = lk_capture(self._fn, graph=graph, mutable=(3,))  # kv: the caller's cache, written in place
 
-    def kv_cache(self, capacity: int) -> Tensor:
+    def kv_cache(self, capacity: int, batch: int = 1) -> Tensor:
         """A zeroed cache for `capacity` positions: f16[L, 2, capacity, kvh 128] on the device (reference kv_cache,
-        model.py:295-305)."""
+        model.py:295-305); variant "q4": of `batch` sequences, u8[L, batch, 2, kvh, 72 P], P = capacity rounded up to a
+        multiple of 32."""
         c = self.cfg
+        if self.variant == "q4":
+            return Q4.kv4_cache(batch, c.kvh, capacity, layers=c.layers)
+        if batch != 1:
+            raise ValueError("caches of more than one sequence need variant 'q4'")
         return Tensor(torch.zeros(c.layers, 2, capacity, c.dk, dtype=torch.float16, device=self.device))
 
     def _layer_opt(self, L, h, pos, kc, vc):
@@ -164,9 +184,27 @@ class Qwen3Lm:
         m, _ = F.rmsnorm_gemm_swiglu_opt_f16_gpu(h, L["ln2.g"], L["gateup"], c.eps)
         return F.gemm_add_opt_f16_gpu(m, L["down"], h)
 
+    def _layer_q4(self, L, h, pos, kv):
+        c = self.cfg
+        qkv = Q4.rmsnorm_gemm_w4_f16_gpu(h, L["ln1.g"], L["qkv"], c.eps)
+        q = Q4.qknorm_rope_kv4_f16_gpu(qkv, L["qn.g"], L["kn.g"], pos, kv, c.eps, c.theta)
+        h = Q4.gemm_w4_add_f16_gpu(Q4.attention_kv4_f16_gpu(q, kv, pos), L["o"], h)
+        m = Q4.rmsnorm_gemm_w4_swiglu_f16_gpu(h, L["ln2.g"], L["gate"], L["up"], c.eps)
+        return Q4.gemm_w4_add_f16_gpu(m, L["down"], h)
+
+    def _fn_q4(self, h: Tensor, pos: Tensor, kv: Tensor):
+        seqs = pos.shape[0]
+        for i, L in enumerate(self.layers):
+            h = self._layer_q4(L, h, pos, Tensor(kv.t[i, :seqs]))
+        last = h if h.shape[0] == seqs else Tensor(h.t.view(seqs, -1, self.cfg.d)[:, -1])
+        logits = Q4.rmsnorm_lm_head_w4_f16_gpu(last, self.norm, self.head, self.cfg.eps)
+        return logits, ops.argmax_f32_gpu(logits)
+
     def _fn(self, ids: Tensor, audio: Tensor, pos: Tensor, kv: Tensor):
         c = self.cfg
         h = F.scatter_audio_f16_gpu(F.embedding_f16_gpu(ids, self.embed), ids, audio)
+        if self.variant == "q4":
+            return self._fn_q4(h, pos, kv)
         opt = self.variant == "opt"
         layer = self._layer_basic
         if opt:
@@ -180,20 +218,29 @@ class Qwen3Lm:
             logits = F.lm_head_last_f16_gpu(F.rmsnorm_f16_gpu(h, self.norm, c.eps), self.embed)
         return logits, ops.argmax_f32_gpu(logits)
 
-    def run(self, ids, audio, pos: int, kv: Tensor):
+    def run(self, ids, audio, pos: int, kv: Tensor, seqs: int = 1):
         """(logits f32[1, V], argmax i64[1]) of the last new token; the compiled graph's own buffers (overwritten by
-        the next call with the same shapes). pos + T must fit the cache."""
+        the next call with the same shapes). pos + T must fit the cache. Variant "q4": of each of the cache's first
+        `seqs` sequences, ids i64[seqs T], all at position pos."""
         c = self.cfg
         ids = self._dev(ids, np.int64)
         audio = self._dev(audio, np.float16)
-        T, P = ids.shape[0], kv.shape[2]
-        if tuple(kv.shape) != (c.layers, 2, P, c.dk) or kv.dtype != f16:
-            raise ValueError(f"kv must be f16[{c.layers}, 2, P, {c.dk}]")
+        if self.variant == "q4":
+            P = Q4.kv4_capacity(kv)
+            if kv.ndim != 5 or tuple(kv.shape[:1] + kv.shape[2:4]) != (c.layers, 2, c.kvh) or not 1 <= seqs <= kv.shape[1]:
+                raise ValueError(f"kv must be u8[{c.layers}, B, 2, {c.kvh}, 72 P] with B >= {seqs}")
+            T, rest = divmod(ids.shape[0], seqs)
+            if rest:
+                raise ValueError(f"{ids.shape[0]} ids for {seqs} sequences")
+        else:
+            T, P = ids.shape[0], kv.shape[2]
+            if tuple(kv.shape) != (c.layers, 2, P, c.dk) or kv.dtype != f16 or seqs != 1:
+                raise ValueError(f"kv must be f16[{c.layers}, 2, P, {c.dk}], one sequence")
         if not (T >= 1 and 0 <= pos and pos + T <= P):
             raise ValueError(f"qwen3: positions {pos}..{pos + T - 1} outside the {P}-row cache")
-        p = Tensor(self.positions[pos:pos + 1] if pos < self.positions.numel()
-                   else torch.tensor([pos], dtype=torch.int64, device=self.device))
-        return self.model.run_inplace(ids, audio, p, kv)
+        p = (self.positions[pos:pos + 1] if pos < self.positions.numel()
+             else torch.tensor([pos], dtype=torch.int64, device=self.device))
+        return self.model.run_inplace(ids, audio, Tensor(p.expand(seqs)), kv)
 
     def __call__(self, ids, audio, pos: int, kv: Tensor) -> np.ndarray:
         """Reference model(ids, audio, pos, kv): logits f32[1, V] (a host copy)."""
@@ -205,24 +252,30 @@ class Qwen3Lm:
         return Tensor(torch.from_numpy(np.ascontiguousarray(x, dtype)).to(self.device))
 
 
+def _prefill(model: Qwen3Lm, ids: np.ndarray, audio: np.ndarray, chunk: int, kv: Tensor):
+    """The prompt in chunks of <= `chunk` ids, each with the audio rows its pad ids take -> the last one's
+    (logits, argmax)."""
+    n_audio = len(audio)
+    dummy = np.zeros((1, model.cfg.d), np.float16)
+    out = None
+    for s in range(0, len(ids), chunk):
+        e = min(len(ids), s + chunk)
+        k0, k1 = min(max(s - AUDIO_START, 0), n_audio), min(max(e - AUDIO_START, 0), n_audio)
+        out = model.run(ids[s:e], audio[k0:k1] if k1 > k0 else dummy, s, kv)
+    return out
+
+
 def transcribe(model: Qwen3Lm, ids: np.ndarray, audio: np.ndarray, max_new: int, chunk: int = 2048,
                kv: Tensor | None = None, stop_at_eos: bool = True) -> list[int]:
     """The reference's caller loop (model.py:309-336) for the LM: prefill in chunks of <= `chunk` ids (each chunk
     gets the audio rows its pad ids take), then greedy decode until eos or max_new tokens. Each step's argmax stays
     on the device and feeds the next step; the tokens come back once at the end (an eos check reads one token per
     step only when stop_at_eos is set)."""
-    c = model.cfg
     T = len(ids)
     if kv is None:
         kv = model.kv_cache(T + max_new)
-    n_audio = len(audio)
-    dummy = np.zeros((1, c.d), np.float16)
-    am = None
-    for s in range(0, T, chunk):
-        e = min(T, s + chunk)
-        k0, k1 = min(max(s - AUDIO_START, 0), n_audio), min(max(e - AUDIO_START, 0), n_audio)
-        rows = audio[k0:k1] if k1 > k0 else dummy
-        _, am = model.run(ids[s:e], rows, s, kv)
+    _, am = _prefill(model, ids, audio, chunk, kv)
+    dummy = np.zeros((1, model.cfg.d), np.float16)
     toks = torch.empty(max_new, dtype=torch.int64, device=model.device)
     dummy_t = model._dev(dummy, np.float16)
     pos, n = T, 0
@@ -234,3 +287,38 @@ def transcribe(model: Qwen3Lm, ids: np.ndarray, audio: np.ndarray, max_new: int,
         _, am = model.run(Tensor(toks[n - 1:n]), dummy_t, pos, kv)
         pos += 1
     return [int(v) for v in toks[:n].cpu()]
+
+
+def beam_search(model: Qwen3Lm, ids: np.ndarray, audio: np.ndarray, beams: int, max_new: int, chunk: int = 2048,
+                kv: Tensor | None = None, length_penalty: float = 1.0, eos: tuple = EOS,
+                stop_when_done: bool = True) -> tuple[list[int], float]:
+    """Beam search with variant "q4" (MI355X backend; the reference decodes greedily): the prompt once, its cache given to
+    every beam, then a step of all beams, the best `beams` of their continuations (ops.beam_select_f32_gpu) and their
+    parents' caches moved (q4_gpu.kv4_reorder_gpu), until every beam has ended or has max_new tokens. Returns the tokens
+    (its eos among them) and the summed log-probability of the beam with the best sum / length^length_penalty. Everything stays
+    on the device; with stop_when_done one flag per step is read."""
+    if model.variant != "q4":
+        raise ValueError("beam search needs variant 'q4'")
+    if not 1 <= beams <= 32 or max_new < 1:
+        raise ValueError("beams must be 1 .. 32, max_new positive")
+    T, dev = len(ids), model.device
+    if kv is None:
+        kv = model.kv_cache(T + max_new, beams)
+    if kv.ndim != 5 or kv.shape[1] != beams or Q4.kv4_capacity(kv) < T + max_new - 1:
+        raise ValueError(f"kv must hold {beams} sequences of {T + max_new - 1} positions")
+    logits, _ = _prefill(model, ids, audio, chunk, kv)
+    scores, done = (Tensor(torch.zeros(1, dtype=t, device=dev)) for t in (torch.float32, torch.int64))
+    dummy = model._dev(np.zeros((1, model.cfg.d), np.float16), np.float16)
+    tokens = torch.full((beams, max_new), eos[0], dtype=torch.int64, device=dev)
+    length = torch.zeros(beams, dtype=torch.int64, device=dev)
+    for n in range(max_new):
+        was = done.t
+        scores, parents, tok, done = ops.beam_select_f32_gpu(logits, scores, done, beams, eos)
+        tokens, length = tokens[parents.t], length[parents.t] + (was[parents.t] == 0)
+        tokens[:, n] = tok.t
+        if n + 1 == max_new or (stop_when_done and bool((done.t > 0).all())):
+            break
+        Q4.kv4_reorder_gpu(kv, parents, Tensor(torch.full((1,), T + n, dtype=torch.int64, device=dev)))
+        logits, _ = model.run(tok, dummy, T + n, kv, seqs=beams)
+    best = int((scores.t / length.float() ** length_penalty).argmax())
+    return [int(t) for t in tokens[best, : int(length[best])].cpu()], float(scores.t[best])

@@ -101,3 +101,35 @@ def beam_select(logits, scores, done, k, eos):
     at = np.argsort(-cand, kind="stable")[:k]
     parent, token = at // v, at % v
     return cand[at], parent, token, np.array([int(bool(done[p]) or t in eos) for p, t in zip(parent, token)])
+
+
+class _Kv:
+    """The cache of OracleLm4: what is written is held in 4 bits."""
+
+    def __init__(self, layers, capacity, dk, dt):
+        self.a = np.zeros((layers, 2, capacity, dk), dt)
+        self.shape = self.a.shape
+
+    def __getitem__(self, at):
+        return self.a[at]
+
+    def __setitem__(self, at, rows):
+        rows = np.asarray(rows).astype(np.float16)
+        codes, s = quantize(rows.reshape(rows.shape[0], -1, 32))
+        self.a[at] = ((codes - 8) * s[..., None]).reshape(rows.shape)
+
+
+def oracle_lm(sd: dict, cfg, ops, capacity: int, group: int):
+    """oracle.qwen3.OracleLm over the values that 4-bit weights, LM head and cache hold."""
+    from . import qwen3 as Q
+
+    sd = dict(sd)
+    for k in list(sd):
+        if k.endswith(".w"):
+            sd[k] = weight_values(sd[k], group)
+    table = weight_values(sd["embed"].T, group).T
+
+    lm = Q.OracleLm(sd, cfg, ops, capacity)
+    lm.kv = _Kv(cfg.layers, capacity, cfg.dk, ops.dt)
+    ops.lm_head_last = lambda x, _: ops.c(x)[-1:] @ ops.c(table).T
+    return lm
