@@ -36,8 +36,8 @@ def lib():
     L.lk_kernel_is_gpu.restype = i32
     L.lk_kernel_arity.argtypes = [vp, C.POINTER(i32), C.POINTER(i32)]
     L.lk_kernel_arity.restype = i32
-    L.lk_run_kernel.argtypes = [vp, C.POINTER(vp), u32, C.POINTER(i64), u32, C.POINTER(C.c_double), u32, vp,
-                                C.c_uint64, vp]
+    # the three arrays by address: ctypes arrays, or the buffer of an array.array (cheaper to make, GpuContext.run)
+    L.lk_run_kernel.argtypes = [vp, vp, u32, vp, u32, vp, u32, vp, C.c_uint64, vp]
     L.lk_run_kernel.restype = i32
     L.lk_last_error.restype = C.c_char_p
     L.lk_take_device_error.argtypes = [C.POINTER(i64)]

@@ -198,6 +198,178 @@ __global__ __launch_bounds__(64 * WAVES) void w4SkinnyKernel(W4Params p) {
   }
 }
 
+// More rows: workgroup of NW x KG waves, tile BM rows x NW 64 columns (SwiGLU: 32 of the gate's and the up weight's same 32).
+// Wave (nw, kg) takes all BM rows of its 64 columns over the k blocks kg, kg + KG, ...; the KG sums meet in LDS. x goes through
+// LDS in stages of 64 k, two buffers, filled from two register sets (a stage is loaded while the one before the last
+// runs); the weights go from memory straight into the registers of the one wave that multiplies by them, two tiles' words
+// being the B operands of 32x32x16 MFMAs: a lane's column is l % 32, its k 8 (l / 32) + 0 .. 7 of each 16, which are words of
+// lanes 16 (2 c + l / 32) + l % 16 of the column's tile, c the half of the 32 k. They are scaled before the product (exact), so
+// the sums run through all k.
+template <int BM, int NW, int KG, int G, int W, bool F32>
+__global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
+  constexpr int RB = BM / 32, THREADS = 64 * NW * KG, PER = 128 / G;
+  constexpr int STAGE = BM * 64;                 // halves of one k group's stage
+  constexpr int CH = BM * 8 / (64 * NW);         // its 16-byte chunks per thread of the group
+  constexpr int SMEM_A = 2 * KG * STAGE * 2, SMEM_R = KG > 1 ? KG * NW * BM * 64 * 4 : 0;
+  __shared__ __attribute__((aligned(16))) char smem[SMEM_A > SMEM_R ? SMEM_A : SMEM_R];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nw = wave % NW, kg = wave / NW, gt = threadIdx.x - kg * NW * 64;
+  const int lr = lane & 31, lh = lane >> 5;
+  const GridItem gi = xcdOrderYFast();
+  const int64_t m0 = static_cast<int64_t>(gi.y) * BM, c0 = static_cast<int64_t>(gi.x) * NW * (W == 2 ? 32 : 64);
+  h16* as = reinterpret_cast<h16*>(smem) + kg * STAGE;  // buffer b at + b KG STAGE
+  // this wave's two blocks of 32 columns
+  const int64_t tiles = (p.n + 15) / 16;
+  const uint4* qp[2];
+  const h16* sp[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int w = W == 2 ? j : 0;
+    const int64_t col = c0 + (W == 2 ? 32 * nw : 64 * nw + 32 * j);
+    const int64_t tile = min<int64_t>(col / 16 + ((lane >> 4) & 1), tiles - 1);
+    qp[j] = p.q[w] + tile * p.kb * 64 + (lane & 15) + 16 * lh;
+    sp[j] = p.s[w] + (tile * p.kb * 16 + (lane & 15)) * PER;
+  }
+  // x: chunk id = gt + 64 NW i -> row id / 8, k 8 (id % 8); 16-byte chunk c of row r lies at slot c ^ (r / 2 % 8)
+  const h16* xp[CH];
+  int xo[CH];
+  const int xc = 8 * (gt & 7);
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int r = (gt + 64 * NW * i) >> 3;
+    xp[i] = p.x + min<int64_t>(m0 + r, p.m - 1) * p.k;
+    xo[i] = r * 64 + 8 * ((gt & 7) ^ ((r >> 1) & 7));
+  }
+  int fo[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) fo[q] = lr * 64 + 8 * ((2 * q + lh) ^ ((lr >> 1) & 7));
+  const int blocks = static_cast<int>((p.kb + KG - 1) / KG);  // of every k group (the last may have one less)
+  half8 xr[2][CH];
+  // stage st of this k group: k block kg + (st / 2) KG, half st % 2
+  const auto kOf = [&](int st) { return (kg + static_cast<int64_t>(st >> 1) * KG) * 128 + 64 * (st & 1) + xc; };
+  const auto xload = [&](int st, int set) {
+    const int64_t k = min<int64_t>(kOf(st), p.k - 8);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) xr[set][i] = ld8(xp[i] + k);
+  };
+  const auto xstore = [&](int st, int set, int buf) {
+    const bool zero = kOf(st) >= p.k;
+    const half8 z = {};
+#pragma unroll
+    for (int i = 0; i < CH; ++i) st8(as + buf * KG * STAGE + xo[i], zero ? z : xr[set][i]);
+  };
+  uint4 q[2][2];
+  h16 sc[2][PER];
+  const auto wload = [&](int blk) {
+    const int64_t kb = min<int64_t>(kg + static_cast<int64_t>(blk) * KG, p.kb - 1);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      q[j][0] = qp[j][kb * 64];
+      q[j][1] = qp[j][kb * 64 + 32];
+#pragma unroll
+      for (int g = 0; g < PER; ++g) sc[j][g] = sp[j][kb * 16 * PER + g];
+    }
+  };
+  f32x16 acc[RB][2];
+#pragma unroll
+  for (int i = 0; i < RB; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  xload(0, 0);
+  xload(1, 1);
+  wload(0);
+  xstore(0, 0, 0);
+  __syncthreads();
+  for (int b = 0; b < blocks; ++b) {
+    uint4 qc[2][2];
+    h16 cur[2][PER];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      qc[j][0] = q[j][0];
+      qc[j][1] = q[j][1];
+#pragma unroll
+      for (int g = 0; g < PER; ++g) cur[j][g] = sc[j][g];
+    }
+    wload(b + 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // stage 2 b + h, in buffer h
+      xload(2 * b + h + 2, h);
+      const h16* a = as + h * KG * STAGE;
+      if (KG == 1 || kg + b * KG < p.kb) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          half8 bf[2], af[RB];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint4 v = qc[j][s & 1];
+            const int i = 2 * h + (s >> 1);
+            const unsigned word = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+            const h16 f = cur[j][32 * i / G];
+            bf[j] = q4Ints(word) * half8{f, f, f, f, f, f, f, f};
+          }
+#pragma unroll
+          for (int i = 0; i < RB; ++i) af[i] = ld8(a + 32 * 64 * i + fo[s]);
+#pragma unroll
+          for (int i = 0; i < RB; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[i], bf[j], acc[i][j], 0, 0, 0);
+        }
+      }
+      xstore(2 * b + h + 1, h ^ 1, h ^ 1);
+      __syncthreads();
+    }
+  }
+  // accumulator r of block (i, j): row 32 i + 8 (r / 4) + 4 lh + r % 4, column lr of column block j
+  const auto put = [&](int64_t row, int64_t col, float y) {
+    if (row >= p.m || col >= p.n) return;
+    if constexpr (F32) {
+      static_cast<float*>(p.out)[row * p.n + col] = y;
+    } else {
+      if (p.bias) y += static_cast<float>(p.bias[col]);
+      if (p.res) y = static_cast<float>(p.res[row * p.n + col]) + y;
+      static_cast<h16*>(p.out)[row * p.n + col] = toH16(y);
+    }
+  };
+  if constexpr (KG == 1) {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int64_t row = m0 + 32 * i + 8 * (r >> 2) + 4 * lh + (r & 3);
+        if constexpr (W == 2) {
+          put(row, c0 + 32 * nw + lr, siluMul(acc[i][0][r], acc[i][1][r]));
+        } else {
+          put(row, c0 + 64 * nw + lr, acc[i][0][r]);
+          put(row, c0 + 64 * nw + 32 + lr, acc[i][1][r]);
+        }
+      }
+  } else {
+    float* red = reinterpret_cast<float*>(smem);  // [KG][NW][BM][64]
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          red[(wave * BM + 32 * i + 8 * (r >> 2) + 4 * lh + (r & 3)) * 64 + 32 * j + lr] = acc[i][j][r];
+    __syncthreads();
+    constexpr int COLS = W == 2 ? 32 : 64;
+    for (int o = threadIdx.x; o < NW * BM * COLS; o += THREADS) {
+      const int c = o % COLS, row = o / COLS % BM, v = o / (COLS * BM);
+      float y = 0.0f, u = 0.0f;
+#pragma unroll
+      for (int g = 0; g < KG; ++g) {
+        const float* at = red + ((g * NW + v) * BM + row) * 64 + c;
+        y += at[0];
+        if (W == 2) u += at[32];
+      }
+      put(m0 + row, c0 + v * COLS + c, W == 2 ? siluMul(y, u) : y);
+    }
+  }
+}
+
 }  // namespace lkd
 
 namespace {
@@ -214,12 +386,20 @@ void launchSkinny(const lkd::W4Params& p, hipStream_t s) {
   hipLaunchKernelGGL((lkd::w4SkinnyKernel<MT, RU, G, W, F32, RMS, WAVES>), grid, dim3(64 * WAVES), 0, s, p);
 }
 
+template <int BM, int NW, int KG, int G, int W, bool F32>
+void launchGemm(const lkd::W4Params& p, hipStream_t s) {
+  constexpr int BN = NW * (W == 2 ? 32 : 64);
+  const dim3 grid(static_cast<unsigned>((p.n + BN - 1) / BN), static_cast<unsigned>((p.m + BM - 1) / BM));
+  hipLaunchKernelGGL((lkd::w4GemmKernel<BM, NW, KG, G, W, F32>), grid, dim3(64 * NW * KG), 0, s, p);
+}
+
 template <int G, int W, bool F32>
 void launchW4(const lkd::W4Params& p, hipStream_t s) {
   if (p.gamma) launchSkinny<1, 1, G, W, F32, true>(p, s);
   else if (p.m <= 4) launchSkinny<1, 1, G, W, F32, false>(p, s);
   else if (p.m <= 16) launchSkinny<1, 4, G, W, F32, false>(p, s);
-  else launchSkinny<2, 4, G, W, F32, false>(p, s);
+  else if (((p.m + 127) / 128) * ((p.n * W + 255) / 256) >= 256) launchGemm<128, 4, 1, G, W, F32>(p, s);
+  else launchGemm<64, 1, 8, G, W, F32>(p, s);
 }
 
 template <int G>

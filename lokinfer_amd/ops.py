@@ -34,6 +34,8 @@ def check(cond: bool, msg: str = "invalid operands") -> None:
 
 def _gpu(*xs: Tensor) -> None:
     for x in xs:
+        if type(x) is Tensor and x.t.is_cuda:
+            continue
         if isinstance(x, Value):
             continue
         if not isinstance(x, Tensor):
@@ -931,20 +933,21 @@ def beam_select_f32_gpu(logits, scores, done, k, eos):
     _gpu(logits, scores, done)
     _f32(logits, rank=2)
     _f32(scores, rank=1)
-    b, v = logits.shape
-    k, eos = int(k), [int(e) for e in eos]
-    dev = GpuContext.shared().device
-    check(all(x.t.device == dev for x in (logits, scores, done)), f"operands must be on {dev}")
+    ctx, k = GpuContext.shared(), int(k)
+    x, s, d = logits.t, scores.t, done.t
+    b, v = x.shape
+    check(x.device == s.device == d.device == ctx.device, f"operands must be on {ctx.device}")
     check(1 <= b <= 32 and 1 <= k <= 32 and 1 <= v <= 262144 and k <= b * v, "B and k at most 32, V at most 262144, k <= B V")
-    check(scores.shape[0] == b and done.dtype == i64 and tuple(done.shape) == (b,), "scores must be f32[B], done i64[B]")
+    check(s.shape[0] == b and d.dtype is torch.int64 and tuple(d.shape) == (b,), "scores must be f32[B], done i64[B]")
     check(1 <= len(eos) <= 4 and all(0 <= e < v for e in eos), "eos must be 1 to 4 ids below V")
-    need = GpuContext.shared().lib.lk_hip_beam_select_workspace_bytes(b, v, k)
-    return _launch("beam_select_f32_gpu", [logits, scores, done], [(k,), (k,), (k,), (k,), (need // 4,)], dict(eos=eos),
-                   out_dtypes=[f32, i64, i64, i64, f32])[:4]
+    work = ctx.lib.lk_hip_beam_select_workspace_bytes(b, v, k) // 4
+    best = torch.empty(k, dtype=torch.float32, device=ctx.device)
+    picks = torch.empty((3, k), dtype=torch.int64, device=ctx.device).unbind(0)
+    scratch = torch.empty(work, dtype=torch.float32, device=ctx.device)
+    ctx.run("beam_select_f32_gpu", [t.data_ptr() for t in (x, s, d, best, *picks, scratch)],
+            [b, v, b, b, k, k, k, k, work, *(int(e) for e in eos)], ())
+    return (Tensor(best), *(Tensor(t) for t in picks))
 
-
-
-# ---- Kokoro token-rate sequence + signal kernels (MI355X backend: the reference runs these on the host) ------
 
 def lstm_bidir_t_f32_gpu(x, w_ih, w_hh_t, b):
     """1-layer bidirectional nn.LSTM (gates i, f, g, o): x f32[T, I], w_ih f32[8H, I] (rows 0..4H forward),

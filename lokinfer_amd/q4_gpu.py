@@ -20,28 +20,49 @@ import numpy as np
 import torch
 
 from .graph import current_graph
-from .ops import OpError, _launch, check
+from .ops import OpError, check
 from .runtime import GpuContext
-from .tensor import Tensor, f16, f32, i32, i64, u8
+from .tensor import Tensor, f16, i32, u8
 
 GROUPS = (32, 64, 128)
 ROW = 72  # bytes of a cache row: 64 of codes, 4 f16 scales
 HD = 128
 
+_F16, _F32, _I32, _I64, _U8 = torch.float16, torch.float32, torch.int32, torch.int64, torch.uint8
 
-def _on_gpu(*xs):
+
+def _ctx() -> GpuContext:
     if current_graph() is not None:
         raise OpError("the 4-bit ops run eagerly or in a stream-captured function (lk.capture), not in a traced one")
-    for x in xs:
-        check(isinstance(x, Tensor), f"expected lk.Tensor, got {type(x).__name__}")
-        check(x.device == "gpu", "GPU kernel operands must be on the GPU (use ops.to_gpu)")
-    dev = GpuContext.shared().device
-    for x in xs:
-        check(x.t.device == dev, f"operands must be on {dev}, got one on {x.t.device}")
+    return GpuContext.shared()
 
 
-def _typed(x, dtype, rank, what):
-    check(isinstance(x, Tensor) and x.dtype == dtype and x.ndim == rank, f"{what} must be a rank {rank} {dtype.name} tensor")
+def _arg(x, dtype, rank, what) -> torch.Tensor:
+    """The torch tensor of an operand: of this type and rank, on the context's GPU."""
+    if not isinstance(x, Tensor):
+        raise OpError(f"{what}: expected lk.Tensor, got {type(x).__name__}")
+    t = x.t
+    if t.dtype is not dtype or t.dim() != rank:
+        raise OpError(f"{what} must be a rank {rank} {str(dtype)[6:]} tensor, got {str(t.dtype)[6:]}{list(t.shape)}")
+    if not t.is_cuda:
+        raise OpError(f"{what}: GPU kernel operands must be on the GPU (use ops.to_gpu)")
+    dev = _ctx().device
+    if t.get_device() != dev.index:
+        raise OpError(f"{what} must be on {dev}, is on {t.device}")
+    return t
+
+
+def _call(name, tensors, attrs=(), floats=()):
+    """Registry kernel `name` over torch tensors (operands, then outs) and its int and float attributes."""
+    ints: list[int] = []
+    for t in tensors:
+        ints.extend(t.shape)
+    ints.extend(attrs)
+    _ctx().run(name, [t.data_ptr() for t in tensors], ints, floats)
+
+
+def _empty(shape, dtype=_F16) -> torch.Tensor:
+    return torch.empty(shape, dtype=dtype, device=GpuContext.shared().device)
 
 
 # ---- weights ------------------------------------------------------------------------------------------------
@@ -57,24 +78,24 @@ class PackedWeight4:
         check(isinstance(q, Tensor) and q.dtype == i32 and tuple(q.shape) == tiles + (256,), "q does not fit the shape")
         check(isinstance(s, Tensor) and s.dtype == f16 and tuple(s.shape) == tiles + (16, 128 // group),
               "s does not fit the shape and group")
+        check(q.t.is_cuda and q.t.device == s.t.device, "q and s must be on one GPU")
         self.q, self.s, self.shape, self.group = q, s, (k, n), group
 
 
-def _w4_shapes(k, n, group):
+def _w4_empty(k, n, group):
     check(group in GROUPS, "group must be 32, 64 or 128")
     check(k > 0 and n > 0, "a weight needs at least one row and column")
-    t = (-(-n // 16), -(-k // 128))
-    return [t + (256,), t + (16, 128 // group)]
+    tiles = (-(-n // 16), -(-k // 128))
+    return _empty(tiles + (256,), _I32), _empty(tiles + (16, 128 // group))
 
 
 def quantize_w4_f16_gpu(w, group: int = 64, nt: bool = False) -> PackedWeight4:
     """w f16[K, N] (nt: f16[N, K], an embedding table as the LM head's weight) -> PackedWeight4."""
-    _on_gpu(w)
-    _typed(w, f16, 2, "w")
-    k, n = (w.shape[1], w.shape[0]) if nt else w.shape
-    q, s = _launch("quantize_w4_f16_gpu", [w], _w4_shapes(k, n, group), dict(group=int(group), nt=int(bool(nt))),
-                   out_dtypes=[i32, f16])
-    return PackedWeight4(q, s, (k, n), group)
+    wt = _arg(w, _F16, 2, "w")
+    n, k = wt.shape if nt else reversed(wt.shape)
+    q, s = _w4_empty(k, n, group)
+    _call("quantize_w4_f16_gpu", [wt, q, s], [group, int(bool(nt))])
+    return PackedWeight4(Tensor(q), Tensor(s), (k, n), group)
 
 
 def _scales_ok(s: torch.Tensor) -> bool:
@@ -97,110 +118,110 @@ def pack_w4(w, scales=None, group: int = 64, nt: bool = False) -> PackedWeight4:
     if scales is None:
         return quantize_w4_f16_gpu(up(w, np.float16), group, nt)
     check(not nt, "codes are given as u8[K, N]")
-    codes, scales = up(w, np.uint8), up(scales, np.float16)
-    _on_gpu(codes, scales)
-    _typed(codes, u8, 2, "codes")
-    _typed(scales, f16, 2, "scales")
-    shapes = _w4_shapes(*codes.shape, group)
-    check(tuple(scales.shape) == (-(-codes.shape[0] // group), codes.shape[1]), "scales must be f16[ceil(K / group), N]")
-    check(bool((codes.t < 16).all()), "codes must be 0 .. 15")
-    check(_scales_ok(scales.t), "scales must be >= 0, at most 8128, of at most 8 significant bits")
-    q, s = _launch("pack_w4_u8_gpu", [codes, scales], shapes, dict(group=int(group)), out_dtypes=[i32, f16])
-    return PackedWeight4(q, s, codes.shape, group)
+    codes, scales = _arg(up(w, np.uint8), _U8, 2, "codes"), _arg(up(scales, np.float16), _F16, 2, "scales")
+    k, n = codes.shape
+    q, s = _w4_empty(k, n, group)
+    check(tuple(scales.shape) == (-(-k // group), n), "scales must be f16[ceil(K / group), N]")
+    check(bool((codes < 16).all()), "codes must be 0 .. 15")
+    check(_scales_ok(scales), "scales must be >= 0, at most 8128, of at most 8 significant bits")
+    _call("pack_w4_u8_gpu", [codes, scales, q, s], [group])
+    return PackedWeight4(Tensor(q), Tensor(s), (k, n), group)
 
 
 def unpack_w4_f16_gpu(w: PackedWeight4):
     """The weight's values, f16[K, N] (exact)."""
-    _w(w)
-    return _launch("unpack_w4_f16_gpu", [w.q, w.s], [w.shape], dict(group=w.group), out_dtypes=[f16])
+    out = _empty(_w(w).shape)
+    _call("unpack_w4_f16_gpu", [w.q.t, w.s.t, out], [w.group])
+    return Tensor(out)
 
 
 def _w(w) -> PackedWeight4:
-    check(isinstance(w, PackedWeight4), "the weight must be a PackedWeight4 (pack_w4)")
-    _on_gpu(w.q, w.s)
+    if not isinstance(w, PackedWeight4):
+        raise OpError("the weight must be a PackedWeight4 (pack_w4)")
+    if w.q.t.get_device() != _ctx().device.index:
+        raise OpError(f"the weight must be on {_ctx().device}, is on {w.q.t.device}")
     return w
 
 
-def _gemm_rule(x, *ws):
-    _on_gpu(x)
-    _typed(x, f16, 2, "x")
-    for w in ws:
-        _w(w)
-        check(x.shape[1] == w.shape[0], f"x [M, K] and w [K, N]: inner dims differ: {x.shape}, {w.shape}")
-        check(w.shape == ws[0].shape and w.group == ws[0].group, "both weights must have one shape and group")
-    check(x.shape[1] % 8 == 0, "K must be a multiple of 8")
-    return x.shape[0], ws[0].shape[1]
-
-
-def _gemm(name, x, ws, extra=(), norm=None, dtype=f16):
-    m, n = _gemm_rule(x, *ws)
-    attrs = dict(group=ws[0].group)
-    ops = [x]
+def _gemm(name, x, w, w2=None, extra=None, norm=None, dtype=_F16):
+    """Registry product `name` of x and one or two weights; extra: (tensor, rank, name) of a bias or residual; norm:
+    (gain, eps)."""
+    xt = _arg(x, _F16, 2, "x")
+    (m, k), (wk, n) = xt.shape, _w(w).shape
+    if k != wk:
+        raise OpError(f"x [M, K] and w [K, N]: inner dims differ: {tuple(xt.shape)}, {w.shape}")
+    if k % 8:
+        raise OpError("K must be a multiple of 8")
+    ops, floats = [xt], ()
     if norm is not None:
-        ops.append(norm[0])
-        attrs["eps"] = float(norm[1])
-    for w in ws:
-        ops += [w.q, w.s]
-    return _launch(name, ops + list(extra), [(m, n)], attrs, out_dtypes=[dtype])
+        g = _arg(norm[0], _F16, 1, "g")
+        if g.shape[0] != k:
+            raise OpError("g must be f16[K]")
+        ops.append(g)
+        floats = (float(norm[1]),)
+    ops += [w.q.t, w.s.t]
+    if w2 is not None:
+        if _w(w2).shape != w.shape or w2.group != w.group:
+            raise OpError("both weights must have one shape and group")
+        ops += [w2.q.t, w2.s.t]
+    if extra is not None:
+        t = _arg(extra[0], _F16, extra[1], extra[2])
+        if tuple(t.shape) != ((m, n) if extra[1] == 2 else (n,)):
+            raise OpError(f"{extra[2]} must be f16{'[M, N]' if extra[1] == 2 else '[N]'}")
+        ops.append(t)
+    out = _empty((m, n), dtype)
+    ops.append(out)
+    _call(name, ops, (w.group,), floats)
+    return Tensor(out)
 
 
 def gemm_w4_f16_gpu(x, w):
     """x f16[M, K] @ w -> f16[M, N] (f32 sums)."""
-    return _gemm("gemm_w4_f16_gpu", x, [w])
+    return _gemm("gemm_w4_f16_gpu", x, w)
 
 
 def gemm_w4_bias_f16_gpu(x, w, b):
     """x @ w + b (b f16[N])."""
-    _on_gpu(b)
-    _typed(b, f16, 1, "b")
-    check(b.shape[0] == _w(w).shape[1], "b must be f16[N]")
-    return _gemm("gemm_w4_bias_f16_gpu", x, [w], [b])
+    return _gemm("gemm_w4_bias_f16_gpu", x, w, extra=(b, 1, "b"))
 
 
 def gemm_w4_add_f16_gpu(x, w, res):
     """res + x @ w (res f16[M, N])."""
-    _on_gpu(x, res)
-    _typed(res, f16, 2, "res")
-    check(tuple(res.shape) == (x.shape[0], _w(w).shape[1]), "res must be f16[M, N]")
-    return _gemm("gemm_w4_add_f16_gpu", x, [w], [res])
+    return _gemm("gemm_w4_add_f16_gpu", x, w, extra=(res, 2, "res"))
 
 
 def gemm_w4_swiglu_f16_gpu(x, gate, up):
     """silu(x @ gate) * (x @ up) -> f16[M, N]; both weights of one shape and group."""
-    return _gemm("gemm_w4_swiglu_f16_gpu", x, [gate, up])
+    return _gemm("gemm_w4_swiglu_f16_gpu", x, gate, up)
 
 
 def lm_head_w4_f16_gpu(x, w):
     """Logits x @ w -> f32[M, V] of every row (w: the table f16[V, D] packed with nt=True)."""
-    return _gemm("lm_head_w4_f16_gpu", x, [w], dtype=f32)
+    return _gemm("lm_head_w4_f16_gpu", x, w, dtype=_F32)
 
 
-def _normed(name, x, g, ws, eps, dtype=f16):
+def _normed(name, x, g, w, w2, eps, dtype=_F16):
     """rmsnorm(x, g) in front of a product: inside it for one row, else by rmsnorm_f16_gpu; the same bits."""
     from .f16_gpu import rmsnorm_f16_gpu
 
-    _gemm_rule(x, *ws)
-    _on_gpu(g)
-    _typed(g, f16, 1, "g")
-    check(g.shape[0] == x.shape[1], "g must be f16[K]")
-    if x.shape[0] == 1:
-        return _gemm("rmsnorm_" + name, x, ws, norm=(g, eps), dtype=dtype)
-    return _gemm(name, rmsnorm_f16_gpu(x, g, eps), ws, dtype=dtype)
+    if _arg(x, _F16, 2, "x").shape[0] == 1:
+        return _gemm("rmsnorm_" + name, x, w, w2, norm=(g, eps), dtype=dtype)
+    return _gemm(name, rmsnorm_f16_gpu(x, g, eps), w, w2, dtype=dtype)
 
 
 def rmsnorm_gemm_w4_f16_gpu(x, g, w, eps=1e-6):
     """gemm_w4(rmsnorm(x, g), w)."""
-    return _normed("gemm_w4_f16_gpu", x, g, [w], eps)
+    return _normed("gemm_w4_f16_gpu", x, g, w, None, eps)
 
 
 def rmsnorm_gemm_w4_swiglu_f16_gpu(x, g, gate, up, eps=1e-6):
     """gemm_w4_swiglu(rmsnorm(x, g), gate, up)."""
-    return _normed("gemm_w4_swiglu_f16_gpu", x, g, [gate, up], eps)
+    return _normed("gemm_w4_swiglu_f16_gpu", x, g, gate, up, eps)
 
 
 def rmsnorm_lm_head_w4_f16_gpu(x, g, w, eps=1e-6):
     """lm_head_w4(rmsnorm(x, g), w) -> f32[M, V]."""
-    return _normed("lm_head_w4_f16_gpu", x, g, [w], eps, dtype=f32)
+    return _normed("lm_head_w4_f16_gpu", x, g, w, None, eps, dtype=_F32)
 
 
 # ---- caches --------------------------------------------------------------------------------------------------
@@ -222,51 +243,58 @@ def kv4_capacity(kv: Tensor) -> int:
 
 
 def _kv(kv, pos):
-    _on_gpu(kv, pos)
-    kv4_capacity(kv)
-    check(kv.ndim == 4 and kv.shape[0] > 0 and kv.shape[1] == 2 and kv.shape[2] > 0, "kv must be u8[B, 2, kvh, 72 P]")
-    check(pos.dtype == i64 and tuple(pos.shape) == (kv.shape[0],), "pos must be i64[B]")
-    return kv.shape[0], kv.shape[2]
+    """(cache u8[B, 2, kvh, 72 P], pos i64[B]) as torch tensors."""
+    kt, pt = _arg(kv, _U8, 4, "kv"), _arg(pos, _I64, 1, "pos")
+    b, two, kvh, row = kt.shape
+    if b <= 0 or two != 2 or kvh <= 0 or row <= 0 or row % (32 * ROW):
+        raise OpError("kv must be u8[B, 2, kvh, 72 P], P a multiple of 32")
+    if pt.shape[0] != b:
+        raise OpError("pos must be i64[B]")
+    return kt, pt
 
 
 def _rows(x, b, what):
-    _typed(x, f16, 2, what)
-    check(x.shape[0] % b == 0, f"{what} must have B T rows")
+    t = _arg(x, _F16, 2, what)
+    if t.shape[0] % b:
+        raise OpError(f"{what} must have B T rows")
+    return t
 
 
 def kv4_write_f16_gpu(kv, k, v, pos):
     """Rows pos[b] .. pos[b] + T - 1 of sequence b = k, v f16[B T, kvh 128], quantised (kv in place); rows outside the cache
     are dropped. A row whose key or value is not finite makes every query that sees it NaN."""
-    b, kvh = _kv(kv, pos)
-    _on_gpu(k, v)
-    _rows(k, b, "k")
-    check(tuple(v.shape) == tuple(k.shape) and v.dtype == f16 and k.shape[1] == HD * kvh, "k, v must be f16[B T, kvh 128]")
-    return _launch("kv4_write_f16_gpu", [kv, k, v, pos], [], outs=[], inout=[0])
+    kt, pt = _kv(kv, pos)
+    key, val = _rows(k, kt.shape[0], "k"), _arg(v, _F16, 2, "v")
+    if val.shape != key.shape or key.shape[1] != HD * kt.shape[2]:
+        raise OpError("k, v must be f16[B T, kvh 128]")
+    _call("kv4_write_f16_gpu", [kt, key, val, pt])
 
 
 def qknorm_rope_kv4_f16_gpu(qkv, qg, kg, pos, kv, eps=1e-6, theta=1e6):
     """QK-norm + RoPE + cache write: qkv f16[B T, (qh + 2 kvh) 128] (q | k | v), row i of sequence b at position pos[b] + i.
     Returns q = rope(rmsnorm_heads(q, qg)) f16[B T, qh 128] and writes k = rope(rmsnorm_heads(k, kg)) and v as
     kv4_write does."""
-    b, kvh = _kv(kv, pos)
-    _on_gpu(qkv, qg, kg)
-    _rows(qkv, b, "qkv")
-    for g in (qg, kg):
-        _typed(g, f16, 1, "qg, kg")
-        check(g.shape[0] == HD, "qg and kg must be f16[128]")
-    dq = qkv.shape[1] - 2 * kvh * HD
-    check(dq > 0 and dq % HD == 0, "qkv must be f16[B T, (qh + 2 kvh) 128]")
-    return _launch("qknorm_rope_kv4_f16_gpu", [qkv, qg, kg, pos, kv], [(qkv.shape[0], dq)],
-                   dict(eps=float(eps), theta=float(theta)), out_dtypes=[f16], inout=[4])
+    kt, pt = _kv(kv, pos)
+    x = _rows(qkv, kt.shape[0], "qkv")
+    gains = [_arg(g, _F16, 1, "qg, kg") for g in (qg, kg)]
+    if any(g.shape[0] != HD for g in gains):
+        raise OpError("qg and kg must be f16[128]")
+    dq = x.shape[1] - 2 * kt.shape[2] * HD
+    if dq <= 0 or dq % HD:
+        raise OpError("qkv must be f16[B T, (qh + 2 kvh) 128]")
+    q = _empty((x.shape[0], dq))
+    _call("qknorm_rope_kv4_f16_gpu", [x, *gains, pt, kt, q], (), (float(eps), float(theta)))
+    return Tensor(q)
 
 
 def kv4_read_f16_gpu(kv):
     """The values that a cache (or any u8[..., 72 P] part of one) holds: f16[..., P, 128]."""
-    _on_gpu(kv)
     cap = kv4_capacity(kv)
-    flat = Tensor(kv.t.view(-1, kv.shape[-1]))
-    out = _launch("kv4_read_f16_gpu", [flat], [(flat.shape[0], cap, HD)], out_dtypes=[f16])
-    return Tensor(out.t.view(*kv.shape[:-1], cap, HD))
+    kt = _arg(kv, _U8, kv.t.dim(), "kv")
+    out = _empty((*kt.shape[:-1], cap, HD))
+    blocks = kt.numel() // (ROW * cap)
+    _ctx().run("kv4_read_f16_gpu", (kt.data_ptr(), out.data_ptr()), (blocks, ROW * cap, blocks, cap, HD), ())
+    return Tensor(out)
 
 
 def attention_kv4_f16_gpu(q, kv, pos):
@@ -274,27 +302,31 @@ def attention_kv4_f16_gpu(q, kv, pos):
     attends to rows 0 .. pos[b] + i of its kv head (already written); qh a multiple of the cache's kvh; scale
     1 / sqrt(128) -> f16[B T, qh 128]. A query whose position is outside the cache (with a negative pos[b], every query of
     the sequence) gives NaN and a device error."""
-    b, kvh = _kv(kv, pos)
-    _on_gpu(q)
-    _rows(q, b, "q")
-    check(q.shape[1] > 0 and q.shape[1] % (HD * kvh) == 0, "q must be f16[B T, qh 128], qh a multiple of kvh")
-    need = GpuContext.shared().lib.lk_hip_kv4_attention_workspace_bytes(b, q.shape[0] // b, q.shape[1] // HD, kvh,
-                                                                        kv4_capacity(kv))
-    out, _ = _launch("attention_kv4_f16_gpu", [q, kv, pos], [tuple(q.shape), (-(-need // 4),)], out_dtypes=[f16, f32])
-    return out
+    kt, pt = _kv(kv, pos)
+    b, _, kvh, row = kt.shape
+    qt = _rows(q, b, "q")
+    rows, width = qt.shape
+    if width <= 0 or width % (HD * kvh):
+        raise OpError("q must be f16[B T, qh 128], qh a multiple of kvh")
+    need = _ctx().lib.lk_hip_kv4_attention_workspace_bytes(b, rows // b, width // HD, kvh, row // ROW)
+    out = _empty((rows, width))
+    work = _empty((-(-need // 4),), _F32)
+    _call("attention_kv4_f16_gpu", [qt, kt, pt, out, work])
+    return Tensor(out)
 
 
 def kv4_reorder_gpu(kv, parents, n):
     """Beam search: rows 0 .. n - 1 of sequence b of kv u8[L, B, 2, kvh, 72 P] become those of sequence parents[b], in
     place (parents i64[B], n i64[1]; B <= 32, L kvh <= 32767). A parent out of range gives NaN rows and a device error."""
-    _on_gpu(kv, parents, n)
-    kv4_capacity(kv)
-    check(kv.ndim == 5 and kv.shape[2] == 2 and 0 < kv.shape[1] <= 32 and kv.shape[0] > 0 and kv.shape[3] > 0,
-          "kv must be u8[L, B, 2, kvh, 72 P] with B <= 32")
-    check(kv.shape[0] * kv.shape[3] <= 32767, "L kvh must be at most 32767")
-    check(parents.dtype == i64 and tuple(parents.shape) == (kv.shape[1],), "parents must be i64[B]")
-    check(n.dtype == i64 and tuple(n.shape) == (1,), "n must be i64[1]")
-    return _launch("kv4_reorder_gpu", [kv, parents, n], [], outs=[], inout=[0])
+    kt, pt, nt = _arg(kv, _U8, 5, "kv"), _arg(parents, _I64, 1, "parents"), _arg(n, _I64, 1, "n")
+    layers, b, two, kvh, row = kt.shape
+    if two != 2 or not 0 < b <= 32 or layers <= 0 or kvh <= 0 or row <= 0 or row % (32 * ROW):
+        raise OpError("kv must be u8[L, B, 2, kvh, 72 P] with B <= 32, P a multiple of 32")
+    if layers * kvh > 32767:
+        raise OpError("L kvh must be at most 32767")
+    if pt.shape[0] != b or nt.shape[0] != 1:
+        raise OpError("parents must be i64[B], n i64[1]")
+    _call("kv4_reorder_gpu", [kt, pt, nt])
 
 
 __all__ = [n for n in dir() if n.endswith(("_f16_gpu", "_reorder_gpu"))] + ["pack_w4", "PackedWeight4", "kv4_cache",

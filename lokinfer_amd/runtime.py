@@ -7,7 +7,7 @@ as LokinferError, the binding-level exception the reference raises from Status (
 """
 from __future__ import annotations
 
-import ctypes as C
+from array import array
 
 import torch
 
@@ -106,13 +106,13 @@ class GpuContext:
 
     def run(self, name: str, ptrs, ints, floats) -> None:
         L = self.lib
-        n_p, n_i, n_f = len(ptrs), len(ints), len(floats)
-        pa = (C.c_void_p * max(1, n_p))(*ptrs)
-        ia = (C.c_int64 * max(1, n_i))(*ints)
-        fa = (C.c_double * max(1, n_f))(*floats)
-        stream = torch.cuda.current_stream(self.device).cuda_stream
-        ws = self.workspace_for(self.slot)
-        rc = L.lk_run_kernel(self.handle(name), pa, n_p, ia, n_i, fa, n_f, ws.data_ptr(), ws.numel() * 4, stream)
+        pa, ia, fa = array("Q", ptrs), array("q", ints), array("d", floats)
+        ws = self._ws_by_slot.get(self.slot)
+        if ws is None:
+            ws = self.workspace_for(self.slot)
+        rc = L.lk_run_kernel(self._handles.get(name) or self.handle(name), pa.buffer_info()[0], len(pa),
+                             ia.buffer_info()[0], len(ia), fa.buffer_info()[0], len(fa), ws.data_ptr(), WORKSPACE_BYTES,
+                             torch._C._cuda_getCurrentRawStream(self.device.index))
         if rc != 0:
             raise LokinferError(L.lk_last_error().decode())
 
