@@ -1,7 +1,7 @@
 // Key / value caches held in 4 bits (lk.ops.q4_gpu; no counterpart in the reference, whose caches are f16 or f32).
 //
 // A cache is u8 [B, 2, kvh, 72 P] (B sequences; keys, values; P rows, a multiple of 32): per (sequence, key or value, kv
-// head) P rows of 64 bytes of codes, then P rows of 4 f16 scales, one for each 32 of the head's 128 values (format: q4.h).
+// head) P rows of 64 bytes of codes, then the scales, f16 [4, P], one for each 32 of the head's 128 values (format: q4.h).
 // A row whose key or value is not finite is held with NaN key scales and a zero value: a query that sees it gets NaN, one
 // that it is masked from is not touched by it.
 //
@@ -49,7 +49,7 @@ __device__ __forceinline__ void kv4PutRow(half4 x, char* kvBlock, int64_t valueO
   word |= __shfl_xor(word, 1, 64);
   char* at = kvBlock + (lane < 32 ? 0 : valueOff);
   if ((l & 1) == 0) *reinterpret_cast<unsigned*>(at + row * 64 + 2 * l) = word;
-  if ((l & 7) == 0) *reinterpret_cast<h16*>(at + cap * 64 + row * 8 + l / 4) = static_cast<h16>(s);
+  if ((l & 7) == 0) *reinterpret_cast<h16*>(at + cap * 64 + (l >> 3) * 2 * cap + 2 * row) = static_cast<h16>(s);
 }
 
 __global__ __launch_bounds__(256) void kv4WriteKernel(char* __restrict__ kv, const h16* __restrict__ k,
@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void kv4ReadKernel(const char* __restrict__ kv
     const int w = static_cast<int>(id & 15);
     const char* at = kv + blk * 72 * cap;
     const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(at + row * 64 + 4 * w));
-    const h16 s = *reinterpret_cast<const h16*>(at + cap * 64 + row * 8 + 2 * (w >> 2));
+    const h16 s = *reinterpret_cast<const h16*>(at + cap * 64 + (w >> 2) * 2 * cap + 2 * row);
     half8 y;
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = v[e] * s;
@@ -144,22 +144,31 @@ struct Kv4Params {
   const char* kv;
   const int64_t* pos;
   h16* out;
-  float* part;  // [splits, B T qh, 130]: (max, sum, out[128]) of each key range
+  float* part;  // [B T qh, splits, 130]: (max, sum, out[128]) of each workgroup's keys
   int64_t b, t, cap;
   int qh, kvh, splits;
   float scale;  // log2(e) / sqrt(128)
   unsigned long long* err;
 };
 
-// Rows of a kv head: r = i group + h, query i's q heads side by side; R of them per wave. Lane (key = lane / 4, g = lane % 4)
-// holds the 32 dims of scale group g: a load instruction reads 16 whole rows. Keys 16 u + lane / 4 of the wave's 64-key
-// chunks are one lane quad's own: it keeps their running max, sum and weighted values by itself, joined at the end.
-template <int R>
-__global__ __launch_bounds__(64) void kv4ChunkKernel(Kv4Params p) {
-  __shared__ float red[R][64][33];
-  const int lane = threadIdx.x, g = lane & 3, kl = lane >> 2;
+// Up to 16 rows a kv head per workgroup of 8 waves: row r = i group + h (query i's q heads side by side). A wave takes 64 keys
+// at a time, four tiles of 16, on 16x16x32 MFMAs:
+// S = K Q^T: lane (key l % 16, kq = l / 16) loads 16 bytes of its key's row, the codes of scale group kq; its word w, scaled
+// (exact in f16), is the A operand of step w, dims 32 kq + 8 w .., the B operand row l % 16's same dims. Its accumulators are
+// then row l % 16's scores of keys 4 kq + 0 .. 3, on which the softmax runs in f32 (log2 units).
+// O^T = V^T P^T over two tiles: the lane's own 8 weights are the B operand as they are, as two f16 parts (hi, and lo = p -
+// hi, so that p keeps some 22 bits). The A operand is 8 keys of one dim: lane (db = l % 16, kq) loads those keys' words
+// db, dims 8 db .. 8 db + 7; the low halves of two keys' words put side by side hold the even dims' codes as pairs, the high
+// halves the odd ones', so each dim's operand is masked out of them as a row's codes are out of a word.
+// Chunks are dealt over the waves of all of a head's workgroups (grid y: splits); the waves' sums meet in LDS.
+// Keys from the longest row's end on have their weight and their value's scale set to zero, whatever the memory holds there.
+constexpr int KW = 8;
+__global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
+  __shared__ __attribute__((aligned(16))) float os[KW][16][KHD + 4];
+  __shared__ float ms[KW][16], ls[KW][16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 15, kq = lane >> 4;
   const int group = p.qh / p.kvh;
-  const int64_t rowsHead = p.t * group, blocksHead = (rowsHead + R - 1) / R;
+  const int64_t rowsHead = p.t * group, blocksHead = (rowsHead + 15) / 16;
   int64_t id = blockIdx.x;
   const int64_t rb = id % blocksHead;
   id /= blocksHead;
@@ -167,150 +176,252 @@ __global__ __launch_bounds__(64) void kv4ChunkKernel(Kv4Params p) {
   const int64_t seq = id / p.kvh;
   const int split = blockIdx.y;
   const int64_t p0 = p.pos[seq];
-  const bool bad = p0 < 0 || p0 + p.t > p.cap;
-  int64_t nkRow[R];
-  int64_t nk = 0;
-  float qf[R][32];
+  const int64_t row = rb * 16 + lc, rowIn = min<int64_t>(row, rowsHead - 1), qi = rowIn / group;
+  const int64_t qAt = (seq * p.t + qi) * p.qh + kvHead * group + (rowIn - qi * group);  // of q and out, in heads
+  half8 qf[4];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int64_t row = min<int64_t>(rb * R + r, rowsHead - 1), i = row / group, h = kvHead * group + (row - i * group);
-    nkRow[r] = p0 < 0 ? 0 : min<int64_t>(p0 + i + 1, p.cap);
-    nk = max(nk, nkRow[r]);
-    const h16* q = p.q + (seq * p.t + i) * p.qh * KHD + h * KHD + 32 * g;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const half8 v = ld8(q + 8 * c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) qf[r][8 * c + e] = static_cast<float>(v[e]);
-    }
-  }
-  if (bad && split == 0 && rb == 0 && kvHead == 0 && lane == 0) raiseDeviceError(p.err, LK_DEVERR_POSITION, p0 < 0 ? p0 : p0 + p.t - 1);
-  const int64_t chunks = (nk + 63) / 64, per = (chunks + p.splits - 1) / p.splits;
-  const int64_t c0 = split * per, c1 = min(c0 + per, chunks);
+  for (int w = 0; w < 4; ++w) qf[w] = ld8(p.q + qAt * KHD + 32 * kq + 8 * w);
+  const int cap = static_cast<int>(p.cap);
+  // rows of the cache that the lane's row, and the block's last and first row, see
+  const auto sees = [&](int64_t i) { return p0 < 0 ? 0 : static_cast<int>(min<int64_t>(p0 + i + 1, p.cap)); };
+  const int nkRow = sees(qi), nk = sees(min<int64_t>(rb * 16 + 15, rowsHead - 1) / group), nkAll = sees(rb * 16 / group);
+  if (split == 0 && rb == 0 && kvHead == 0 && threadIdx.x == 0 && (p0 < 0 || p0 + p.t > p.cap))
+    raiseDeviceError(p.err, LK_DEVERR_POSITION, p0 < 0 ? p0 : p0 + p.t - 1);
   const int64_t block = 72 * p.cap;
   const char* kb = p.kv + (seq * 2 * p.kvh + kvHead) * block;
   const char* vb = kb + p.kvh * block;
-  float m[R], l[R], acc[R][32];
+  const h16* ksc = reinterpret_cast<const h16*>(kb + 64 * p.cap) + kq * p.cap;
+  const h16* vsc = reinterpret_cast<const h16*>(vb + 64 * p.cap) + (lc >> 2) * p.cap;
+  const int chunks = (nk + 63) / 64, step = p.splits * KW;
+  f32x4 acc[8];
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < 32; ++d) acc[r][d] = 0.0f;
-  }
-  for (int64_t c = c0; c < c1; ++c) {
+  for (int e = 0; e < 8; ++e) acc[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  // m: the running maximum times the scale, rounded once and taken off everywhere as it is
+  float m = -INFINITY, l = 0.0f;
+  struct Chunk {
+    uint4 k[4];
+    h16 ks[4];
+    unsigned v[4][4];
+    half4 vs[4];
+  };
+  const auto load = [&](int c) {
+    Chunk x;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t key = c * 64 + 16 * u + kl, at = min(key, nk - 1);
-      const uint4 kw = *reinterpret_cast<const uint4*>(kb + at * 64 + 16 * g);
-      const uint4 vw = *reinterpret_cast<const uint4*>(vb + at * 64 + 16 * g);
-      const float ks = static_cast<float>(*reinterpret_cast<const h16*>(kb + p.cap * 64 + at * 8 + 2 * g));
-      const float vs = static_cast<float>(*reinterpret_cast<const h16*>(vb + p.cap * 64 + at * 8 + 2 * g));
-      const unsigned kws[4] = {kw.x, kw.y, kw.z, kw.w}, vws[4] = {vw.x, vw.y, vw.z, vw.w};
-      float dot[R];
+      const int64_t at = min(c * 64 + 16 * u + lc, nk - 1);
+      x.k[u] = *reinterpret_cast<const uint4*>(kb + at * 64 + 16 * kq);
+      x.ks[u] = ksc[at];
+    }
 #pragma unroll
-      for (int r = 0; r < R; ++r) dot[r] = 0.0f;
+    for (int u = 0; u < 4; ++u) {
+      const int64_t at = min(c * 64 + 16 * u + 4 * kq, cap - 4);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const half8 x = q4Ints(kws[w]);
+      for (int r = 0; r < 4; ++r) x.v[u][r] = *reinterpret_cast<const unsigned*>(vb + (at + r) * 64 + 4 * lc);
+      x.vs[u] = *reinterpret_cast<const half4*>(vsc + at);
+    }
+    return x;
+  };
+  const auto compute = [&](int c, Chunk& x) {
+    f32x4 s[4];
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+    for (int u = 0; u < 4; ++u) {
+      const unsigned w4[4] = {x.k[u].x, x.k[u].y, x.k[u].z, x.k[u].w};
+      const h16 f = x.ks[u];
+      s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dot[r] = fmaf(static_cast<float>(x[e]), qf[r][8 * w + e], dot[r]);
+      for (int w = 0; w < 4; ++w)
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4Ints(w4[w]) * half8{f, f, f, f, f, f, f, f}, qf[w], s[u], 0, 0, 0);
+    }
+    if (c * 64 + 64 > nkAll) {  // keys past some row's
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = c * 64 + 16 * u + 4 * kq + r;
+          if (key >= nkRow) s[u][r] = -INFINITY;
+          if (key >= nk) x.vs[u][r] = static_cast<h16>(0.0f);
+        }
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][r]);
+    mx = crossRowMax(mx) * p.scale;
+    if (__any(mx > m)) {  // some row's maximum grew
+      const float to = fmaxf(m, mx), corr = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
+      l *= corr;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] *= corr;
+      m = to;
+    }
+    const float base = m == -INFINITY ? 0.0f : m;  // no key so far: every weight 0 (or a NaN kept)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], p.scale, -base));
+        l += s[u][r];
       }
-      float wgt[R];
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float d = dot[r] * ks;
-        d += __shfl_xor(d, 1, 64);
-        d += __shfl_xor(d, 2, 64);
-        const float s = key < nkRow[r] ? d * p.scale : -INFINITY;
-        const float mx = fmaxf(m[r], s);
-        const float base = mx == -INFINITY ? 0.0f : mx;
-        const float corr = __builtin_amdgcn_exp2f(m[r] - base);
-        const float e = __builtin_amdgcn_exp2f(s - base);
-        l[r] = l[r] * corr + e;
-        m[r] = mx;
-        wgt[r] = e * vs;
-        if (__any(corr != 1.0f)) {
+    for (int t = 0; t < 2; ++t) {  // keys 32 t ..: tiles 2 t, 2 t + 1
+      half8 ph, pl;
 #pragma unroll
-          for (int d2 = 0; d2 < 32; ++d2) acc[r][d2] *= corr;
+      for (int j = 0; j < 8; ++j) {
+        const float v = s[2 * t + (j >> 2)][j & 3];
+        ph[j] = static_cast<h16>(v);
+        pl[j] = static_cast<h16>(v - static_cast<float>(ph[j]));
+      }
+      unsigned even[4], odd[4];
+      half2v sc[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // keys 2 j, 2 j + 1 of the lane's 8
+        const unsigned a = x.v[2 * t + (j >> 1)][2 * (j & 1)], b = x.v[2 * t + (j >> 1)][2 * (j & 1) + 1];
+        even[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        odd[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        sc[j] = half2v{x.vs[2 * t + (j >> 1)][2 * (j & 1)], x.vs[2 * t + (j >> 1)][2 * (j & 1) + 1]};
+      }
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        half2v dims[4][4];  // [dim 2 i + o][pair of keys]
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const half8 v = q4Ints(o ? odd[j] : even[j]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dims[i][j] = half2v{v[2 * i], v[2 * i + 1]} * sc[j];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const half8 a{dims[i][0][0], dims[i][0][1], dims[i][1][0], dims[i][1][1],
+                        dims[i][2][0], dims[i][2][1], dims[i][3][0], dims[i][3][1]};
+          acc[2 * i + o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, acc[2 * i + o], 0, 0, 0);
+          acc[2 * i + o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, acc[2 * i + o], 0, 0, 0);
         }
       }
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const half8 x = q4Ints(vws[w]);
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[r][8 * w + e] = fmaf(static_cast<float>(x[e]), wgt[r], acc[r][8 * w + e]);
-      }
     }
+  };
+  int c = split * KW + wave;
+  if (c < chunks) {
+    Chunk cur = load(c);
+    for (; c + step < chunks; c += step) {
+      const Chunk next = load(c + step);
+      compute(c, cur);
+      cur = next;
+    }
+    compute(c, cur);
   }
-  // join the 16 lane quads
-  float mAll[R], lAll[R];
+  // accumulator r of dim e: dim 8 (4 kq + r) + e of row l % 16
+  l = crossRowSum(l);
+  const int rows = static_cast<int>(min<int64_t>(rowsHead - rb * 16, 16));
+  if (lc < rows) {
+    if (kq == 0) {
+      ms[wave][lc] = m;
+      ls[wave][lc] = l;
+    }
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    float mm = m[r];
-#pragma unroll
-    for (int o = 4; o < 64; o <<= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
-    mAll[r] = mm;
-    const float f = m[r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[r] - mm);
-    float ll = m[r] == -INFINITY ? l[r] : l[r] * f;  // a NaN score leaves m alone: the NaN is in l
-#pragma unroll
-    for (int o = 4; o < 64; o <<= 1) ll += __shfl_xor(ll, o, 64);
-    lAll[r] = ll;
-#pragma unroll
-    for (int d = 0; d < 32; ++d) red[r][lane][d] = acc[r][d] * f;
+    for (int r = 0; r < 4; ++r) {
+      float* o = &os[wave][lc][8 * (4 * kq + r)];
+      *reinterpret_cast<f32x4*>(o) = f32x4{acc[0][r], acc[1][r], acc[2][r], acc[3][r]};
+      *reinterpret_cast<f32x4*>(o + 4) = f32x4{acc[4][r], acc[5][r], acc[6][r], acc[7][r]};
+    }
   }
   __syncthreads();
+  for (int o = threadIdx.x; o < rows * KHD; o += 64 * KW) {
+    const int r = o / KHD, d = o % KHD;
+    float mm = -INFINITY;
 #pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int64_t row = rb * R + r;
-    if (row >= rowsHead) continue;
-    const int64_t i = row / group, h = kvHead * group + (row - i * group), at = (seq * p.t + i) * p.qh + h;
+    for (int w = 0; w < KW; ++w) mm = fmaxf(mm, ms[w][r]);
+    float ll = 0.0f, y = 0.0f;
 #pragma unroll
-    for (int d0 = 0; d0 < KHD; d0 += 64) {
-      const int d = d0 + lane;
-      float o = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) o += red[r][4 * j + (d >> 5)][d & 31];
-      if (p.splits == 1) {
-        const bool noRow = p0 < 0 || p0 + i >= p.cap;
-        p.out[at * KHD + d] = noRow ? static_cast<h16>(__builtin_nanf("")) : toH16(o / lAll[r]);
-      } else {
-        p.part[(split * p.b * p.t * p.qh + at) * (KHD + 2) + 2 + d] = o;
-      }
+    for (int w = 0; w < KW; ++w) {
+      const float f = ms[w][r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms[w][r] - mm);  // no key: zeros, or a NaN
+      ll = fmaf(f, ls[w][r], ll);
+      y = fmaf(f, os[w][r][d], y);
     }
-    if (p.splits > 1 && lane == 0) {
-      float* pp = p.part + (split * p.b * p.t * p.qh + at) * (KHD + 2);
-      pp[0] = mAll[r];
-      pp[1] = lAll[r];
+    const int64_t i = (rb * 16 + r) / group, at = (seq * p.t + i) * p.qh + kvHead * group + (rb * 16 + r - i * group);
+    if (p.splits == 1) {
+      const bool noRow = p0 < 0 || p0 + i >= p.cap;
+      p.out[at * KHD + d] = noRow ? static_cast<h16>(__builtin_nanf("")) : toH16(y / ll);
+    } else {
+      float* pp = p.part + (at * p.splits + split) * (KHD + 2);
+      pp[2 + d] = y;
+      if (d == 0) {
+        pp[0] = mm;
+        pp[1] = ll;
+      }
     }
   }
 }
 
-// one workgroup per (query, q head)
+// one workgroup per (query, q head): the splits' partials, 32 at a time
 __global__ __launch_bounds__(128) void kv4MergeKernel(Kv4Params p) {
   const int d = threadIdx.x;
-  const int64_t at = blockIdx.x, rows = p.b * p.t * p.qh, qi = at / p.qh, seq = qi / p.t, p0 = p.pos[seq] + (qi - seq * p.t);
-  const bool noRow = p.pos[seq] < 0 || p0 >= p.cap;
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, p.part[(s * rows + at) * (KHD + 2)]);
-  float l = 0.0f, o = 0.0f;
-  for (int s = 0; s < p.splits; ++s) {
-    const float* pp = p.part + (s * rows + at) * (KHD + 2);
-    const float f = pp[0] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(pp[0] - m);  // no key: zeros, or a NaN to pass on
-    l = fmaf(f, pp[1], l);
-    o = fmaf(f, pp[2 + d], o);
+  const int64_t at = blockIdx.x, qi = at / p.qh, seq = qi / p.t, p0 = p.pos[seq];
+  const bool noRow = p0 < 0 || p0 + (qi - seq * p.t) >= p.cap;
+  const float* part = p.part + at * p.splits * (KHD + 2);
+  float m = -INFINITY, l = 0.0f, o = 0.0f;
+  for (int s0 = 0; s0 < p.splits; s0 += 32) {
+    float mc[32], lc[32], oc[32], mb = m;
+#pragma unroll
+    for (int s = 0; s < 32; ++s) {
+      const bool in = s0 + s < p.splits;
+      const float* pp = part + (in ? s0 + s : 0) * (KHD + 2);
+      mc[s] = in ? pp[0] : -INFINITY;
+      lc[s] = in ? pp[1] : 0.0f;
+      oc[s] = in ? pp[2 + d] : 0.0f;
+    }
+#pragma unroll
+    for (int s = 0; s < 32; ++s) mb = fmaxf(mb, mc[s]);
+    const float corr = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mb);
+    l *= corr;
+    o *= corr;
+#pragma unroll
+    for (int s = 0; s < 32; ++s) {
+      const float f = mc[s] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(mc[s] - mb);  // no key: zeros, or a NaN
+      l = fmaf(f, lc[s], l);
+      o = fmaf(f, oc[s], o);
+    }
+    m = mb;
   }
   p.out[at * KHD + d] = noRow ? static_cast<h16>(__builtin_nanf("")) : toH16(o / l);
 }
 
+// Many rows: the rows 0 .. pos + T - 1 of one sequence as f16 [P, kvh 128], keys then values, for the f16 tiles of
+// lk_hip_f16_attention_gqa: they are dequantised once instead of by every block of queries. 8 values per thread.
+__global__ __launch_bounds__(256) void kv4ExpandKernel(const char* __restrict__ kv, const int64_t* __restrict__ pos,
+                                                       h16* __restrict__ out, int64_t t, int kvh, int64_t cap) {
+  const int64_t p0 = *pos, rows = p0 < 0 ? 0 : min<int64_t>(p0 + t, cap), per = static_cast<int64_t>(kvh) * 16;
+  const char* base = kv + blockIdx.y * kvh * 72 * cap;
+  h16* o = out + blockIdx.y * cap * kvh * KHD;
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < rows * per;
+       id += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t row = id / per;
+    const int at = static_cast<int>(id - row * per), w = at & 15;
+    const char* blk = base + (at >> 4) * 72 * cap;
+    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(blk + row * 64 + 4 * w));
+    const h16 s = *reinterpret_cast<const h16*>(blk + cap * 64 + (w >> 2) * 2 * cap + 2 * row);
+    st8(o + id * 8, v * half8{s, s, s, s, s, s, s, s});
+  }
+}
+
 // ---- moving caches between sequences ------------------------------------------------------------------------------
-// One thread per 8 bytes of a (layer, key or value, kv head)'s live rows: it reads the piece of every sequence whose parent
-// is another from that parent, then writes them, so that no write comes before a read of the same bytes.
+// One thread per 8 bytes of codes, or 2 of scales, of a (layer, key or value, kv head)'s live rows: it reads the piece of
+// every sequence from that sequence's parent, then writes them, so that no write comes before a read of the same bytes.
 constexpr int kMaxBeams = 32;
+template <typename T>
+__device__ __forceinline__ void kv4Move(char* at, int64_t seqStride, const int64_t* parents, int b, T none) {
+  T v[kMaxBeams];
+#pragma unroll
+  for (int i = 0; i < kMaxBeams; ++i)
+    if (i < b) {
+      const int64_t from = parents[i];
+      v[i] = from >= 0 && from < b ? *reinterpret_cast<const T*>(at + from * seqStride) : none;
+    }
+#pragma unroll
+  for (int i = 0; i < kMaxBeams; ++i)
+    if (i < b && parents[i] != i) *reinterpret_cast<T*>(at + i * seqStride) = v[i];
+}
+
 __global__ __launch_bounds__(256) void kv4ReorderKernel(char* __restrict__ kv, const int64_t* __restrict__ parents,
                                                         const int64_t* __restrict__ n, int64_t layers, int b, int kvh,
                                                         int64_t cap, unsigned long long* err) {
@@ -322,20 +433,14 @@ __global__ __launch_bounds__(256) void kv4ReorderKernel(char* __restrict__ kv, c
     for (int i = 0; i < b; ++i)
       if (parents[i] < 0 || parents[i] >= b) raiseDeviceError(err, LK_DEVERR_INDEX, parents[i]);
   }
-  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < rows * 9;
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < rows * 12;
        id += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t off = id < rows * 8 ? id * 8 : cap * 64 + (id - rows * 8) * 8;
-    unsigned long long v[kMaxBeams];
-#pragma unroll
-    for (int i = 0; i < kMaxBeams; ++i)
-      if (i < b) {
-        const int64_t from = parents[i];
-        v[i] = from >= 0 && from < b ? *reinterpret_cast<const unsigned long long*>(base + from * seqStride + off)
-                                     : 0x7E007E007E007E00ull;  // NaN where it lands in the scales
-      }
-#pragma unroll
-    for (int i = 0; i < kMaxBeams; ++i)
-      if (i < b && parents[i] != i) *reinterpret_cast<unsigned long long*>(base + i * seqStride + off) = v[i];
+    if (id < rows * 8) {
+      kv4Move<unsigned long long>(base + id * 8, seqStride, parents, b, 0ull);
+    } else {
+      const int64_t j = id - rows * 8, g = j / rows;
+      kv4Move<unsigned short>(base + 64 * cap + g * 2 * cap + 2 * (j - g * rows), seqStride, parents, b, 0x7E00);  // NaN
+    }
   }
 }
 
@@ -348,6 +453,17 @@ bool al8(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 7) == 0; }
 int launched() { return hipGetLastError() == hipSuccess ? 0 : 2; }
 bool kvOk(const void* kv, int64_t b, int kvh, int64_t cap) {
   return b > 0 && kvh > 0 && cap > 0 && cap % 32 == 0 && al16(kv);
+}
+
+// Many rows: expanded to f16 once
+bool kv4Expands(int64_t t, int64_t group) { return t > 1 && t * group > 32; }
+
+int kv4Splits(int64_t b, int64_t t, int qh, int kvh, int64_t cap) {
+  const int64_t groups = b * kvh * ((t * (qh / kvh) + 15) / 16);
+  const char* f = getenv("LKSP");
+  if (f) return atoi(f);
+  if (cap <= 2048 || groups >= 256) return 1;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((cap + 511) / 512, 512 / groups)));
 }
 
 }  // namespace
@@ -392,14 +508,9 @@ int lk_hip_kv4_read(const void* kv, void* out, int64_t blocks, int64_t cap, void
   return launched();
 }
 
-static int kv4Splits(int64_t b, int64_t t, int qh, int kvh, int64_t cap) {
-  if (b <= 0 || t <= 0 || qh <= 0 || kvh <= 0 || qh % kvh != 0 || cap <= 0) return 1;
-  const int64_t waves = b * kvh * ((t * (qh / kvh) + 1) / 2);
-  const int64_t most = std::max<int64_t>(1, (cap + 63) / 64);
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({most, 128, 2048 / std::max<int64_t>(waves, 1)})));
-}
-
 int64_t lk_hip_kv4_attention_workspace_bytes(int64_t b, int64_t t, int qh, int kvh, int64_t cap) {
+  if (b <= 0 || t <= 0 || qh <= 0 || kvh <= 0 || qh % kvh != 0 || cap <= 0) return 0;
+  if (kv4Expands(t, qh / kvh)) return 2 * cap * kvh * lkd::KHD * 2;
   const int64_t s = kv4Splits(b, t, qh, kvh, cap);
   return s > 1 ? s * b * t * qh * (lkd::KHD + 2) * 4 : 0;
 }
@@ -409,15 +520,29 @@ int lk_hip_kv4_attention(const void* q, const void* kv, const int64_t* pos, void
   using namespace lkd;
   if (!kvOk(kv, b, kvh, cap) || t < 0 || qh <= 0 || qh % kvh != 0 || !al16(q)) return 1;
   if (t == 0) return 0;
+  const int64_t need = lk_hip_kv4_attention_workspace_bytes(b, t, qh, kvh, cap);
+  if (need > 0 && (!workspace || workspace_bytes < need || !al16(workspace))) return 3;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (kv4Expands(t, qh / kvh)) {
+    h16* rows = static_cast<h16*>(workspace);
+    const unsigned gx = static_cast<unsigned>(std::min<int64_t>((cap * kvh * 16 + 255) / 256, 2048));
+    for (int64_t i = 0; i < b; ++i) {  // one sequence after the other through the same rows
+      hipLaunchKernelGGL(kv4ExpandKernel, dim3(gx, 2), dim3(256), 0, s,
+                         static_cast<const char*>(kv) + i * 2 * kvh * 72 * cap, pos + i, rows, t, kvh, cap);
+      const int rc = lk_hip_f16_attention_gqa(static_cast<const h16*>(q) + i * t * qh * KHD, rows, rows + cap * kvh * KHD,
+                                              pos + i, static_cast<h16*>(out) + i * t * qh * KHD, t, qh, kvh, cap, nullptr, 0,
+                                              stream);
+      if (rc) return rc;
+    }
+    return launched();
+  }
   const int splits = kv4Splits(b, t, qh, kvh, cap);
-  if (workspace_bytes < lk_hip_kv4_attention_workspace_bytes(b, t, qh, kvh, cap) || (splits > 1 && !workspace)) return 3;
   const Kv4Params p{static_cast<const h16*>(q), static_cast<const char*>(kv), pos, static_cast<h16*>(out),
                     static_cast<float*>(workspace), b, t, cap, qh, kvh, splits,
                     kLog2e / std::sqrt(static_cast<float>(KHD)), lkh::deviceErrorRecord()};
-  hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t blocks = b * kvh * ((t * (qh / kvh) + 1) / 2);
-  if (blocks > 0x7FFFFFFF || b * t * qh > 0x7FFFFFFF) return 1;
-  hipLaunchKernelGGL(kv4ChunkKernel<2>, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(splits)), dim3(64), 0, s, p);
+  const int64_t blocks = b * kvh * ((t * (qh / kvh) + 15) / 16);
+  if (blocks > 0x7FFFFFFF || b * t * qh > 0x7FFFFFFF || cap > 0x7FFFFFFF - 64) return 1;
+  hipLaunchKernelGGL(kv4DecodeKernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(splits)), dim3(64 * KW), 0, s, p);
   if (splits > 1)
     hipLaunchKernelGGL(kv4MergeKernel, dim3(static_cast<unsigned>(b * t * qh)), dim3(128), 0, s, p);
   return launched();

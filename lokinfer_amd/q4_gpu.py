@@ -28,6 +28,7 @@ GROUPS = (32, 64, 128)
 ROW = 72  # bytes of a cache row: 64 of codes, 4 f16 scales
 HD = 128
 
+_NO_WORK = torch.empty(0, dtype=torch.float32)
 _F16, _F32, _I32, _I64, _U8 = torch.float16, torch.float32, torch.int32, torch.int64, torch.uint8
 
 
@@ -310,8 +311,7 @@ def attention_kv4_f16_gpu(q, kv, pos):
         raise OpError("q must be f16[B T, qh 128], qh a multiple of kvh")
     need = _ctx().lib.lk_hip_kv4_attention_workspace_bytes(b, rows // b, width // HD, kvh, row // ROW)
     out = _empty((rows, width))
-    work = _empty((-(-need // 4),), _F32)
-    _call("attention_kv4_f16_gpu", [qt, kt, pt, out, work])
+    _call("attention_kv4_f16_gpu", [qt, kt, pt, out, _empty((-(-need // 4),), _F32) if need else _NO_WORK])
     return Tensor(out)
 
 

@@ -212,7 +212,7 @@ def test_cache_rows_are_exact_and_the_others_stay(gpu, b, t, kvh, cap, pos):
             assert np.array_equal(read[s, 0, :, row], key[s * t + i]) and np.array_equal(read[s, 1, :, row], val[s * t + i])
     for s in range(b):  # rows that the call does not name keep every byte
         codes = lambda x: x[s, :, :, : 64 * cap].reshape(2, kvh, cap, 64)[:, :, ~touched[s]]  # noqa: E731
-        scales = lambda x: x[s, :, :, 64 * cap:].reshape(2, kvh, cap, 8)[:, :, ~touched[s]]   # noqa: E731
+        scales = lambda x: x[s, :, :, 64 * cap:].reshape(2, kvh, 4, cap, 2)[:, :, :, ~touched[s]]   # noqa: E731
         assert np.array_equal(codes(before), codes(after)) and np.array_equal(scales(before), scales(after))
 
 
@@ -342,7 +342,9 @@ def test_reorder(gpu, parents, n):
     q4.kv4_reorder_gpu(kv, I(lk, *parents), I(lk, n))
     want = was.copy()
     want[..., : n * 64] = was[:, parents, ..., : n * 64]
-    want[..., 64 * 64: 64 * 64 + n * 8] = was[:, parents, ..., 64 * 64: 64 * 64 + n * 8]
+    for g in range(4):
+        at = slice(64 * 64 + g * 2 * 64, 64 * 64 + g * 2 * 64 + 2 * n)
+        want[..., at] = was[:, parents, ..., at]
     assert np.array_equal(kv.t.cpu().numpy(), want)
 
 
