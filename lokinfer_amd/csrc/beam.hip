@@ -5,10 +5,13 @@
 // The k best of all B V, ties to the lowest b V + t. What has no value (a NaN, a row without a finite log-sum, a beam whose
 // score is not finite) counts as -inf.
 //
-// Three launches: beamScanKernel, one pass over the logits: each wave takes 1024 of a row, keeps them in registers, and
-// leaves their maximum, sum of exponentials and k best; beamRowKernel joins a row's; beamPickKernel takes the k best
-// of the beams' lists. Within a row the order is that of the logits (exact); between beams that of the candidates in
-// 64 bits, the sum of exponentials added in 64 bits over the waves' 32-bit sums.
+// Two launches. beamScanKernel passes once over the logits: each wave keeps 1024 of a row in registers and takes their k
+// best one after the other (a maximum over the wave of (order of the logit, index) keys by DPP moves), a workgroup
+// joins its four waves' lists by counting for each entry the better ones, and leaves one list, the maximum and the sum of
+// exponentials of its 4096 logits. beamPickKernel, one workgroup, joins a row's lists with one wave (lane i at the head
+// of list i), adds up its log-sum, and takes the k best of the rows' heads. Within a row the order is that of the logits
+// (exact); between beams that of the candidates in 64 bits, the sums of exponentials of 4096 logits each (32 bits) added
+// in 64 bits.
 #include <algorithm>
 
 #include "common.h"
@@ -17,23 +20,21 @@
 namespace lkd {
 
 constexpr int kBeamMost = 32;    // beams and k
-constexpr int kBeamWave = 1024;  // logits per wave
-constexpr int kBeamLists = 256;  // waves per row
+constexpr int kBeamTile = 4096;  // logits per workgroup of 4 waves
+constexpr int kBeamLists = 64;   // lists per row at most: V <= 262144
 
 struct BeamParams {
   const float* logits;   // [B, V]
   const float* scores;   // [B]
   const int64_t* done;   // [B]
-  float* sums;           // [B, waves, 2]: max, sum
-  uint2* lists;          // [B, waves, k]: (order of the logit, index), best first
-  double* cand;          // [B, k]
-  int* tok;              // [B, k]
+  float2* sums;          // [B, tiles]: max, sum
+  uint2* lists;          // [B, tiles, k]: (order of the logit, index), best first
   float* outScores;      // [k]
   int64_t* outParents;
   int64_t* outTokens;
   int64_t* outDone;
   int64_t v;
-  int b, k, waves;
+  int b, k, tiles;
   int eos[4];
 };
 
@@ -47,84 +48,100 @@ __device__ __forceinline__ float valueOf(unsigned key) {
   return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
 }
 
-// the wave's best (key, index): the larger key, then the smaller index
-__device__ __forceinline__ void waveBest(unsigned& key, unsigned& idx) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const unsigned k2 = __shfl_xor(key, o, 64), i2 = __shfl_xor(idx, o, 64);
-    if (k2 > key || (k2 == key && i2 < idx)) {
-      key = k2;
-      idx = i2;
-    }
-  }
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 pairOf(unsigned hi, unsigned lo) { return (static_cast<u64>(hi) << 32) | lo; }
+
+// the wave's largest value, in every lane
+template <int CTRL>
+__device__ __forceinline__ u64 maxDpp(u64 v) {
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<unsigned>(v >> 32), CTRL, 0xF, 0xF, false);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<unsigned>(v), CTRL, 0xF, 0xF, false);
+  return max(v, pairOf(hi, lo));
+}
+__device__ __forceinline__ u64 waveMaxU64(u64 v) {
+  v = maxDpp<0xB1>(v);   // quad_perm [1, 0, 3, 2]
+  v = maxDpp<0x4E>(v);   // quad_perm [2, 3, 0, 1]
+  v = maxDpp<0x141>(v);  // row_half_mirror
+  v = maxDpp<0x140>(v);  // row_mirror
+  const auto h = __builtin_amdgcn_permlane16_swap(static_cast<unsigned>(v >> 32), static_cast<unsigned>(v >> 32), false, false);
+  const auto l = __builtin_amdgcn_permlane16_swap(static_cast<unsigned>(v), static_cast<unsigned>(v), false, false);
+  v = max(pairOf(h[0], l[0]), pairOf(h[1], l[1]));
+  const auto h2 = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(v >> 32), static_cast<unsigned>(v >> 32), false, false);
+  const auto l2 = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(v), static_cast<unsigned>(v), false, false);
+  return max(pairOf(h2[0], l2[0]), pairOf(h2[1], l2[1]));
 }
 
 __global__ __launch_bounds__(256) void beamScanKernel(BeamParams p) {
-  const int lane = threadIdx.x & 63, w = blockIdx.x * 4 + (threadIdx.x >> 6), beam = blockIdx.y;
-  if (w >= p.waves) return;
+  __shared__ u64 best[4][kBeamMost];
+  __shared__ float2 part[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = blockIdx.x, beam = blockIdx.y;
   const float* x = p.logits + static_cast<int64_t>(beam) * p.v;
-  const int64_t first = static_cast<int64_t>(w) * kBeamWave;
-  constexpr int E = kBeamWave / 64;
+  constexpr int E = kBeamTile / 256;
+  const unsigned first = static_cast<unsigned>(tile) * kBeamTile + wave * 64 * E + lane;
   unsigned key[E];
-  float m = -INFINITY;
-  float val[E];
+  float val[E], m = -INFINITY;
+#pragma unroll
+  for (int e = 0; e < E; ++e) val[e] = x[min<int64_t>(first + 64 * e, p.v - 1)];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int64_t i = first + lane + 64 * e;
-    val[e] = i < p.v ? x[i] : -INFINITY;
-    key[e] = i < p.v ? orderOf(val[e]) : 0u;
+    const bool in = first + 64 * e < p.v;
+    if (!in) val[e] = -INFINITY;
+    key[e] = in ? orderOf(val[e]) : 0u;
     m = fmaxf(m, val[e]);
   }
-  m = waveMax(m);
+  m = waveMaxDpp(m);
   float s = 0.0f;
   const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
   for (int e = 0; e < E; ++e) s += expf(val[e] - base);  // a NaN stays one; inf - inf is one
-  s = waveSum(s);
-  const int64_t at = static_cast<int64_t>(beam) * p.waves + w;
-  if (lane == 0) {
-    p.sums[2 * at] = m;
-    p.sums[2 * at + 1] = s;
-  }
+  s = waveSumDpp(s);
+  if (lane == 0) part[wave] = make_float2(m, s);
   for (int j = 0; j < p.k; ++j) {
-    unsigned bk = 0u, be = 0u;
+    unsigned bk = key[0], be = 0u;  // equal keys of one lane: the first has the smallest index
+#pragma unroll
+    for (int e = 1; e < E; ++e) {
+      const bool more = key[e] > bk;
+      bk = more ? key[e] : bk;
+      be = more ? e : be;
+    }
+    const u64 top = waveMaxU64(pairOf(bk, ~(first + 64 * be)));
+    if (lane == 0) best[wave][j] = top;
+    const unsigned at = ~static_cast<unsigned>(top) - first;  // a multiple of 64 below 64 E in the lane that holds it
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      if (key[e] > bk) {
-        bk = key[e];
-        be = e;
-      }
-    unsigned wk = bk, wi = lane + 64 * be;  // equal keys of one lane: the first, its smallest index
-    waveBest(wk, wi);
-    if (lane == 0) p.lists[at * p.k + j] = make_uint2(wk, static_cast<unsigned>(first) + wi);
-    if ((wi & 63) == static_cast<unsigned>(lane)) {
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (static_cast<unsigned>(e) == wi >> 6) key[e] = 0u;
-    }
+      if (at == 64u * e) key[e] = 0u;
+  }
+  __syncthreads();
+  if (threadIdx.x < 4u * p.k) {  // entries without a logit (key 0) are distinct by their index
+    const u64 mine = best[threadIdx.x / p.k][threadIdx.x % p.k];
+    int rank = 0;
+    for (int w = 0; w < 4; ++w)
+      for (int j = 0; j < p.k; ++j) rank += best[w][j] > mine;
+    if (rank < p.k)
+      p.lists[(static_cast<int64_t>(beam) * p.tiles + tile) * p.k + rank] =
+          make_uint2(static_cast<unsigned>(mine >> 32), ~static_cast<unsigned>(mine));
+  }
+  if (threadIdx.x == 0) {
+    float mm = -INFINITY, ss = 0.0f;
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, part[w].x);
+    for (int w = 0; w < 4; ++w)
+      ss += part[w].x == -INFINITY ? (part[w].y == part[w].y ? 0.0f : part[w].y) : part[w].y * expf(part[w].x - mm);
+    p.sums[static_cast<int64_t>(beam) * p.tiles + tile] = make_float2(mm, ss);
   }
 }
 
-// one wave per beam: the row's log-sum, then k times the best head of its lists
-__global__ __launch_bounds__(64) void beamRowKernel(BeamParams p) {
-  extern __shared__ uint2 heads[];  // [waves, k]
-  const int lane = threadIdx.x, beam = blockIdx.x;
-  const int64_t at = static_cast<int64_t>(beam) * p.waves;
-  double* cand = p.cand + static_cast<int64_t>(beam) * p.k;
-  int* tok = p.tok + static_cast<int64_t>(beam) * p.k;
+// Row `beam`'s k candidates, best first, by one wave: the best heads of its lists one after the other.
+__device__ __forceinline__ void beamRow(const BeamParams& p, int beam, uint2* heads, double* cand, int* tok) {
+  const int lane = threadIdx.x & 63;
+  const int64_t at = static_cast<int64_t>(beam) * p.tiles;
   const float score = p.scores[beam];
-  float m = -INFINITY;
-  for (int w = lane; w < p.waves; w += 64) m = fmaxf(m, p.sums[2 * (at + w)]);
-  m = waveMax(m);
-  double sum = 0.0;
-  for (int w = lane; w < p.waves; w += 64) {
-    const float mw = p.sums[2 * (at + w)];
-    const double part = static_cast<double>(p.sums[2 * (at + w) + 1]);
-    sum += mw == -INFINITY ? (part == part ? 0.0 : part) : part * exp(static_cast<double>(mw) - static_cast<double>(m));
-  }
+  const float2 mine = lane < p.tiles ? p.sums[at + lane] : make_float2(-INFINITY, 0.0f);
+  for (int i = lane; i < p.tiles * p.k; i += 64) heads[i] = p.lists[at * p.k + i];
+  const float m = waveMaxDpp(mine.x);
+  double sum = mine.x == -INFINITY ? (mine.y == mine.y ? 0.0 : mine.y)
+                                   : mine.y * exp(static_cast<double>(mine.x) - static_cast<double>(m));
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  const bool done = p.done[beam] != 0;
-  const bool live = fabsf(score) < INFINITY;
+  const bool done = p.done[beam] != 0, live = fabsf(score) < INFINITY;
   if (done || !live || !(sum > 0.0 && fabsf(m) < INFINITY)) {
     // at most the finished beam's eos; else tokens in order, without a value
     const bool one = done && live;
@@ -136,73 +153,62 @@ __global__ __launch_bounds__(64) void beamRowKernel(BeamParams p) {
     return;
   }
   const double lse = static_cast<double>(m) + log(sum);
-  for (int i = lane; i < p.waves * p.k; i += 64) heads[i] = p.lists[at * p.k + i];
-  constexpr int L = kBeamLists / 64;
-  int next[L];
-#pragma unroll
-  for (int i = 0; i < L; ++i) next[i] = 0;
-  __syncthreads();
+  // the wave's own slice of LDS, written above by its other lanes
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  int next = 0;
+  uint2 h = lane < p.tiles ? heads[lane * p.k] : make_uint2(0u, 0u);
   for (int j = 0; j < p.k; ++j) {
-    unsigned bk = 0u, bi = 0xFFFFFFFFu;
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-      const int w = lane + 64 * i;
-      if (w < p.waves && next[i] < p.k) {
-        const uint2 h = heads[w * p.k + next[i]];
-        if (h.x > bk || (h.x == bk && h.x != 0u && h.y < bi)) {
-          bk = h.x;
-          bi = h.y;
-        }
-      }
-    }
-    waveBest(bk, bi);
-    const bool any = bk != 0u;  // fewer than k logits: none left
+    const u64 top = waveMaxU64(pairOf(h.x, ~h.y));
+    const unsigned bk = static_cast<unsigned>(top >> 32), bi = ~static_cast<unsigned>(top);
     if (lane == 0) {
-      const double c = any ? static_cast<double>(score) + (static_cast<double>(valueOf(bk)) - lse) : -INFINITY;
-      cand[j] = c == c ? c : -INFINITY;
-      tok[j] = any ? static_cast<int>(bi) : -1;
+      const double c = static_cast<double>(score) + (static_cast<double>(valueOf(bk)) - lse);
+      cand[j] = bk != 0u && c == c ? c : -INFINITY;
+      tok[j] = bk != 0u ? static_cast<int>(bi) : -1;  // fewer than k logits: none left
     }
-    const int w = static_cast<int>(bi / kBeamWave);
-#pragma unroll
-    for (int i = 0; i < L; ++i)
-      if (any && w == lane + 64 * i) ++next[i];
+    if (bk != 0u && h.x == bk && h.y == bi) {
+      ++next;
+      h = next < p.k ? heads[lane * p.k + next] : make_uint2(0u, 0u);
+    }
   }
 }
 
-// one wave: k times the best head of the beams' lists; lane b holds beam b's
-__global__ __launch_bounds__(64) void beamPickKernel(BeamParams p) {
-  const int lane = threadIdx.x;
+// one workgroup: a wave per row (rows w, w + waves, ...), then the first wave, lane b at the head of row b's candidates
+__global__ __launch_bounds__(1024) void beamPickKernel(BeamParams p) {
+  extern __shared__ uint2 heads[];  // [waves, tiles, k]
+  __shared__ double cand[kBeamMost][kBeamMost];
+  __shared__ int tok[kBeamMost][kBeamMost];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int beam = wave; beam < p.b; beam += blockDim.x / 64)
+    beamRow(p, beam, heads + static_cast<int64_t>(wave) * p.tiles * p.k, cand[beam], tok[beam]);
+  __syncthreads();
+  if (wave != 0) return;
+  // (candidate, beam) as keys: an order-preserving map of the double; 0 where nothing is left
   int next = 0;
+  double c = 0.0;
+  int t = -1;
+  u64 key = 0;
+  const auto head = [&] {
+    t = lane < p.b && next < p.k ? tok[lane][next] : -1;
+    c = t >= 0 ? cand[lane][next] : 0.0;
+    const u64 u = static_cast<u64>(__double_as_longlong(c == 0.0 ? 0.0 : c));
+    key = t < 0 ? 0 : (u >> 63) ? ~u : u | 0x8000000000000000ull;
+  };
+  head();
   for (int j = 0; j < p.k; ++j) {
-    // a list that is used up, or a token that is not there, is below every -inf
-    double c = -INFINITY;
-    int t = -1;
-    if (lane < p.b && next < p.k) {
-      c = p.cand[lane * p.k + next];
-      t = p.tok[lane * p.k + next];
-    }
-    int who = lane;
-    bool has = t >= 0;
-    for (int o = 32; o > 0; o >>= 1) {
-      const double c2 = __shfl_xor(c, o, 64);
-      const int w2 = __shfl_xor(who, o, 64), t2 = __shfl_xor(t, o, 64), h2 = __shfl_xor(static_cast<int>(has), o, 64);
-      const bool other = h2 && (!has || c2 > c || (c2 == c && w2 < who));
-      if (other) {
-        c = c2;
-        who = w2;
-        t = t2;
-        has = true;
-      }
-    }
-    if (lane == 0) {
+    const u64 top = waveMaxU64(key);
+    const int who = __ffsll(static_cast<unsigned long long>(__ballot(key == top))) - 1;  // the lowest beam
+    if (lane == who) {
       p.outScores[j] = static_cast<float>(c);
       p.outParents[j] = who;
       p.outTokens[j] = t;
       bool end = p.done[who] != 0;
-      for (int e = 0; e < 4; ++e) end = end || (t >= 0 && t == p.eos[e]);
+      for (int e = 0; e < 4; ++e) end = end || t == p.eos[e];
       p.outDone[j] = end ? 1 : 0;
+      ++next;
+      head();
     }
-    if (lane == who) ++next;
   }
 }
 
@@ -210,7 +216,7 @@ __global__ __launch_bounds__(64) void beamPickKernel(BeamParams p) {
 
 namespace {
 
-int64_t beamWaves(int64_t v) { return (v + lkd::kBeamWave - 1) / lkd::kBeamWave; }
+int64_t beamTiles(int64_t v) { return (v + lkd::kBeamTile - 1) / lkd::kBeamTile; }
 
 }  // namespace
 
@@ -218,15 +224,14 @@ extern "C" {
 
 int64_t lk_hip_beam_select_workspace_bytes(int64_t b, int64_t v, int k) {
   if (b <= 0 || v <= 0 || k <= 0) return 0;
-  const int64_t w = beamWaves(v);
-  return (b * w * (8 + 8 * static_cast<int64_t>(k)) + b * k * 12 + 15) / 16 * 16;
+  return (b * beamTiles(v) * (8 + 8 * static_cast<int64_t>(k)) + 15) / 16 * 16;
 }
 
 int lk_hip_beam_select_f32(const float* logits, const float* scores, const int64_t* done, float* out_scores,
                            int64_t* out_parents, int64_t* out_tokens, int64_t* out_done, int64_t b, int64_t v, int k,
                            const int* eos, int num_eos, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace lkd;
-  if (b <= 0 || b > kBeamMost || k <= 0 || k > kBeamMost || v <= 0 || v > int64_t{kBeamWave} * kBeamLists || k > b * v ||
+  if (b <= 0 || b > kBeamMost || k <= 0 || k > kBeamMost || v <= 0 || v > int64_t{kBeamTile} * kBeamLists || k > b * v ||
       num_eos < 1 || num_eos > 4)
     return 1;
   for (int i = 0; i < num_eos; ++i)
@@ -238,15 +243,9 @@ int lk_hip_beam_select_f32(const float* logits, const float* scores, const int64
   p.logits = logits;
   p.scores = scores;
   p.done = done;
-  p.waves = static_cast<int>(beamWaves(v));
-  char* w = static_cast<char*>(workspace);
-  p.lists = reinterpret_cast<uint2*>(w);
-  w += b * p.waves * k * 8;
-  p.cand = reinterpret_cast<double*>(w);
-  w += b * k * 8;
-  p.sums = reinterpret_cast<float*>(w);
-  w += b * p.waves * 8;
-  p.tok = reinterpret_cast<int*>(w);
+  p.tiles = static_cast<int>(beamTiles(v));
+  p.lists = static_cast<uint2*>(workspace);
+  p.sums = reinterpret_cast<float2*>(static_cast<char*>(workspace) + b * p.tiles * k * 8);
   p.outScores = out_scores;
   p.outParents = out_parents;
   p.outTokens = out_tokens;
@@ -256,9 +255,11 @@ int lk_hip_beam_select_f32(const float* logits, const float* scores, const int64
   p.k = k;
   for (int i = 0; i < 4; ++i) p.eos[i] = i < num_eos ? eos[i] : -1;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(beamScanKernel, dim3(static_cast<unsigned>((p.waves + 3) / 4), static_cast<unsigned>(b)), dim3(256), 0, s, p);
-  hipLaunchKernelGGL(beamRowKernel, dim3(static_cast<unsigned>(b)), dim3(64), static_cast<size_t>(p.waves) * k * 8, s, p);
-  hipLaunchKernelGGL(beamPickKernel, dim3(1), dim3(64), 0, s, p);
+  hipLaunchKernelGGL(beamScanKernel, dim3(static_cast<unsigned>(p.tiles), static_cast<unsigned>(b)), dim3(256), 0, s, p);
+  // as many rows at a time as their lists fit 48 KiB (one row's: at most 16)
+  const int64_t row = int64_t{8} * p.tiles * k;
+  const int waves = static_cast<int>(std::min<int64_t>({b, 16, (48 << 10) / row}));
+  hipLaunchKernelGGL(beamPickKernel, dim3(1), dim3(static_cast<unsigned>(64 * waves)), static_cast<size_t>(waves * row), s, p);
   return hipGetLastError() == hipSuccess ? 0 : 2;
 }
 

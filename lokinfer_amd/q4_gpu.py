@@ -16,9 +16,12 @@ from torch's allocator there, so calls on different streams, or in different cap
 """
 from __future__ import annotations
 
+import functools
+
 import numpy as np
 import torch
 
+from ._lib import lib
 from .graph import current_graph
 from .ops import OpError, check
 from .runtime import GpuContext
@@ -32,34 +35,40 @@ _NO_WORK = torch.empty(0, dtype=torch.float32)
 _F16, _F32, _I32, _I64, _U8 = torch.float16, torch.float32, torch.int32, torch.int64, torch.uint8
 
 
-def _ctx() -> GpuContext:
-    if current_graph() is not None:
-        raise OpError("the 4-bit ops run eagerly or in a stream-captured function (lk.capture), not in a traced one")
-    return GpuContext.shared()
+_index = None  # of the context's GPU
 
 
 def _arg(x, dtype, rank, what) -> torch.Tensor:
     """The torch tensor of an operand: of this type and rank, on the context's GPU."""
-    if not isinstance(x, Tensor):
-        raise OpError(f"{what}: expected lk.Tensor, got {type(x).__name__}")
-    t = x.t
-    if t.dtype is not dtype or t.dim() != rank:
-        raise OpError(f"{what} must be a rank {rank} {str(dtype)[6:]} tensor, got {str(t.dtype)[6:]}{list(t.shape)}")
-    if not t.is_cuda:
-        raise OpError(f"{what}: GPU kernel operands must be on the GPU (use ops.to_gpu)")
-    dev = _ctx().device
-    if t.get_device() != dev.index:
-        raise OpError(f"{what} must be on {dev}, is on {t.device}")
+    global _index
+    t = getattr(x, "t", None)
+    if t is None or t.dtype is not dtype or t.dim() != rank or t.get_device() != _index or _index is None:
+        if not isinstance(x, Tensor):
+            raise OpError(f"{what}: expected lk.Tensor, got {type(x).__name__}")
+        if t.dtype is not dtype or t.dim() != rank:
+            raise OpError(f"{what} must be a rank {rank} {str(dtype)[6:]} tensor, got {str(t.dtype)[6:]}{list(t.shape)}")
+        if not t.is_cuda:
+            raise OpError(f"{what}: GPU kernel operands must be on the GPU (use ops.to_gpu)")
+        _index = GpuContext.shared().device.index
+        if t.get_device() != _index:
+            raise OpError(f"{what} must be on cuda:{_index}, is on {t.device}")
     return t
 
 
 def _call(name, tensors, attrs=(), floats=()):
     """Registry kernel `name` over torch tensors (operands, then outs) and its int and float attributes."""
+    if current_graph() is not None:
+        raise OpError("the 4-bit ops run eagerly or in a stream-captured function (lk.capture), not in a traced one")
     ints: list[int] = []
     for t in tensors:
-        ints.extend(t.shape)
-    ints.extend(attrs)
-    _ctx().run(name, [t.data_ptr() for t in tensors], ints, floats)
+        ints += t.shape
+    ints += attrs
+    GpuContext.shared().run(name, [t.data_ptr() for t in tensors], ints, floats)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_bytes(b, t, qh, kvh, cap) -> int:
+    return lib().lk_hip_kv4_attention_workspace_bytes(b, t, qh, kvh, cap)
 
 
 def _empty(shape, dtype=_F16) -> torch.Tensor:
@@ -139,8 +148,7 @@ def unpack_w4_f16_gpu(w: PackedWeight4):
 def _w(w) -> PackedWeight4:
     if not isinstance(w, PackedWeight4):
         raise OpError("the weight must be a PackedWeight4 (pack_w4)")
-    if w.q.t.get_device() != _ctx().device.index:
-        raise OpError(f"the weight must be on {_ctx().device}, is on {w.q.t.device}")
+    _arg(w.q, _I32, 3, "the weight")
     return w
 
 
@@ -293,8 +301,7 @@ def kv4_read_f16_gpu(kv):
     cap = kv4_capacity(kv)
     kt = _arg(kv, _U8, kv.t.dim(), "kv")
     out = _empty((*kt.shape[:-1], cap, HD))
-    blocks = kt.numel() // (ROW * cap)
-    _ctx().run("kv4_read_f16_gpu", (kt.data_ptr(), out.data_ptr()), (blocks, ROW * cap, blocks, cap, HD), ())
+    _call("kv4_read_f16_gpu", [kt.view(-1, ROW * cap), out.view(-1, cap, HD)])
     return Tensor(out)
 
 
@@ -309,7 +316,7 @@ def attention_kv4_f16_gpu(q, kv, pos):
     rows, width = qt.shape
     if width <= 0 or width % (HD * kvh):
         raise OpError("q must be f16[B T, qh 128], qh a multiple of kvh")
-    need = _ctx().lib.lk_hip_kv4_attention_workspace_bytes(b, rows // b, width // HD, kvh, row // ROW)
+    need = _attention_bytes(b, rows // b, width // HD, kvh, row // ROW)
     out = _empty((rows, width))
     _call("attention_kv4_f16_gpu", [qt, kt, pt, out, _empty((-(-need // 4),), _F32) if need else _NO_WORK])
     return Tensor(out)
