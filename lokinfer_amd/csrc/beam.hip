@@ -5,13 +5,14 @@
 // The k best of all B V, ties to the lowest b V + t. What has no value (a NaN, a row without a finite log-sum, a beam whose
 // score is not finite) counts as -inf.
 //
-// Two launches. beamScanKernel passes once over the logits: each wave keeps 1024 of a row in registers and takes their k
-// best one after the other (a maximum over the wave of (order of the logit, index) keys by DPP moves), a workgroup
-// joins its four waves' lists by counting for each entry the better ones, and leaves one list, the maximum and the sum of
-// exponentials of its 4096 logits. beamPickKernel, one workgroup, joins a row's lists with one wave (lane i at the head
-// of list i), adds up its log-sum, and takes the k best of the rows' heads. Within a row the order is that of the logits
-// (exact); between beams that of the candidates in 64 bits, the sums of exponentials of 4096 logits each (32 bits) added
-// in 64 bits.
+// Two launches. beamScanKernel passes once over the logits, 8192 of a row per workgroup, 32 per lane in registers, and leaves
+// their k best, maximum and sum of exponentials. At least k of a wave's 64 lane maxima, so k of its logits, are not below the
+// k-th largest of them (found by counting); the logits not below the largest such bound of the four waves, k and some
+// more, go to LDS and are ranked by counting. Where they are more than fit (thousands of equal logits), each wave takes
+// its k best one after the other instead. beamPickKernel, one workgroup, joins a row's lists with one wave (lane i at the
+// head of list i), adds up its log-sum, and takes the k best of the rows' heads. Within a row the order is that of the
+// logits (exact); between beams that of the candidates in 64 bits, the sums of exponentials of 8192 logits each (32
+// bits) added in 64 bits.
 #include <algorithm>
 
 #include "common.h"
@@ -20,8 +21,10 @@
 namespace lkd {
 
 constexpr int kBeamMost = 32;    // beams and k
-constexpr int kBeamTile = 4096;  // logits per workgroup of 4 waves
-constexpr int kBeamLists = 64;   // lists per row at most: V <= 262144
+constexpr int kBeamWaves = 4;    // per workgroup of the scan
+constexpr int kBeamTile = 8192;  // its logits, 32 per lane
+constexpr int kBeamFit = 256;    // logits of a tile that are ranked by counting: one per thread, at least 4 kBeamMost
+constexpr int kBeamLists = 32;   // lists per row at most: V <= 262144
 
 struct BeamParams {
   const float* logits;   // [B, V]
@@ -40,9 +43,8 @@ struct BeamParams {
 
 // order-preserving key: larger logit, larger key; 0 is below all. NaN counts as -inf, -0 as 0
 __device__ __forceinline__ unsigned orderOf(float x) {
-  if (!(x == x)) x = -INFINITY;
-  const unsigned u = __float_as_uint(x == 0.0f ? 0.0f : x);
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  const unsigned u = __float_as_uint((x == x ? x : -INFINITY) + 0.0f);
+  return u ^ (static_cast<unsigned>(static_cast<int>(u) >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float valueOf(unsigned key) {
   return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
@@ -53,39 +55,42 @@ __device__ __forceinline__ u64 pairOf(unsigned hi, unsigned lo) { return (static
 
 // the wave's largest value, in every lane
 template <int CTRL>
-__device__ __forceinline__ u64 maxDpp(u64 v) {
-  const unsigned hi = __builtin_amdgcn_update_dpp(0, static_cast<unsigned>(v >> 32), CTRL, 0xF, 0xF, false);
-  const unsigned lo = __builtin_amdgcn_update_dpp(0, static_cast<unsigned>(v), CTRL, 0xF, 0xF, false);
-  return max(v, pairOf(hi, lo));
+__device__ __forceinline__ unsigned maxDpp(unsigned v) {
+  return max(v, static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, false)));
 }
-__device__ __forceinline__ u64 waveMaxU64(u64 v) {
+__device__ __forceinline__ unsigned waveMaxU32(unsigned v) {
   v = maxDpp<0xB1>(v);   // quad_perm [1, 0, 3, 2]
   v = maxDpp<0x4E>(v);   // quad_perm [2, 3, 0, 1]
   v = maxDpp<0x141>(v);  // row_half_mirror
   v = maxDpp<0x140>(v);  // row_mirror
-  const auto h = __builtin_amdgcn_permlane16_swap(static_cast<unsigned>(v >> 32), static_cast<unsigned>(v >> 32), false, false);
-  const auto l = __builtin_amdgcn_permlane16_swap(static_cast<unsigned>(v), static_cast<unsigned>(v), false, false);
-  v = max(pairOf(h[0], l[0]), pairOf(h[1], l[1]));
-  const auto h2 = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(v >> 32), static_cast<unsigned>(v >> 32), false, false);
-  const auto l2 = __builtin_amdgcn_permlane32_swap(static_cast<unsigned>(v), static_cast<unsigned>(v), false, false);
-  return max(pairOf(h2[0], l2[0]), pairOf(h2[1], l2[1]));
+  const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(p[0], p[1]);
+  const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(h[0], h[1]);
+}
+__device__ __forceinline__ u64 waveMaxU64(unsigned hi, unsigned lo) {
+  const unsigned top = waveMaxU32(hi);
+  return pairOf(top, waveMaxU32(hi == top ? lo : 0u));
 }
 
-__global__ __launch_bounds__(256) void beamScanKernel(BeamParams p) {
-  __shared__ u64 best[4][kBeamMost];
-  __shared__ float2 part[4];
+__global__ __launch_bounds__(64 * kBeamWaves) void beamScanKernel(BeamParams p) {
+  __shared__ u64 fit[kBeamFit];
+  __shared__ unsigned bounds[kBeamWaves];
+  __shared__ int count;
+  __shared__ float2 part[kBeamWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = blockIdx.x, beam = blockIdx.y;
   const float* x = p.logits + static_cast<int64_t>(beam) * p.v;
-  constexpr int E = kBeamTile / 256;
+  constexpr int E = kBeamTile / (64 * kBeamWaves);
   const unsigned first = static_cast<unsigned>(tile) * kBeamTile + wave * 64 * E + lane;
   unsigned key[E];
   float val[E], m = -INFINITY;
+  const unsigned v = static_cast<unsigned>(p.v);
 #pragma unroll
-  for (int e = 0; e < E; ++e) val[e] = x[min<int64_t>(first + 64 * e, p.v - 1)];
+  for (int e = 0; e < E; ++e) val[e] = x[min(first + 64 * e, v - 1)];
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const bool in = first + 64 * e < p.v;
-    if (!in) val[e] = -INFINITY;
+    const bool in = first + 64 * e < v;
+    val[e] = in ? val[e] : -INFINITY;
     key[e] = in ? orderOf(val[e]) : 0u;
     m = fmaxf(m, val[e]);
   }
@@ -93,38 +98,63 @@ __global__ __launch_bounds__(256) void beamScanKernel(BeamParams p) {
   float s = 0.0f;
   const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-  for (int e = 0; e < E; ++e) s += expf(val[e] - base);  // a NaN stays one; inf - inf is one
+  for (int e = 0; e < E; ++e) s += __builtin_amdgcn_exp2f((val[e] - base) * kLog2e);  // a NaN stays one; inf - inf is one
   s = waveSumDpp(s);
   if (lane == 0) part[wave] = make_float2(m, s);
-  for (int j = 0; j < p.k; ++j) {
-    unsigned bk = key[0], be = 0u;  // equal keys of one lane: the first has the smallest index
+  unsigned top = key[0];
 #pragma unroll
-    for (int e = 1; e < E; ++e) {
-      const bool more = key[e] > bk;
-      bk = more ? key[e] : bk;
-      be = more ? e : be;
-    }
-    const u64 top = waveMaxU64(pairOf(bk, ~(first + 64 * be)));
-    if (lane == 0) best[wave][j] = top;
-    const unsigned at = ~static_cast<unsigned>(top) - first;  // a multiple of 64 below 64 E in the lane that holds it
+  for (int e = 1; e < E; ++e) top = max(top, key[e]);
+  int above = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (at == 64u * e) key[e] = 0u;
-  }
+  for (int i = 0; i < 64; ++i) above += static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(top), i)) > top;
+  // the smallest of the lane maxima with fewer than k above them
+  const unsigned bound = ~waveMaxU32(above < p.k ? ~top : 0u);
+  if (lane == 0) bounds[wave] = bound;
+  if (threadIdx.x == 0) count = 0;
   __syncthreads();
-  if (threadIdx.x < 4u * p.k) {  // entries without a logit (key 0) are distinct by their index
-    const u64 mine = best[threadIdx.x / p.k][threadIdx.x % p.k];
+  unsigned least = bounds[0];
+#pragma unroll
+  for (int w = 1; w < kBeamWaves; ++w) least = max(least, bounds[w]);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (key[e] >= least) {
+      const int at = atomicAdd(&count, 1);
+      if (at < kBeamFit) fit[at] = pairOf(key[e], ~(first + 64 * e));
+    }
+  __syncthreads();
+  int n = count;
+  if (n > kBeamFit) {  // the same for every thread
+    __syncthreads();
+    for (int j = 0; j < p.k; ++j) {
+      unsigned bk = key[0], be = 0u;  // equal keys of one lane: the first has the smallest index
+#pragma unroll
+      for (int e = 1; e < E; ++e) {
+        const bool more = key[e] > bk;
+        bk = more ? key[e] : bk;
+        be = more ? e : be;
+      }
+      const u64 best = waveMaxU64(bk, ~(first + 64 * be));
+      if (lane == 0) fit[wave * p.k + j] = best;
+      const unsigned at = ~static_cast<unsigned>(best) - first;  // a multiple of 64 below 64 E in the lane that holds it
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at == 64u * e) key[e] = 0u;
+    }
+    __syncthreads();
+    n = kBeamWaves * p.k;
+  }
+  if (static_cast<int>(threadIdx.x) < n) {  // entries without a logit (key 0) are distinct by their index
+    const u64 mine = fit[threadIdx.x];
     int rank = 0;
-    for (int w = 0; w < 4; ++w)
-      for (int j = 0; j < p.k; ++j) rank += best[w][j] > mine;
+    for (int j = 0; j < n; ++j) rank += fit[j] > mine;
     if (rank < p.k)
       p.lists[(static_cast<int64_t>(beam) * p.tiles + tile) * p.k + rank] =
           make_uint2(static_cast<unsigned>(mine >> 32), ~static_cast<unsigned>(mine));
   }
   if (threadIdx.x == 0) {
     float mm = -INFINITY, ss = 0.0f;
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, part[w].x);
-    for (int w = 0; w < 4; ++w)
+    for (int w = 0; w < kBeamWaves; ++w) mm = fmaxf(mm, part[w].x);
+    for (int w = 0; w < kBeamWaves; ++w)
       ss += part[w].x == -INFINITY ? (part[w].y == part[w].y ? 0.0f : part[w].y) : part[w].y * expf(part[w].x - mm);
     p.sums[static_cast<int64_t>(beam) * p.tiles + tile] = make_float2(mm, ss);
   }
@@ -136,7 +166,16 @@ __device__ __forceinline__ void beamRow(const BeamParams& p, int beam, uint2* he
   const int64_t at = static_cast<int64_t>(beam) * p.tiles;
   const float score = p.scores[beam];
   const float2 mine = lane < p.tiles ? p.sums[at + lane] : make_float2(-INFINITY, 0.0f);
-  for (int i = lane; i < p.tiles * p.k; i += 64) heads[i] = p.lists[at * p.k + i];
+  const uint2* lists = p.lists + at * p.k;
+  const int entries = p.tiles * p.k;
+  for (int i0 = lane; i0 < entries; i0 += 64 * 8) {  // 8 loads in flight
+    uint2 e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = lists[min(i0 + 64 * i, entries - 1)];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + 64 * i < entries) heads[i0 + 64 * i] = e[i];
+  }
   const float m = waveMaxDpp(mine.x);
   double sum = mine.x == -INFINITY ? (mine.y == mine.y ? 0.0 : mine.y)
                                    : mine.y * exp(static_cast<double>(mine.x) - static_cast<double>(m));
@@ -158,19 +197,20 @@ __device__ __forceinline__ void beamRow(const BeamParams& p, int beam, uint2* he
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   int next = 0;
-  uint2 h = lane < p.tiles ? heads[lane * p.k] : make_uint2(0u, 0u);
+  uint2 h = lane < p.tiles ? heads[lane * p.k] : make_uint2(0u, 0u), mineOf{0u, 0u};  // lane j keeps the j-th best
   for (int j = 0; j < p.k; ++j) {
-    const u64 top = waveMaxU64(pairOf(h.x, ~h.y));
+    const u64 top = waveMaxU64(h.x, ~h.y);
     const unsigned bk = static_cast<unsigned>(top >> 32), bi = ~static_cast<unsigned>(top);
-    if (lane == 0) {
-      const double c = static_cast<double>(score) + (static_cast<double>(valueOf(bk)) - lse);
-      cand[j] = bk != 0u && c == c ? c : -INFINITY;
-      tok[j] = bk != 0u ? static_cast<int>(bi) : -1;  // fewer than k logits: none left
-    }
+    if (lane == j) mineOf = make_uint2(bk, bi);
     if (bk != 0u && h.x == bk && h.y == bi) {
       ++next;
       h = next < p.k ? heads[lane * p.k + next] : make_uint2(0u, 0u);
     }
+  }
+  if (lane < p.k) {
+    const double c = static_cast<double>(score) + (static_cast<double>(valueOf(mineOf.x)) - lse);
+    cand[lane] = mineOf.x != 0u && c == c ? c : -INFINITY;
+    tok[lane] = mineOf.x != 0u ? static_cast<int>(mineOf.y) : -1;  // fewer than k logits: none left
   }
 }
 
@@ -185,6 +225,7 @@ __global__ __launch_bounds__(1024) void beamPickKernel(BeamParams p) {
   __syncthreads();
   if (wave != 0) return;
   // (candidate, beam) as keys: an order-preserving map of the double; 0 where nothing is left
+  const bool over = lane < p.b && p.done[lane] != 0;
   int next = 0;
   double c = 0.0;
   int t = -1;
@@ -197,13 +238,13 @@ __global__ __launch_bounds__(1024) void beamPickKernel(BeamParams p) {
   };
   head();
   for (int j = 0; j < p.k; ++j) {
-    const u64 top = waveMaxU64(key);
+    const u64 top = waveMaxU64(static_cast<unsigned>(key >> 32), static_cast<unsigned>(key));
     const int who = __ffsll(static_cast<unsigned long long>(__ballot(key == top))) - 1;  // the lowest beam
     if (lane == who) {
       p.outScores[j] = static_cast<float>(c);
       p.outParents[j] = who;
       p.outTokens[j] = t;
-      bool end = p.done[who] != 0;
+      bool end = over;
       for (int e = 0; e < 4; ++e) end = end || t == p.eos[e];
       p.outDone[j] = end ? 1 : 0;
       ++next;
@@ -255,7 +296,8 @@ int lk_hip_beam_select_f32(const float* logits, const float* scores, const int64
   p.k = k;
   for (int i = 0; i < 4; ++i) p.eos[i] = i < num_eos ? eos[i] : -1;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(beamScanKernel, dim3(static_cast<unsigned>(p.tiles), static_cast<unsigned>(b)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(beamScanKernel, dim3(static_cast<unsigned>(p.tiles), static_cast<unsigned>(b)),
+                     dim3(64 * kBeamWaves), 0, s, p);
   // as many rows at a time as their lists fit 48 KiB (one row's: at most 16)
   const int64_t row = int64_t{8} * p.tiles * k;
   const int waves = static_cast<int>(std::min<int64_t>({b, 16, (48 << 10) / row}));

@@ -405,23 +405,27 @@ __global__ __launch_bounds__(256) void kv4ExpandKernel(const char* __restrict__ 
 }
 
 // ---- moving caches between sequences ------------------------------------------------------------------------------
-// One thread per 8 bytes of codes, or 2 of scales, of a (layer, key or value, kv head)'s live rows: it reads the piece of
-// every sequence from that sequence's parent, then writes them, so that no write comes before a read of the same bytes.
+// One thread per 16 bytes of codes or of a scale plane (2 bytes behind its last whole 8 rows) of a (layer, key or value, kv
+// head)'s live rows: it reads the piece of the
+// parent of every sequence whose parent is another, then writes them, so that no write comes before a read of the same
+// bytes. MB: B rounded up, so that the pieces stay in registers, all reads in flight together.
 constexpr int kMaxBeams = 32;
-template <typename T>
-__device__ __forceinline__ void kv4Move(char* at, int64_t seqStride, const int64_t* parents, int b, T none) {
-  T v[kMaxBeams];
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+template <int MB, typename T>
+__device__ __forceinline__ void kv4Move(char* at, int64_t seqStride, const int64_t* __restrict__ parents, int b, T none) {
+  T v[MB];
 #pragma unroll
-  for (int i = 0; i < kMaxBeams; ++i)
-    if (i < b) {
-      const int64_t from = parents[i];
-      v[i] = from >= 0 && from < b ? *reinterpret_cast<const T*>(at + from * seqStride) : none;
-    }
+  for (int i = 0; i < MB; ++i) {
+    v[i] = none;
+    const int64_t from = i < b ? parents[i] : i;
+    if (from != i && from >= 0 && from < b) v[i] = *reinterpret_cast<const T*>(at + from * seqStride);
+  }
 #pragma unroll
-  for (int i = 0; i < kMaxBeams; ++i)
+  for (int i = 0; i < MB; ++i)
     if (i < b && parents[i] != i) *reinterpret_cast<T*>(at + i * seqStride) = v[i];
 }
 
+template <int MB>
 __global__ __launch_bounds__(256) void kv4ReorderKernel(char* __restrict__ kv, const int64_t* __restrict__ parents,
                                                         const int64_t* __restrict__ n, int64_t layers, int b, int kvh,
                                                         int64_t cap, unsigned long long* err) {
@@ -433,13 +437,21 @@ __global__ __launch_bounds__(256) void kv4ReorderKernel(char* __restrict__ kv, c
     for (int i = 0; i < b; ++i)
       if (parents[i] < 0 || parents[i] >= b) raiseDeviceError(err, LK_DEVERR_INDEX, parents[i]);
   }
-  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < rows * 12;
+  const int64_t whole = rows / 8, rest = rows - whole * 8, codes = rows * 4, items = codes + 4 * (whole + rest);
+  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < items;
        id += static_cast<int64_t>(gridDim.x) * 256) {
-    if (id < rows * 8) {
-      kv4Move<unsigned long long>(base + id * 8, seqStride, parents, b, 0ull);
+    constexpr unsigned kNan2 = 0x7E007E00u;  // where a parent is not there
+    if (id < codes + 4 * whole) {
+      int64_t at = id * 16;
+      if (id >= codes) {
+        const int64_t j = id - codes, g = j / whole;
+        at = 64 * cap + g * 2 * cap + 16 * (j - g * whole);
+      }
+      kv4Move<MB>(base + at, seqStride, parents, b, u32x4{kNan2, kNan2, kNan2, kNan2});
     } else {
-      const int64_t j = id - rows * 8, g = j / rows;
-      kv4Move<unsigned short>(base + 64 * cap + g * 2 * cap + 2 * (j - g * rows), seqStride, parents, b, 0x7E00);  // NaN
+      const int64_t j = id - codes - 4 * whole, g = j / rest;
+      kv4Move<MB, unsigned short>(base + 64 * cap + g * 2 * cap + 16 * whole + 2 * (j - g * rest), seqStride, parents, b,
+                                  kNan2 & 0xFFFFu);
     }
   }
 }
@@ -553,10 +565,12 @@ int lk_hip_kv4_reorder(void* kv, const int64_t* parents, const int64_t* n, int64
   using namespace lkd;
   if (!kvOk(kv, b, kvh, cap) || layers < 0 || b > kMaxBeams || layers * 2 * kvh > 65535) return 1;
   if (layers == 0) return 0;
-  const unsigned gx = static_cast<unsigned>(std::min<int64_t>((cap * 9 + 255) / 256, 64));
-  hipLaunchKernelGGL(kv4ReorderKernel, dim3(gx, static_cast<unsigned>(layers * 2 * kvh)), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), static_cast<char*>(kv), parents, n, layers, static_cast<int>(b), kvh,
-                     cap, lkh::deviceErrorRecord());
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((cap * 9 / 2 + 255) / 256, 64)),
+                  static_cast<unsigned>(layers * 2 * kvh));
+  const auto kernel = b <= 4 ? kv4ReorderKernel<4> : b <= 8 ? kv4ReorderKernel<8> : b <= 16 ? kv4ReorderKernel<16>
+                                                                                         : kv4ReorderKernel<32>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<char*>(kv), parents, n, layers,
+                     static_cast<int>(b), kvh, cap, lkh::deviceErrorRecord());
   return launched();
 }
 

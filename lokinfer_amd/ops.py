@@ -929,23 +929,31 @@ def beam_select_f32_gpu(logits, scores, done, k, eos):
     ties to the lowest b V + t -> (scores f32[k], parents i64[k], tokens i64[k], done i64[k]), best first; done: the parent's,
     or the token is one of `eos` (1 to 4 ids). What has no value (a NaN, a row or a score that is not finite) counts as
     -inf. B, k <= 32, V <= 262144. Not traceable."""
-    check(current_graph() is None, "beam_select runs eagerly or in a stream-captured function, not in a traced one")
+    if current_graph() is not None:
+        raise OpError("beam_select runs eagerly or in a stream-captured function, not in a traced one")
     _gpu(logits, scores, done)
-    _f32(logits, rank=2)
-    _f32(scores, rank=1)
     ctx, k = GpuContext.shared(), int(k)
     x, s, d = logits.t, scores.t, done.t
+    if x.dtype is not torch.float32 or s.dtype is not torch.float32 or d.dtype is not torch.int64 or x.dim() != 2:
+        raise OpError("logits must be f32[B, V], scores f32[B], done i64[B]")
     b, v = x.shape
-    check(x.device == s.device == d.device == ctx.device, f"operands must be on {ctx.device}")
-    check(1 <= b <= 32 and 1 <= k <= 32 and 1 <= v <= 262144 and k <= b * v, "B and k at most 32, V at most 262144, k <= B V")
-    check(s.shape[0] == b and d.dtype is torch.int64 and tuple(d.shape) == (b,), "scores must be f32[B], done i64[B]")
-    check(1 <= len(eos) <= 4 and all(0 <= e < v for e in eos), "eos must be 1 to 4 ids below V")
+    if not (x.get_device() == s.get_device() == d.get_device() == ctx.device.index):
+        raise OpError(f"operands must be on {ctx.device}")
+    if not (1 <= b <= 32 and 1 <= k <= 32 and 1 <= v <= 262144 and k <= b * v):
+        raise OpError("B and k at most 32, V at most 262144, k <= B V")
+    if s.shape != (b,) or d.shape != (b,):
+        raise OpError("scores must be f32[B], done i64[B]")
+    if not (1 <= len(eos) <= 4 and all(0 <= e < v for e in eos)):
+        raise OpError("eos must be 1 to 4 ids below V")
     work = ctx.lib.lk_hip_beam_select_workspace_bytes(b, v, k) // 4
     best = torch.empty(k, dtype=torch.float32, device=ctx.device)
-    picks = torch.empty((3, k), dtype=torch.int64, device=ctx.device).unbind(0)
+    picks = torch.empty((3, k), dtype=torch.int64, device=ctx.device)
     scratch = torch.empty(work, dtype=torch.float32, device=ctx.device)
-    ctx.run("beam_select_f32_gpu", [t.data_ptr() for t in (x, s, d, best, *picks, scratch)],
-            [b, v, b, b, k, k, k, k, work, *(int(e) for e in eos)], ())
+    at = picks.data_ptr()
+    ctx.run("beam_select_f32_gpu",
+            (x.data_ptr(), s.data_ptr(), d.data_ptr(), best.data_ptr(), at, at + 8 * k, at + 16 * k, scratch.data_ptr()),
+            (b, v, b, b, k, k, k, k, work, *(int(e) for e in eos)), ())
+    picks = picks.unbind(0)
     return (Tensor(best), *(Tensor(t) for t in picks))
 
 

@@ -25,7 +25,7 @@ from ._lib import lib
 from .graph import current_graph
 from .ops import OpError, check
 from .runtime import GpuContext
-from .tensor import Tensor, f16, i32, u8
+from .tensor import Tensor, f16, i32
 
 GROUPS = (32, 64, 128)
 ROW = 72  # bytes of a cache row: 64 of codes, 4 f16 scales
@@ -55,15 +55,19 @@ def _arg(x, dtype, rank, what) -> torch.Tensor:
     return t
 
 
-def _call(name, tensors, attrs=(), floats=()):
-    """Registry kernel `name` over torch tensors (operands, then outs) and its int and float attributes."""
+def _run(name, ptrs, ints, floats=()):
     if current_graph() is not None:
         raise OpError("the 4-bit ops run eagerly or in a stream-captured function (lk.capture), not in a traced one")
+    GpuContext.shared().run(name, ptrs, ints, floats)
+
+
+def _call(name, tensors, attrs=(), floats=()):
+    """Registry kernel `name` over torch tensors (operands, then outs) and its int and float attributes."""
     ints: list[int] = []
     for t in tensors:
         ints += t.shape
     ints += attrs
-    GpuContext.shared().run(name, [t.data_ptr() for t in tensors], ints, floats)
+    _run(name, [t.data_ptr() for t in tensors], ints, floats)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -246,9 +250,10 @@ def kv4_cache(batch: int, kv_heads: int, capacity: int, layers: int | None = Non
 
 def kv4_capacity(kv: Tensor) -> int:
     """Rows of a cache."""
-    check(isinstance(kv, Tensor) and kv.dtype == u8 and kv.shape[-1] > 0 and kv.shape[-1] % (32 * ROW) == 0,
-          "a 4-bit cache is u8[..., 72 P] with P a multiple of 32")
-    return kv.shape[-1] // ROW
+    if not (isinstance(kv, Tensor) and kv.t.dtype is _U8 and kv.t.dim() and kv.t.shape[-1] > 0
+            and kv.t.shape[-1] % (32 * ROW) == 0):
+        raise OpError("a 4-bit cache is u8[..., 72 P] with P a multiple of 32")
+    return kv.t.shape[-1] // ROW
 
 
 def _kv(kv, pos):
@@ -301,7 +306,8 @@ def kv4_read_f16_gpu(kv):
     cap = kv4_capacity(kv)
     kt = _arg(kv, _U8, kv.t.dim(), "kv")
     out = _empty((*kt.shape[:-1], cap, HD))
-    _call("kv4_read_f16_gpu", [kt.view(-1, ROW * cap), out.view(-1, cap, HD)])
+    blocks = kt.numel() // (ROW * cap)
+    _run("kv4_read_f16_gpu", (kt.data_ptr(), out.data_ptr()), (blocks, ROW * cap, blocks, cap, HD))
     return Tensor(out)
 
 
