@@ -123,13 +123,14 @@ __global__ __launch_bounds__(256) void kv4QkRopeKernel(Kv4QkrParams p) {
 // one thread per 8 values: blocks of 72 cap bytes -> f16 [blocks, cap, 128]
 __global__ __launch_bounds__(256) void kv4ReadKernel(const char* __restrict__ kv, h16* __restrict__ out, int64_t blocks,
                                                      int64_t cap) {
+  const Q4Masks masks;
   const int64_t total = blocks * cap * 16;
   for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
        id += static_cast<int64_t>(gridDim.x) * 256) {
     const int64_t r = id >> 4, blk = r / cap, row = r - blk * cap;
     const int w = static_cast<int>(id & 15);
     const char* at = kv + blk * 72 * cap;
-    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(at + row * 64 + 4 * w));
+    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(at + row * 64 + 4 * w), masks);
     const h16 s = *reinterpret_cast<const h16*>(at + cap * 64 + (w >> 2) * 2 * cap + 2 * row);
     half8 y;
 #pragma unroll
@@ -164,6 +165,7 @@ struct Kv4Params {
 // Keys from the longest row's end on have their weight and their value's scale set to zero, whatever the memory holds there.
 constexpr int KW = 8;
 __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
+  const Q4Masks masks;
   __shared__ __attribute__((aligned(16))) float os[KW][16][KHD + 4];
   __shared__ float ms[KW][16], ls[KW][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 15, kq = lane >> 4;
@@ -230,7 +232,7 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
       s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int w = 0; w < 4; ++w)
-        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4Ints(w4[w]) * half8{f, f, f, f, f, f, f, f}, qf[w], s[u], 0, 0, 0);
+        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4Ints(w4[w], masks) * half8{f, f, f, f, f, f, f, f}, qf[w], s[u], 0, 0, 0);
     }
     if (c * 64 + 64 > nkAll) {  // keys past some row's
 #pragma unroll
@@ -286,7 +288,7 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
         half2v dims[4][4];  // [dim 2 i + o][pair of keys]
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const half8 v = q4Ints(o ? odd[j] : even[j]);
+          const half8 v = q4Ints(o ? odd[j] : even[j], masks);
 #pragma unroll
           for (int i = 0; i < 4; ++i) dims[i][j] = half2v{v[2 * i], v[2 * i + 1]} * sc[j];
         }
@@ -390,6 +392,7 @@ __global__ __launch_bounds__(128) void kv4MergeKernel(Kv4Params p) {
 // lk_hip_f16_attention_gqa: they are dequantised once instead of by every block of queries. 8 values per thread.
 __global__ __launch_bounds__(256) void kv4ExpandKernel(const char* __restrict__ kv, const int64_t* __restrict__ pos,
                                                        h16* __restrict__ out, int64_t t, int kvh, int64_t cap) {
+  const Q4Masks masks;
   const int64_t p0 = *pos, rows = p0 < 0 ? 0 : min<int64_t>(p0 + t, cap), per = static_cast<int64_t>(kvh) * 16;
   const char* base = kv + blockIdx.y * kvh * 72 * cap;
   h16* o = out + blockIdx.y * cap * kvh * KHD;
@@ -398,7 +401,7 @@ __global__ __launch_bounds__(256) void kv4ExpandKernel(const char* __restrict__ 
     const int64_t row = id / per;
     const int at = static_cast<int>(id - row * per), w = at & 15;
     const char* blk = base + (at >> 4) * 72 * cap;
-    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(blk + row * 64 + 4 * w));
+    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(blk + row * 64 + 4 * w), masks);
     const h16 s = *reinterpret_cast<const h16*>(blk + cap * 64 + (w >> 2) * 2 * cap + 2 * row);
     st8(o + id * 8, v * half8{s, s, s, s, s, s, s, s});
   }

@@ -34,17 +34,23 @@ __device__ __forceinline__ unsigned q4Code(float x, float s) {
 // bit position of the word's j-th code
 __device__ __forceinline__ constexpr int q4Shift(int j) { return 4 * (j >> 1) + 16 * (j & 1); }
 
+// The constants of q4Ints in registers: as literals they would not fit one and-or instruction. Made once, at a kernel's start.
+struct Q4Masks {
+  unsigned low = 0x000F000Fu, high = 0x00F000F0u, magic = 0x64006400u;
+  __device__ __forceinline__ Q4Masks() { asm("" : "+v"(low), "+v"(high), "+v"(magic)); }
+};
+
 // the 8 integers c - 8 of a word, in order, exact in f16: a code under the mantissa of 1024 reads 1024 + c, four bits
 // higher 1024 + 16 c
-__device__ __forceinline__ half8 q4Ints(unsigned w) {
+__device__ __forceinline__ half8 q4Ints(unsigned w, const Q4Masks& m) {
   const half2v k0 = {static_cast<h16>(-1032.0f), static_cast<h16>(-1032.0f)};
   const half2v k1 = {static_cast<h16>(-72.0f), static_cast<h16>(-72.0f)};
   const half2v r = {static_cast<h16>(0.0625f), static_cast<h16>(0.0625f)};
   const unsigned v = w >> 8;
-  const half2v a = __builtin_bit_cast(half2v, (w & 0x000F000Fu) | 0x64006400u) + k0;
-  const half2v b = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w & 0x00F000F0u) | 0x64006400u), r, k1);
-  const half2v c = __builtin_bit_cast(half2v, (v & 0x000F000Fu) | 0x64006400u) + k0;
-  const half2v d = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (v & 0x00F000F0u) | 0x64006400u), r, k1);
+  const half2v a = __builtin_bit_cast(half2v, (w & m.low) | m.magic) + k0;
+  const half2v b = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (w & m.high) | m.magic), r, k1);
+  const half2v c = __builtin_bit_cast(half2v, (v & m.low) | m.magic) + k0;
+  const half2v d = __builtin_elementwise_fma(__builtin_bit_cast(half2v, (v & m.high) | m.magic), r, k1);
   return half8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 

@@ -74,6 +74,7 @@ __global__ __launch_bounds__(256) void w4PackKernel(const void* __restrict__ src
 // one thread per (8 k, column): out f16[K, N]
 __global__ __launch_bounds__(256) void w4UnpackKernel(const unsigned* __restrict__ q, const h16* __restrict__ s,
                                                       h16* __restrict__ out, W4Layout p) {
+  const Q4Masks masks;
   const int per = 128 / p.group;
   const int64_t total = (p.k + 7) / 8 * p.n;
   for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
@@ -81,7 +82,7 @@ __global__ __launch_bounds__(256) void w4UnpackKernel(const unsigned* __restrict
     const int64_t k8 = id / p.n, n = id - k8 * p.n, k = 8 * k8, tile = (n >> 4) * p.kb + k / 128;
     const int in = static_cast<int>(k & 127);
     const h16 sc = s[(tile * 16 + (n & 15)) * per + in / p.group];
-    const half8 v = q4Ints(q[(tile * 64 + (n & 15) + 16 * ((in >> 3) & 3)) * 4 + (in >> 5)]);
+    const half8 v = q4Ints(q[(tile * 64 + (n & 15) + 16 * ((in >> 3) & 3)) * 4 + (in >> 5)], masks);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (k + j < p.k) out[(k + j) * p.n + n] = v[j] * sc;
@@ -100,175 +101,284 @@ struct W4Params {
   float eps;
 };
 
-// Up to 16 MT rows: WAVES waves of a workgroup share one tile of 16 columns (SwiGLU: one of each weight), wave w taking the
-// k blocks w, w + WAVES, ...; their sums meet in LDS. x row j of a 16-row block is the A operand's row 4 (j % 4) + j / 4, so
-// that its sums are accumulator j / 4 of lanes 16 (j % 4) ..: a few rows need only RU = ceil(rows / 4) of the 4
-// accumulators scaled. A group's products are summed on its integers and scaled once, in f32.
-template <int MT, int RU, int G, int W, bool F32, bool RMS, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void w4SkinnyKernel(W4Params p) {
-  __shared__ float red[WAVES][W][MT][RU][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int a = lane & 15, kq = lane >> 4;
-  const int64_t tile = blockIdx.x, m0 = static_cast<int64_t>(blockIdx.y) * 16 * MT;
-  constexpr int PER = 128 / G, STEPS = G / 32;
-  float rf = 1.0f;
-  if constexpr (RMS) rf = rmsFactor(rowSumSq(p.x, p.k, lane), p.k, p.eps);
-  float acc[W][MT][RU];
-#pragma unroll
-  for (int w = 0; w < W; ++w)
-#pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int r = 0; r < RU; ++r) acc[w][t][r] = 0.0f;
-  for (int64_t kb = wave; kb < p.kb; kb += WAVES) {
-    uint4 q[W];
-    h16 sc[W][PER];
+// ---- up to 16 rows: 16x16x32 MFMAs, x as A (its row j is the operand's row 4 (j % 4) + j / 4, so that its sums are
+// accumulator j / 4 of lanes 16 (j % 4) ..: few rows need only RU = ceil(rows / 4) of the 4 accumulators), 16 columns of the
+// weight as B. A group's products are summed on its integers and scaled once, in f32.
+template <int G, int W>
+struct W4Block {  // a tile's k block, as loaded
+  static constexpr int PER = 128 / G;
+  uint4 q[W];
+  h16 s[W][PER];
+  __device__ __forceinline__ void load(const W4Params& p, int64_t tile, int64_t kb, int lane) {
+    const int64_t at = tile * p.kb + kb;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const int64_t at = tile * p.kb + kb;
-      q[w] = p.q[w][at * 64 + lane];
+      typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+      const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p.q[w] + at * 64 + lane));  // read once
+      q[w] = make_uint4(v[0], v[1], v[2], v[3]);
+      const h16* sp = p.s[w] + (at * 16 + (lane & 15)) * PER;
 #pragma unroll
-      for (int g = 0; g < PER; ++g) sc[w][g] = p.s[w][(at * 16 + a) * PER + g];
+      for (int g = 0; g < PER; ++g) s[w][g] = sp[g];
     }
-    half8 xa[4][MT];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        const int64_t row = m0 + 16 * t + 4 * (a & 3) + (a >> 2), k = kb * 128 + 32 * i + 8 * kq;
-        xa[i][t] = half8{};
-        if (row < p.m && k < p.k) {
-          xa[i][t] = ld8(p.x + row * p.k + k);
-          if constexpr (RMS) {
-            const half8 gv = ld8(p.gamma + k);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) xa[i][t][e] = rmsElem(xa[i][t][e], gv[e], rf);
-          }
-        }
-      }
+  }
+  // acc += x (the block's 4 operands) times the block
+  template <int RU>
+  __device__ __forceinline__ void multiply(const half8 (&x)[4], float (&acc)[W][RU], const Q4Masks& masks) const {
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const unsigned word[4] = {q[w].x, q[w].y, q[w].z, q[w].w};
 #pragma unroll
       for (int g = 0; g < PER; ++g) {
-        f32x4 d[MT];
+        f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < MT; ++t) d[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = g * G / 32; i < (g + 1) * G / 32; ++i)
+          d = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[i], q4Ints(word[i], masks), d, 0, 0, 0);
+        const float f = static_cast<float>(s[w][g]);
 #pragma unroll
-        for (int i = g * STEPS; i < (g + 1) * STEPS; ++i) {
-          const half8 b = q4Ints(word[i]);
-#pragma unroll
-          for (int t = 0; t < MT; ++t) d[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(xa[i][t], b, d[t], 0, 0, 0);
-        }
-        const float s = static_cast<float>(sc[w][g]);
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int r = 0; r < RU; ++r) acc[w][t][r] = fmaf(s, d[t][r], acc[w][t][r]);
+        for (int r = 0; r < RU; ++r) acc[w][r] = fmaf(f, d[r], acc[w][r]);
       }
     }
+  }
+};
+
+template <bool F32, int W>
+__device__ __forceinline__ void w4Put(const W4Params& p, int64_t row, int64_t col, const float (&y)[W]) {
+  if (row >= p.m || col >= p.n) return;
+  if constexpr (F32) {
+    static_cast<float*>(p.out)[row * p.n + col] = y[0];
+  } else {
+    float v = y[0];
+    if constexpr (W == 2) v = siluMul(y[0], y[W - 1]);
+    if (p.bias) v += static_cast<float>(p.bias[col]);
+    if (p.res) v = static_cast<float>(p.res[row * p.n + col]) + v;
+    static_cast<h16*>(p.out)[row * p.n + col] = toH16(v);
+  }
+}
+
+// Few tiles: the WAVES waves of a workgroup share one tile's k blocks (wave w takes w, w + WAVES, ..., U at a time, all loads
+// first) and their sums meet in LDS.
+template <int RU, int G, int W, bool F32, bool RMS, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void w4SplitKernel(W4Params p) {
+  const Q4Masks masks;
+  __shared__ float red[WAVES][W][RU][64];
+  constexpr int U = W == 2 ? 2 : 4;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = lane & 15, kq = lane >> 4;
+  const int64_t tile = blockIdx.x, row = 4 * (a & 3) + (a >> 2);
+  float acc[W][RU];
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int r = 0; r < RU; ++r) acc[w][r] = 0.0f;
+  float rf = 1.0f;
+  for (int64_t k0 = wave; k0 < p.kb; k0 += U * WAVES) {
+    W4Block<G, W> blk[U];
+    half8 x[U][4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) blk[u].load(p, tile, min<int64_t>(k0 + u * WAVES, p.kb - 1), lane);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t k = (k0 + u * WAVES) * 128 + 32 * i + 8 * kq;
+        x[u][i] = half8{};
+        if (row < p.m && k < p.k) x[u][i] = ld8(p.x + row * p.k + k);
+      }
+    if constexpr (RMS) {
+      if (k0 == wave) rf = rmsFactor(rowSumSq(p.x, p.k, lane), p.k, p.eps);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t k = (k0 + u * WAVES) * 128 + 32 * i + 8 * kq;
+          if (row < p.m && k < p.k) {
+            const half8 gv = ld8(p.gamma + k);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[u][i][e] = rmsElem(x[u][i][e], gv[e], rf);
+          }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + u * WAVES < p.kb) blk[u].multiply(x[u], acc, masks);
   }
 #pragma unroll
   for (int w = 0; w < W; ++w)
 #pragma unroll
-    for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int r = 0; r < RU; ++r) red[wave][w][t][r][lane] = acc[w][t][r];
+    for (int r = 0; r < RU; ++r) red[wave][w][r][lane] = acc[w][r];
   __syncthreads();
-  for (int o = threadIdx.x; o < MT * RU * 64; o += 64 * WAVES) {
-    const int l = o & 63, r = (o >> 6) % RU, t = (o >> 6) / RU;
-    const int64_t row = m0 + 16 * t + 4 * r + (l >> 4), col = tile * 16 + (l & 15);
-    if (row >= p.m || col >= p.n) continue;
+  for (int o = threadIdx.x; o < RU * 64; o += 64 * WAVES) {
+    const int l = o & 63, r = o >> 6;
     float y[W];
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       y[w] = 0.0f;
 #pragma unroll
-      for (int v = 0; v < WAVES; ++v) y[w] += red[v][w][t][r][l];
+      for (int v = 0; v < WAVES; ++v) y[w] += red[v][w][r][l];
     }
-    if constexpr (F32) {
-      static_cast<float*>(p.out)[row * p.n + col] = y[0];
-    } else {
-      float v = y[0];
-      if constexpr (W == 2) v = siluMul(y[0], y[W - 1]);
-      if (p.bias) v += static_cast<float>(p.bias[col]);
-      if (p.res) v = static_cast<float>(p.res[row * p.n + col]) + v;
-      static_cast<h16*>(p.out)[row * p.n + col] = toH16(v);
+    w4Put<F32, W>(p, 4 * r + (l >> 4), tile * 16 + (l & 15), y);
+  }
+}
+
+// Many tiles: x (normalized with RMS) goes to LDS once per workgroup, then each wave streams tiles of its own, U k blocks
+// ahead, over the tiles' ends.
+constexpr int kStreamPad = 32;  // halves between x's rows in LDS
+template <int RU, int G, int W, bool F32, bool RMS>
+__global__ __launch_bounds__(256) void w4StreamKernel(W4Params p) {
+  const Q4Masks masks;
+  extern __shared__ __attribute__((aligned(16))) h16 xs[];  // [M][kb 128 + kStreamPad]
+  constexpr int U = 4 / W;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = lane & 15, kq = lane >> 4;
+  const int64_t ld = p.kb * 128 + kStreamPad;
+  float rf = 1.0f;
+  if constexpr (RMS) rf = rmsFactor(rowSumSq(p.x, p.k, lane), p.k, p.eps);
+  for (int64_t i = threadIdx.x; i < p.m * p.kb * 16; i += 256) {
+    const int64_t row = i / (p.kb * 16), k = (i - row * p.kb * 16) * 8;
+    half8 v = {};
+    if (k < p.k) {
+      v = ld8(p.x + row * p.k + k);
+      if constexpr (RMS) {
+        const half8 gv = ld8(p.gamma + k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = rmsElem(v[e], gv[e], rf);
+      }
+    }
+    st8(xs + row * ld + k, v);
+  }
+  __syncthreads();
+  const int64_t tiles = (p.n + 15) / 16, step = static_cast<int64_t>(gridDim.x) * 4;
+  const int64_t batches = (p.kb + U - 1) / U;
+  // rows past M read row 0: their sums are not used
+  const int64_t rowOf = 4 * (a & 3) + (a >> 2);
+  const h16* xr = xs + (rowOf < p.m ? rowOf : 0) * ld + 8 * kq;
+  int64_t tile = blockIdx.x * 4 + wave;
+  if (tile >= tiles) return;
+  W4Block<G, W> blk[U];
+  const auto load = [&](int64_t t, int64_t b) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) blk[u].load(p, t, min<int64_t>(b * U + u, p.kb - 1), lane);
+  };
+  load(tile, 0);
+  for (; tile < tiles; tile += step) {
+    float acc[W][RU];
+#pragma unroll
+    for (int w = 0; w < W; ++w)
+#pragma unroll
+      for (int r = 0; r < RU; ++r) acc[w][r] = 0.0f;
+    for (int64_t b = 0; b < batches; ++b) {
+      W4Block<G, W> cur[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) cur[u] = blk[u];
+      if (b + 1 < batches) load(tile, b + 1);
+      else load(min(tile + step, tiles - 1), 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (b * U + u < p.kb) {
+          half8 x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = ld8(xr + (b * U + u) * 128 + 32 * i);
+          cur[u].multiply(x, acc, masks);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < RU; ++r) {
+      float y[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) y[w] = acc[w][r];
+      w4Put<F32, W>(p, 4 * r + kq, tile * 16 + a, y);
     }
   }
 }
 
 // More rows: workgroup of NW x KG waves, tile BM rows x NW 64 columns (SwiGLU: 32 of the gate's and the up weight's same 32).
-// Wave (nw, kg) takes all BM rows of its 64 columns over the k blocks kg, kg + KG, ...; the KG sums meet in LDS. x goes through
-// LDS in stages of 64 k, two buffers, filled from two register sets (a stage is loaded while the one before the last
-// runs); the weights go from memory straight into the registers of the one wave that multiplies by them, two tiles' words
-// being the B operands of 32x32x16 MFMAs: a lane's column is l % 32, its k 8 (l / 32) + 0 .. 7 of each 16, which are words of
-// lanes 16 (2 c + l / 32) + l % 16 of the column's tile, c the half of the 32 k. They are scaled before the product (exact), so
-// the sums run through all k.
+// Wave (nw, kg) takes all BM rows of its 64 columns over the k blocks kg, kg + KG, ... of 128 k; the KG sums meet in LDS. x goes
+// through LDS, a block ahead in registers; the weights go from memory straight into the registers of the one wave that
+// multiplies by them, two tiles' words being the B operands of 32x32x16 MFMAs: a lane's column is l % 32, its k 8 (l / 32) +
+// 0 .. 7 of each 16, which are words of lanes 16 (2 c + l / 32) + l % 16 of the column's tile, c the half of the 32 k. They are
+// scaled before the product (exact), so the sums run through all k. A block's 8 steps take c = 0 first, so that the next
+// block's words of one c are loaded while the other c's are used. Each step's operands are made during the MFMAs of the one
+// before.
 template <int BM, int NW, int KG, int G, int W, bool F32>
 __global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
+  const Q4Masks masks;
   constexpr int RB = BM / 32, THREADS = 64 * NW * KG, PER = 128 / G;
-  constexpr int STAGE = BM * 64;                 // halves of one k group's stage
-  constexpr int CH = BM * 8 / (64 * NW);         // its 16-byte chunks per thread of the group
-  constexpr int SMEM_A = 2 * KG * STAGE * 2, SMEM_R = KG > 1 ? KG * NW * BM * 64 * 4 : 0;
+  constexpr int BUF = NW == 1 ? 1 : 2;           // a wave alone orders its own stores and reads
+  constexpr int STAGE = BM * 128;                // halves of a k group's block
+  constexpr int CH = BM * 16 / (64 * NW);        // its 16-byte chunks per thread of the group
+  constexpr int SMEM_A = BUF * KG * STAGE * 2, SMEM_R = KG > 1 ? KG * NW * BM * 64 * 4 : 0;
   __shared__ __attribute__((aligned(16))) char smem[SMEM_A > SMEM_R ? SMEM_A : SMEM_R];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nw = wave % NW, kg = wave / NW, gt = threadIdx.x - kg * NW * 64;
   const int lr = lane & 31, lh = lane >> 5;
   const GridItem gi = xcdOrderYFast();
   const int64_t m0 = static_cast<int64_t>(gi.y) * BM, c0 = static_cast<int64_t>(gi.x) * NW * (W == 2 ? 32 : 64);
-  h16* as = reinterpret_cast<h16*>(smem) + kg * STAGE;  // buffer b at + b KG STAGE
-  // this wave's two blocks of 32 columns
+  h16* as = reinterpret_cast<h16*>(smem) + kg * BUF * STAGE;
+  // Addresses are a wave-uniform base and a lane's 32-bit offset in bytes. This wave's two blocks of 32 columns:
   const int64_t tiles = (p.n + 15) / 16;
-  const uint4* qp[2];
-  const h16* sp[2];
+  const char* qb[2];
+  const char* sb[2];
+  unsigned qo[2], so[2];
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int w = W == 2 ? j : 0;
-    const int64_t col = c0 + (W == 2 ? 32 * nw : 64 * nw + 32 * j);
-    const int64_t tile = min<int64_t>(col / 16 + ((lane >> 4) & 1), tiles - 1);
-    qp[j] = p.q[w] + tile * p.kb * 64 + (lane & 15) + 16 * lh;
-    sp[j] = p.s[w] + (tile * p.kb * 16 + (lane & 15)) * PER;
+    const int64_t tile = min<int64_t>((c0 + (W == 2 ? 32 * nw : 64 * nw + 32 * j)) / 16, tiles - 1);
+    const unsigned more = ((lane >> 4) & 1) && tile + 1 < tiles ? 1u : 0u;  // the lane's tile is this one or the next
+    qb[j] = reinterpret_cast<const char*>(p.q[w] + tile * p.kb * 64);
+    sb[j] = reinterpret_cast<const char*>(p.s[w] + tile * p.kb * 16 * PER);
+    qo[j] = more * static_cast<unsigned>(p.kb) * 1024u + ((lane & 15) + 16 * lh) * 16;
+    so[j] = (more * static_cast<unsigned>(p.kb) * 16u + (lane & 15)) * PER * 2;
   }
-  // x: chunk id = gt + 64 NW i -> row id / 8, k 8 (id % 8); 16-byte chunk c of row r lies at slot c ^ (r / 2 % 8)
-  const h16* xp[CH];
-  int xo[CH];
-  const int xc = 8 * (gt & 7);
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const int r = (gt + 64 * NW * i) >> 3;
-    xp[i] = p.x + min<int64_t>(m0 + r, p.m - 1) * p.k;
-    xo[i] = r * 64 + 8 * ((gt & 7) ^ ((r >> 1) & 7));
-  }
-  int fo[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) fo[q] = lr * 64 + 8 * ((2 * q + lh) ^ ((lr >> 1) & 7));
+  // x: chunk id = gt + 64 NW i -> row id / 16, k 8 (id % 16); 16-byte chunk c of row r lies at slot c ^ (r % 16), so that the
+  // rows of a fragment read, one chunk of each, fall on all banks
+  const char* xb = reinterpret_cast<const char*>(p.x + m0 * p.k);
+  constexpr int RP = 4 * NW;  // rows per chunk of all lanes
+  const int xc = 8 * (gt & 15), r0 = gt >> 4, s0 = (gt & 15) ^ (r0 & 15);
+  const unsigned xo = static_cast<unsigned>(r0) * static_cast<unsigned>(p.k) * 2u + xc * 2;
+  const int last = static_cast<int>(min<int64_t>(p.m - 1 - m0, BM - 1));  // the tile's last row
+  // (r0 + i RP) % 16 = r0 % 16 ^ i RP % 16: r0 < RP, a power of two
+  const auto slot = [&](int i) { return (r0 + i * RP) * 128 + 8 * (s0 ^ (i * RP & 15)); };
   const int blocks = static_cast<int>((p.kb + KG - 1) / KG);  // of every k group (the last may have one less)
-  half8 xr[2][CH];
-  // stage st of this k group: k block kg + (st / 2) KG, half st % 2
-  const auto kOf = [&](int st) { return (kg + static_cast<int64_t>(st >> 1) * KG) * 128 + 64 * (st & 1) + xc; };
-  const auto xload = [&](int st, int set) {
-    const int64_t k = min<int64_t>(kOf(st), p.k - 8);
+  half8 xr[CH];
+  // Block b of this k group starts at k = 128 (kg + b KG). In one that K ends in, a lane whose k lie behind K loads the row's
+  // last 8 and stores zeros; rows past M load the last row.
+  const auto kOf = [&](int b) { return (kg + static_cast<int64_t>(b) * KG) * 128; };
+  const auto xload = [&](int b) {
+    const int64_t k = kOf(b);
+    if (k + 128 <= p.k && last == BM - 1) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i) xr[set][i] = ld8(xp[i] + k);
-  };
-  const auto xstore = [&](int st, int set, int buf) {
-    const bool zero = kOf(st) >= p.k;
-    const half8 z = {};
+      for (int i = 0; i < CH; ++i)
+        xr[i] = *reinterpret_cast<const half8*>(xb + (k + static_cast<int64_t>(i) * RP * p.k) * 2 + xo);
+    } else {
+      const char* at = xb + min<int64_t>(k + xc, p.k - 8) * 2;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) st8(as + buf * KG * STAGE + xo[i], zero ? z : xr[set][i]);
-  };
-  uint4 q[2][2];
-  h16 sc[2][PER];
-  const auto wload = [&](int blk) {
-    const int64_t kb = min<int64_t>(kg + static_cast<int64_t>(blk) * KG, p.kb - 1);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      q[j][0] = qp[j][kb * 64];
-      q[j][1] = qp[j][kb * 64 + 32];
-#pragma unroll
-      for (int g = 0; g < PER; ++g) sc[j][g] = sp[j][kb * 16 * PER + g];
+      for (int i = 0; i < CH; ++i)
+        xr[i] = *reinterpret_cast<const half8*>(at + static_cast<unsigned>(min(r0 + i * RP, last)) * static_cast<unsigned>(p.k) * 2u);
     }
+  };
+  const auto xstore = [&](int b, int buf) {
+    const int64_t k = kOf(b);
+    if (k + 128 <= p.k) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i) st8(as + buf * STAGE + slot(i), xr[i]);
+    } else {
+      const half8 z = {};
+#pragma unroll
+      for (int i = 0; i < CH; ++i) st8(as + buf * STAGE + slot(i), k + xc < p.k ? xr[i] : z);
+    }
+  };
+  uint4 q[2][2];  // [column block][c]
+  h16 sc[2][PER], scNext[2][PER];
+  const auto kbOf = [&](int b) { return min<int64_t>(kg + static_cast<int64_t>(b) * KG, p.kb - 1); };
+  const auto wload = [&](int b, int c) {
+    const int64_t kb = kbOf(b);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) q[j][c] = *reinterpret_cast<const uint4*>(qb[j] + kb * 1024 + 512 * c + qo[j]);
+  };
+  const auto sload = [&](int b, h16 (&s)[2][PER]) {
+    const int64_t kb = kbOf(b);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < PER; ++g) s[j][g] = *reinterpret_cast<const h16*>(sb[j] + kb * 32 * PER + so[j] + 2 * g);
   };
   f32x16 acc[RB][2];
 #pragma unroll
@@ -277,75 +387,110 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-  xload(0, 0);
-  xload(1, 1);
-  wload(0);
-  xstore(0, 0, 0);
-  __syncthreads();
-  for (int b = 0; b < blocks; ++b) {
-    uint4 qc[2][2];
-    h16 cur[2][PER];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      qc[j][0] = q[j][0];
-      qc[j][1] = q[j][1];
-#pragma unroll
-      for (int g = 0; g < PER; ++g) cur[j][g] = sc[j][g];
-    }
-    wload(b + 1);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {  // stage 2 b + h, in buffer h
-      xload(2 * b + h + 2, h);
-      const h16* a = as + h * KG * STAGE;
-      if (KG == 1 || kg + b * KG < p.kb) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          half8 bf[2], af[RB];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint4 v = qc[j][s & 1];
-            const int i = 2 * h + (s >> 1);
-            const unsigned word = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-            const h16 f = cur[j][32 * i / G];
-            bf[j] = q4Ints(word) * half8{f, f, f, f, f, f, f, f};
-          }
-#pragma unroll
-          for (int i = 0; i < RB; ++i) af[i] = ld8(a + 32 * 64 * i + fo[s]);
-#pragma unroll
-          for (int i = 0; i < RB; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[i], bf[j], acc[i][j], 0, 0, 0);
-        }
-      }
-      xstore(2 * b + h + 1, h ^ 1, h ^ 1);
+  // With one wave to a k group the fences keep the compiler from moving its LDS stores and reads, which are served in
+  // order, across each other, and the waves run at their own pace.
+  const auto staged = [] {
+    if constexpr (NW == 1) {
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
       __syncthreads();
     }
-  }
-  // accumulator r of block (i, j): row 32 i + 8 (r / 4) + 4 lh + r % 4, column lr of column block j
-  const auto put = [&](int64_t row, int64_t col, float y) {
-    if (row >= p.m || col >= p.n) return;
-    if constexpr (F32) {
-      static_cast<float*>(p.out)[row * p.n + col] = y;
-    } else {
-      if (p.bias) y += static_cast<float>(p.bias[col]);
-      if (p.res) y = static_cast<float>(p.res[row * p.n + col]) + y;
-      static_cast<h16*>(p.out)[row * p.n + col] = toH16(y);
+  };
+  // step t: c = t / 4, 32-k piece i = t % 4 of the block
+  const auto operands = [&](const h16* a, int t, half8 (&af)[RB], half8 (&bf)[2]) {
+    const int c = t >> 2, i = t & 3;
+#pragma unroll
+    for (int r = 0; r < RB; ++r) af[r] = ld8(a + (32 * r + lr) * 128 + 8 * ((4 * i + 2 * c + lh) ^ (lr & 15)));
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint4 v = q[j][c];
+      const h16 f = sc[j][32 * i / G];
+      bf[j] = q4Ints(i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w, masks) * half8{f, f, f, f, f, f, f, f};
     }
   };
-  if constexpr (KG == 1) {
+  xload(0);
+  wload(0, 0);
+  wload(0, 1);
+  sload(0, sc);
+  xstore(0, 0);
+  staged();
+  for (int b = 0; b < blocks; ++b) {
+    const h16* a = as + (BUF == 2 ? b & 1 : 0) * STAGE;
+    xload(b + 1);
+    sload(b + 1, scNext);
+    if (KG == 1 || kg + b * KG < p.kb) {
+      half8 af[2][RB], bf[2][2];
+      operands(a, 0, af[0], bf[0]);
 #pragma unroll
-    for (int i = 0; i < RB; ++i)
+      for (int t = 0; t < 8; ++t) {
+        if (t < 7) operands(a, t + 1, af[(t + 1) & 1], bf[(t + 1) & 1]);
+        if (t == 3) wload(b + 1, 0);
+        if (t == 7) wload(b + 1, 1);
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[t & 1][i], bf[t & 1][j], acc[i][j], 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int g = 0; g < PER; ++g) sc[j][g] = scNext[j][g];
+    if (NW == 1) staged();
+    xstore(b + 1, BUF == 2 ? (b + 1) & 1 : 0);
+    staged();
+  }
+  if constexpr (NW == 1 && KG > 1) __syncthreads();  // the sums take the blocks' place
+  // What the epilogue adds (bias, residual) is loaded for many outputs at once, before their stores: a load behind a store
+  // waits for it.
+  const auto in = [&](int64_t row, int64_t col) { return row < p.m && col < p.n; };
+  const auto added = [&](int64_t row, int64_t col) {
+    if (F32 || !in(row, col)) return static_cast<h16>(0.0f);
+    return p.res ? p.res[row * p.n + col] : p.bias ? p.bias[col] : static_cast<h16>(0.0f);
+  };
+  const auto put = [&](int64_t row, int64_t col, float y, h16 add) {
+    if (!in(row, col)) return;
+    if constexpr (F32) static_cast<float*>(p.out)[row * p.n + col] = y;
+    else static_cast<h16*>(p.out)[row * p.n + col] = toH16(y + static_cast<float>(add));
+  };
+  const bool adds = W == 1 && (p.res || p.bias);
+  if constexpr (KG == 1) {
+    // accumulator r of block (i, j): row 32 i + 8 (r / 4) + 4 lh + r % 4, column lr of column block j
+#pragma unroll
+    for (int i = 0; i < RB; ++i) {
+      h16 add[16][2];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) add[r][0] = add[r][1] = static_cast<h16>(0.0f);
+      if (adds) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            add[r][j] = added(m0 + 32 * i + 8 * (r >> 2) + 4 * lh + (r & 3), c0 + 64 * nw + 32 * j + lr);
+      }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int64_t row = m0 + 32 * i + 8 * (r >> 2) + 4 * lh + (r & 3);
         if constexpr (W == 2) {
-          put(row, c0 + 32 * nw + lr, siluMul(acc[i][0][r], acc[i][1][r]));
+          put(row, c0 + 32 * nw + lr, siluMul(acc[i][0][r], acc[i][1][r]), add[r][0]);
         } else {
-          put(row, c0 + 64 * nw + lr, acc[i][0][r]);
-          put(row, c0 + 64 * nw + 32 + lr, acc[i][1][r]);
+          put(row, c0 + 64 * nw + lr, acc[i][0][r], add[r][0]);
+          put(row, c0 + 64 * nw + 32 + lr, acc[i][1][r], add[r][1]);
         }
       }
+    }
   } else {
+    // 4 columns of a row per item
+    constexpr int COLS = W == 2 ? 32 : 64, ITEMS = NW * BM * COLS / 4 / THREADS;
+    h16 add[ITEMS][4];
+#pragma unroll
+    for (int t = 0; t < ITEMS; ++t) {
+      const int o = threadIdx.x + t * THREADS, c = o % (COLS / 4) * 4, row = o / (COLS / 4) % BM, v = o / (COLS / 4 * BM);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) add[t][e] = adds ? added(m0 + row, c0 + v * COLS + c + e) : static_cast<h16>(0.0f);
+    }
     float* red = reinterpret_cast<float*>(smem);  // [KG][NW][BM][64]
 #pragma unroll
     for (int i = 0; i < RB; ++i)
@@ -355,17 +500,19 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
         for (int r = 0; r < 16; ++r)
           red[(wave * BM + 32 * i + 8 * (r >> 2) + 4 * lh + (r & 3)) * 64 + 32 * j + lr] = acc[i][j][r];
     __syncthreads();
-    constexpr int COLS = W == 2 ? 32 : 64;
-    for (int o = threadIdx.x; o < NW * BM * COLS; o += THREADS) {
-      const int c = o % COLS, row = o / COLS % BM, v = o / (COLS * BM);
-      float y = 0.0f, u = 0.0f;
+#pragma unroll
+    for (int t = 0; t < ITEMS; ++t) {
+      const int o = threadIdx.x + t * THREADS, c = o % (COLS / 4) * 4, row = o / (COLS / 4) % BM, v = o / (COLS / 4 * BM);
+      f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f}, u = y;
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
         const float* at = red + ((g * NW + v) * BM + row) * 64 + c;
-        y += at[0];
-        if (W == 2) u += at[32];
+        y += *reinterpret_cast<const f32x4*>(at);
+        if (W == 2) u += *reinterpret_cast<const f32x4*>(at + 32);
       }
-      put(m0 + row, c0 + v * COLS + c, W == 2 ? siluMul(y, u) : y);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        put(m0 + row, c0 + v * COLS + c + e, W == 2 ? siluMul(y[e], u[e]) : y[e], add[t][e]);
     }
   }
 }
@@ -379,11 +526,20 @@ bool groupOk(int g) { return g == 32 || g == 64 || g == 128; }
 int launched() { return hipGetLastError() == hipSuccess ? 0 : 2; }
 unsigned gridFor(int64_t threads) { return static_cast<unsigned>(std::min<int64_t>((threads + 255) / 256, 65536)); }
 
-template <int MT, int RU, int G, int W, bool F32, bool RMS>
-void launchSkinny(const lkd::W4Params& p, hipStream_t s) {
-  constexpr int WAVES = 4;
-  const dim3 grid(static_cast<unsigned>((p.n + 15) / 16), static_cast<unsigned>((p.m + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((lkd::w4SkinnyKernel<MT, RU, G, W, F32, RMS, WAVES>), grid, dim3(64 * WAVES), 0, s, p);
+template <int RU, int G, int W, bool F32, bool RMS>
+void launchFew(const lkd::W4Params& p, hipStream_t s) {
+  const int64_t tiles = (p.n + 15) / 16, lds = p.m * (p.kb * 128 + lkd::kStreamPad) * 2;
+  const char* f = getenv("LKQ4");
+  const int mode = f ? atoi(f) : 0;
+  const int64_t most = getenv("LKWG") ? atoi(getenv("LKWG")) : 1024;
+  if ((mode == 0 ? tiles >= 2048 : mode == 2) && lds <= 64 << 10) {
+    hipLaunchKernelGGL((lkd::w4StreamKernel<RU, G, W, F32, RMS>), dim3(static_cast<unsigned>(std::min<int64_t>((tiles + 3) / 4, most))),
+                       dim3(256), static_cast<size_t>(lds), s, p);
+  } else if (mode == 8) {
+    hipLaunchKernelGGL((lkd::w4SplitKernel<RU, G, W, F32, RMS, 8>), dim3(static_cast<unsigned>(tiles)), dim3(512), 0, s, p);
+  } else {
+    hipLaunchKernelGGL((lkd::w4SplitKernel<RU, G, W, F32, RMS, 4>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, s, p);
+  }
 }
 
 template <int BM, int NW, int KG, int G, int W, bool F32>
@@ -395,9 +551,9 @@ void launchGemm(const lkd::W4Params& p, hipStream_t s) {
 
 template <int G, int W, bool F32>
 void launchW4(const lkd::W4Params& p, hipStream_t s) {
-  if (p.gamma) launchSkinny<1, 1, G, W, F32, true>(p, s);
-  else if (p.m <= 4) launchSkinny<1, 1, G, W, F32, false>(p, s);
-  else if (p.m <= 16) launchSkinny<1, 4, G, W, F32, false>(p, s);
+  if (p.gamma) launchFew<1, G, W, F32, true>(p, s);
+  else if (p.m <= 4) launchFew<1, G, W, F32, false>(p, s);
+  else if (p.m <= 16 && !(getenv("LKQ4") && atoi(getenv("LKQ4")) == 9)) launchFew<4, G, W, F32, false>(p, s);
   else if (((p.m + 127) / 128) * ((p.n * W + 255) / 256) >= 256) launchGemm<128, 4, 1, G, W, F32>(p, s);
   else launchGemm<64, 1, 8, G, W, F32>(p, s);
 }
@@ -458,7 +614,7 @@ int lk_hip_w4_gemm(const void* x, const void* gamma, const void* q, const void* 
   if (f32_out && (bias || res)) return 1;
   if (gamma && (m > 1 || !al16(gamma))) return 1;
   if (m == 0) return 0;
-  if (m > 16 * 2 * 65535) return 1;
+  if (m > 64 * int64_t{65535} || k > (int64_t{1} << 23)) return 1;  // the grid; 32-bit offsets within 128 rows
   const W4Params p{static_cast<const h16*>(x), static_cast<const h16*>(gamma),
                    {static_cast<const uint4*>(q), static_cast<const uint4*>(q2)},
                    {static_cast<const h16*>(s), static_cast<const h16*>(s2)},
