@@ -52,18 +52,19 @@ __device__ __forceinline__ void kv4PutRow(half4 x, char* kvBlock, int64_t valueO
   if ((l & 7) == 0) *reinterpret_cast<h16*>(at + cap * 64 + (l >> 3) * 2 * cap + 2 * row) = static_cast<h16>(s);
 }
 
+// grid: rows / 4, kv heads
 __global__ __launch_bounds__(256) void kv4WriteKernel(char* __restrict__ kv, const h16* __restrict__ k,
                                                       const h16* __restrict__ v, const int64_t* __restrict__ pos,
-                                                      int64_t b, int64_t t, int kvh, int64_t cap) {
-  const int lane = threadIdx.x & 63;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (item >= b * t * kvh) return;
-  const int64_t seqRow = item / kvh, seq = seqRow / t, row = pos[seq] + (seqRow - seq * t);
-  const int h = static_cast<int>(item - seqRow * kvh);
+                                                      unsigned rows, unsigned t, int kvh, int64_t cap) {
+  const int lane = threadIdx.x & 63, h = blockIdx.y;
+  const unsigned r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows) return;
+  const unsigned seq = r / t;
+  const int64_t row = pos[seq] + (r - seq * t);
   if (row < 0 || row >= cap) return;  // uniform over the wave
-  const h16* src = (lane < 32 ? k : v) + seqRow * kvh * KHD + h * KHD + 4 * (lane & 31);
+  const h16* src = (lane < 32 ? k : v) + (static_cast<int64_t>(r) * kvh + h) * KHD + 4 * (lane & 31);
   const int64_t block = 72 * cap;
-  kv4PutRow(*reinterpret_cast<const half4*>(src), kv + (seq * 2 * kvh + h) * block, kvh * block, cap, row);
+  kv4PutRow(*reinterpret_cast<const half4*>(src), kv + (static_cast<int64_t>(seq) * 2 * kvh + h) * block, kvh * block, cap, row);
 }
 
 struct Kv4QkrParams {
@@ -73,22 +74,23 @@ struct Kv4QkrParams {
   const int64_t* pos;
   char* kv;
   h16* q;
-  int64_t b, t, cap;
+  unsigned rows, t;  // B T
+  int64_t cap;
   int qh, kvh;
   float eps;
   RopeTable tab;
 };
 
-// One wave per (row, q head) and (row, kv head): a q head is normalized and rotated to q, a kv head's key likewise and
+// One wave per (row, q head) and (row, kv head), grid rows / 4, heads: a q head is normalized and rotated to q, a kv head's key likewise and
 // quantised with its value. Arithmetic and roundings of the norm and the rotation as qkRopeKvKernel's.
 __global__ __launch_bounds__(256) void kv4QkRopeKernel(Kv4QkrParams p) {
   __shared__ __attribute__((aligned(16))) h16 rows[4][2 * KHD];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int slots = p.qh + p.kvh;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + wave;
-  if (item >= p.b * p.t * slots) return;
-  const int64_t r = item / slots, seq = r / p.t, row = p.pos[seq] + (r - seq * p.t);
-  const int slot = static_cast<int>(item - r * slots);
+  const int slot = blockIdx.y;
+  const unsigned ri = blockIdx.x * 4 + wave;
+  if (ri >= p.rows) return;
+  const unsigned seq = ri / p.t;
+  const int64_t r = ri, row = p.pos[seq] + (ri - seq * p.t);
   const int64_t width = static_cast<int64_t>(p.qh + 2 * p.kvh) * KHD;
   const bool isQ = slot < p.qh;
   if (!isQ && (row < 0 || row >= p.cap)) return;
@@ -115,27 +117,24 @@ __global__ __launch_bounds__(256) void kv4QkRopeKernel(Kv4QkrParams p) {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   const int64_t block = 72 * p.cap;
-  kv4PutRow(*reinterpret_cast<const half4*>(mine + 4 * lane), p.kv + (seq * 2 * p.kvh + (slot - p.qh)) * block,
+  kv4PutRow(*reinterpret_cast<const half4*>(mine + 4 * lane), p.kv + (static_cast<int64_t>(seq) * 2 * p.kvh + (slot - p.qh)) * block,
             p.kvh * block, p.cap, row);
 }
 
 // ---- reading ----------------------------------------------------------------------------------------------------
-// one thread per 8 values: blocks of 72 cap bytes -> f16 [blocks, cap, 128]
+// one thread per 8 values, grid cap 16 / 256, blocks: blocks of 72 cap bytes -> f16 [blocks, cap, 128]
 __global__ __launch_bounds__(256) void kv4ReadKernel(const char* __restrict__ kv, h16* __restrict__ out, int64_t blocks,
-                                                     int64_t cap) {
+                                                     unsigned cap) {
   const Q4Masks masks;
-  const int64_t total = blocks * cap * 16;
-  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
-       id += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t r = id >> 4, blk = r / cap, row = r - blk * cap;
-    const int w = static_cast<int>(id & 15);
+  for (int64_t blk = blockIdx.y; blk < blocks; blk += gridDim.y) {
     const char* at = kv + blk * 72 * cap;
-    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(at + row * 64 + 4 * w), masks);
-    const h16 s = *reinterpret_cast<const h16*>(at + cap * 64 + (w >> 2) * 2 * cap + 2 * row);
-    half8 y;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = v[e] * s;
-    st8(out + 8 * id, y);
+    h16* o = out + blk * cap * KHD;
+    for (unsigned id = blockIdx.x * 256 + threadIdx.x; id < cap * 16; id += gridDim.x * 256) {
+      const unsigned row = id >> 4, w = id & 15;
+      const h16 s = *reinterpret_cast<const h16*>(at + static_cast<int64_t>(cap) * (64 + (w >> 2) * 2) + 2 * row);
+      const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(at + static_cast<int64_t>(id) * 4), masks);
+      st8(o + static_cast<int64_t>(id) * 8, v * half8{s, s, s, s, s, s, s, s});
+    }
   }
 }
 
@@ -146,8 +145,9 @@ struct Kv4Params {
   const int64_t* pos;
   h16* out;
   float* part;  // [B T qh, splits, 130]: (max, sum, out[128]) of each workgroup's keys
-  int64_t b, t, cap;
-  int qh, kvh, splits;
+  int64_t cap;
+  unsigned t;
+  int qh, kvh, group, splits;  // group = qh / kvh
   float scale;  // log2(e) / sqrt(128)
   unsigned long long* err;
 };
@@ -169,16 +169,12 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
   __shared__ __attribute__((aligned(16))) float os[KW][16][KHD + 4];
   __shared__ float ms[KW][16], ls[KW][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 15, kq = lane >> 4;
-  const int group = p.qh / p.kvh;
-  const int64_t rowsHead = p.t * group, blocksHead = (rowsHead + 15) / 16;
-  int64_t id = blockIdx.x;
-  const int64_t rb = id % blocksHead;
-  id /= blocksHead;
-  const int kvHead = static_cast<int>(id % p.kvh);
-  const int64_t seq = id / p.kvh;
-  const int split = blockIdx.y;
+  const unsigned group = static_cast<unsigned>(p.group), rowsHead = p.t * group;
+  const unsigned split = blockIdx.x % static_cast<unsigned>(p.splits), rb = blockIdx.x / static_cast<unsigned>(p.splits);
+  const unsigned kvHead = blockIdx.y;
+  const int64_t seq = blockIdx.z;
   const int64_t p0 = p.pos[seq];
-  const int64_t row = rb * 16 + lc, rowIn = min<int64_t>(row, rowsHead - 1), qi = rowIn / group;
+  const unsigned rowIn = min(rb * 16 + lc, rowsHead - 1), qi = rowIn / group;
   const int64_t qAt = (seq * p.t + qi) * p.qh + kvHead * group + (rowIn - qi * group);  // of q and out, in heads
   half8 qf[4];
 #pragma unroll
@@ -186,7 +182,7 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
   const int cap = static_cast<int>(p.cap);
   // rows of the cache that the lane's row, and the block's last and first row, see
   const auto sees = [&](int64_t i) { return p0 < 0 ? 0 : static_cast<int>(min<int64_t>(p0 + i + 1, p.cap)); };
-  const int nkRow = sees(qi), nk = sees(min<int64_t>(rb * 16 + 15, rowsHead - 1) / group), nkAll = sees(rb * 16 / group);
+  const int nkRow = sees(qi), nk = sees(min(rb * 16 + 15, rowsHead - 1) / group), nkAll = sees(rb * 16 / group);
   if (split == 0 && rb == 0 && kvHead == 0 && threadIdx.x == 0 && (p0 < 0 || p0 + p.t > p.cap))
     raiseDeviceError(p.err, LK_DEVERR_POSITION, p0 < 0 ? p0 : p0 + p.t - 1);
   const int64_t block = 72 * p.cap;
@@ -302,19 +298,13 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
       }
     }
   };
-  int c = split * KW + wave;
-  if (c < chunks) {
-    Chunk cur = load(c);
-    for (; c + step < chunks; c += step) {
-      const Chunk next = load(c + step);
-      compute(c, cur);
-      cur = next;
-    }
-    compute(c, cur);
+  for (int c = static_cast<int>(split) * KW + wave; c < chunks; c += step) {
+    Chunk x = load(c);
+    compute(c, x);
   }
   // accumulator r of dim e: dim 8 (4 kq + r) + e of row l % 16
   l = crossRowSum(l);
-  const int rows = static_cast<int>(min<int64_t>(rowsHead - rb * 16, 16));
+  const int rows = static_cast<int>(min(rowsHead - rb * 16, 16u));
   if (lc < rows) {
     if (kq == 0) {
       ms[wave][lc] = m;
@@ -340,7 +330,8 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
       ll = fmaf(f, ls[w][r], ll);
       y = fmaf(f, os[w][r][d], y);
     }
-    const int64_t i = (rb * 16 + r) / group, at = (seq * p.t + i) * p.qh + kvHead * group + (rb * 16 + r - i * group);
+    const unsigned i = (rb * 16 + r) / group;
+    const int64_t at = (seq * p.t + i) * p.qh + kvHead * group + (rb * 16 + r - i * group);
     if (p.splits == 1) {
       const bool noRow = p0 < 0 || p0 + i >= p.cap;
       p.out[at * KHD + d] = noRow ? static_cast<h16>(__builtin_nanf("")) : toH16(y / ll);
@@ -355,10 +346,11 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
   }
 }
 
-// one workgroup per (query, q head): the splits' partials, 32 at a time
+// one workgroup per (q head, query): the splits' partials, 32 at a time
 __global__ __launch_bounds__(128) void kv4MergeKernel(Kv4Params p) {
   const int d = threadIdx.x;
-  const int64_t at = blockIdx.x, qi = at / p.qh, seq = qi / p.t, p0 = p.pos[seq];
+  const unsigned qi = blockIdx.y, seq = qi / p.t;
+  const int64_t at = static_cast<int64_t>(qi) * p.qh + blockIdx.x, p0 = p.pos[seq];
   const bool noRow = p0 < 0 || p0 + (qi - seq * p.t) >= p.cap;
   const float* part = p.part + at * p.splits * (KHD + 2);
   float m = -INFINITY, l = 0.0f, o = 0.0f;
@@ -389,21 +381,21 @@ __global__ __launch_bounds__(128) void kv4MergeKernel(Kv4Params p) {
 }
 
 // Many rows: the rows 0 .. pos + T - 1 of one sequence as f16 [P, kvh 128], keys then values, for the f16 tiles of
-// lk_hip_f16_attention_gqa: they are dequantised once instead of by every block of queries. 8 values per thread.
+// lk_hip_f16_attention_gqa: they are dequantised once instead of by every block of queries. 8 values per thread, grid
+// rows 16 / 256, kv heads, 2.
 __global__ __launch_bounds__(256) void kv4ExpandKernel(const char* __restrict__ kv, const int64_t* __restrict__ pos,
-                                                       h16* __restrict__ out, int64_t t, int kvh, int64_t cap) {
+                                                       h16* __restrict__ out, unsigned t, int kvh, unsigned cap) {
   const Q4Masks masks;
-  const int64_t p0 = *pos, rows = p0 < 0 ? 0 : min<int64_t>(p0 + t, cap), per = static_cast<int64_t>(kvh) * 16;
-  const char* base = kv + blockIdx.y * kvh * 72 * cap;
-  h16* o = out + blockIdx.y * cap * kvh * KHD;
-  for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < rows * per;
-       id += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t row = id / per;
-    const int at = static_cast<int>(id - row * per), w = at & 15;
-    const char* blk = base + (at >> 4) * 72 * cap;
-    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(blk + row * 64 + 4 * w), masks);
-    const h16 s = *reinterpret_cast<const h16*>(blk + cap * 64 + (w >> 2) * 2 * cap + 2 * row);
-    st8(o + id * 8, v * half8{s, s, s, s, s, s, s, s});
+  const int64_t p0 = *pos;
+  const unsigned rows = p0 < 0 ? 0 : static_cast<unsigned>(min<int64_t>(p0 + t, cap));
+  const unsigned h = blockIdx.y;
+  const char* at = kv + (static_cast<int64_t>(blockIdx.z) * kvh + h) * 72 * cap;
+  h16* o = out + static_cast<int64_t>(blockIdx.z) * cap * kvh * KHD + h * KHD;
+  for (unsigned id = blockIdx.x * 256 + threadIdx.x; id < rows * 16; id += gridDim.x * 256) {
+    const unsigned row = id >> 4, w = id & 15;
+    const h16 s = *reinterpret_cast<const h16*>(at + static_cast<int64_t>(cap) * (64 + (w >> 2) * 2) + 2 * row);
+    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(at + static_cast<int64_t>(id) * 4), masks);
+    st8(o + static_cast<int64_t>(row) * kvh * KHD + 8 * w, v * half8{s, s, s, s, s, s, s, s});
   }
 }
 
@@ -466,19 +458,22 @@ namespace {
 bool al16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
 bool al8(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 7) == 0; }
 int launched() { return hipGetLastError() == hipSuccess ? 0 : 2; }
+constexpr int64_t kMostRows = int64_t{1} << 27;  // of a cache: a row's 16 words and a chunk of 64 rows fit 32 bits
 bool kvOk(const void* kv, int64_t b, int kvh, int64_t cap) {
-  return b > 0 && kvh > 0 && cap > 0 && cap % 32 == 0 && al16(kv);
+  return b > 0 && kvh > 0 && kvh <= 65535 && cap > 0 && cap % 32 == 0 && cap <= kMostRows && al16(kv);
 }
+// rows of a call: they are counted in 32 bits
+bool rowsOk(int64_t b, int64_t t) { return t >= 0 && t <= 0x7FFFFFFF && b <= 65535 && b * t <= 0x7FFFFFFF; }
 
 // Many rows: expanded to f16 once
 bool kv4Expands(int64_t t, int64_t group) { return t > 1 && t * group > 32; }
 
 int kv4Splits(int64_t b, int64_t t, int qh, int kvh, int64_t cap) {
   const int64_t groups = b * kvh * ((t * (qh / kvh) + 15) / 16);
-  const char* f = getenv("LKSP");
-  if (f) return atoi(f);
+
+
   if (cap <= 2048 || groups >= 256) return 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((cap + 511) / 512, 512 / groups)));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((cap + 511) / 512, 256 / groups)));
 }
 
 }  // namespace
@@ -488,38 +483,36 @@ extern "C" {
 int lk_hip_kv4_write(void* kv, const void* k, const void* v, const int64_t* pos, int64_t b, int64_t t, int kvh, int64_t cap,
                      void* stream) {
   using namespace lkd;
-  if (!kvOk(kv, b, kvh, cap) || t < 0 || !al8(k) || !al8(v)) return 1;
-  const int64_t items = b * t * kvh;
-  if (items == 0) return 0;
-  if (items > int64_t{4} * 0x7FFFFFFF) return 1;
-  hipLaunchKernelGGL(kv4WriteKernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0,
+  if (!kvOk(kv, b, kvh, cap) || !rowsOk(b, t) || !al8(k) || !al8(v)) return 1;
+  if (t == 0) return 0;
+  hipLaunchKernelGGL(kv4WriteKernel, dim3(static_cast<unsigned>((b * t + 3) / 4), static_cast<unsigned>(kvh)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), static_cast<char*>(kv), static_cast<const h16*>(k),
-                     static_cast<const h16*>(v), pos, b, t, kvh, cap);
+                     static_cast<const h16*>(v), pos, static_cast<unsigned>(b * t), static_cast<unsigned>(t), kvh, cap);
   return launched();
 }
 
 int lk_hip_kv4_qknorm_rope(const void* qkv, const void* qg, const void* kg, const int64_t* pos, void* kv, void* q, int64_t b,
                            int64_t t, int qh, int kvh, int64_t cap, float eps, float theta, void* stream) {
   using namespace lkd;
-  if (!kvOk(kv, b, kvh, cap) || t < 0 || qh <= 0 || !al16(qkv)) return 1;
-  const int64_t items = b * t * (qh + kvh);
-  if (items == 0) return 0;
-  if (items > int64_t{4} * 0x7FFFFFFF) return 1;
+  if (!kvOk(kv, b, kvh, cap) || !rowsOk(b, t) || qh <= 0 || !al16(qkv)) return 1;
+  if (t == 0) return 0;
+  if (qh + kvh > 65535) return 1;
   Kv4QkrParams p{static_cast<const h16*>(qkv), static_cast<const h16*>(qg), static_cast<const h16*>(kg), pos,
-                 static_cast<char*>(kv), static_cast<h16*>(q), b, t, cap, qh, kvh, eps, {}};
+                 static_cast<char*>(kv), static_cast<h16*>(q), static_cast<unsigned>(b * t), static_cast<unsigned>(t), cap, qh, kvh,
+                 eps, {}};
   for (int j = 0; j < 64; ++j) p.tab.invf[j] = 1.0f / std::pow(theta, static_cast<float>(2 * j) / 128.0f);
-  hipLaunchKernelGGL(kv4QkRopeKernel, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(256), 0,
+  hipLaunchKernelGGL(kv4QkRopeKernel, dim3(static_cast<unsigned>((b * t + 3) / 4), static_cast<unsigned>(qh + kvh)), dim3(256), 0,
                      static_cast<hipStream_t>(stream), p);
   return launched();
 }
 
 int lk_hip_kv4_read(const void* kv, void* out, int64_t blocks, int64_t cap, void* stream) {
   using namespace lkd;
-  if (blocks < 0 || cap <= 0 || cap % 32 != 0 || !al16(kv) || !al16(out)) return 1;
+  if (blocks < 0 || cap <= 0 || cap % 32 != 0 || cap > kMostRows || !al16(kv) || !al16(out)) return 1;
   if (blocks == 0) return 0;
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((blocks * cap * 16 + 255) / 256, 65536));
-  hipLaunchKernelGGL(kv4ReadKernel, dim3(grid), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const char*>(kv),
-                     static_cast<h16*>(out), blocks, cap);
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cap / 16, 256)), static_cast<unsigned>(std::min<int64_t>(blocks, 65535)));
+  hipLaunchKernelGGL(kv4ReadKernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const char*>(kv),
+                     static_cast<h16*>(out), blocks, static_cast<unsigned>(cap));
   return launched();
 }
 
@@ -533,17 +526,17 @@ int64_t lk_hip_kv4_attention_workspace_bytes(int64_t b, int64_t t, int qh, int k
 int lk_hip_kv4_attention(const void* q, const void* kv, const int64_t* pos, void* out, int64_t b, int64_t t, int qh, int kvh,
                          int64_t cap, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace lkd;
-  if (!kvOk(kv, b, kvh, cap) || t < 0 || qh <= 0 || qh % kvh != 0 || !al16(q)) return 1;
+  if (!kvOk(kv, b, kvh, cap) || !rowsOk(b, t) || qh <= 0 || qh % kvh != 0 || !al16(q)) return 1;
   if (t == 0) return 0;
   const int64_t need = lk_hip_kv4_attention_workspace_bytes(b, t, qh, kvh, cap);
   if (need > 0 && (!workspace || workspace_bytes < need || !al16(workspace))) return 3;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (kv4Expands(t, qh / kvh)) {
     h16* rows = static_cast<h16*>(workspace);
-    const unsigned gx = static_cast<unsigned>(std::min<int64_t>((cap * kvh * 16 + 255) / 256, 2048));
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cap / 16, 256)), static_cast<unsigned>(kvh), 2);
     for (int64_t i = 0; i < b; ++i) {  // one sequence after the other through the same rows
-      hipLaunchKernelGGL(kv4ExpandKernel, dim3(gx, 2), dim3(256), 0, s,
-                         static_cast<const char*>(kv) + i * 2 * kvh * 72 * cap, pos + i, rows, t, kvh, cap);
+      hipLaunchKernelGGL(kv4ExpandKernel, grid, dim3(256), 0, s, static_cast<const char*>(kv) + i * 2 * kvh * 72 * cap, pos + i,
+                         rows, static_cast<unsigned>(t), kvh, static_cast<unsigned>(cap));
       const int rc = lk_hip_f16_attention_gqa(static_cast<const h16*>(q) + i * t * qh * KHD, rows, rows + cap * kvh * KHD,
                                               pos + i, static_cast<h16*>(out) + i * t * qh * KHD, t, qh, kvh, cap, nullptr, 0,
                                               stream);
@@ -553,13 +546,14 @@ int lk_hip_kv4_attention(const void* q, const void* kv, const int64_t* pos, void
   }
   const int splits = kv4Splits(b, t, qh, kvh, cap);
   const Kv4Params p{static_cast<const h16*>(q), static_cast<const char*>(kv), pos, static_cast<h16*>(out),
-                    static_cast<float*>(workspace), b, t, cap, qh, kvh, splits,
+                    static_cast<float*>(workspace), cap, static_cast<unsigned>(t), qh, kvh, qh / kvh, splits,
                     kLog2e / std::sqrt(static_cast<float>(KHD)), lkh::deviceErrorRecord()};
-  const int64_t blocks = b * kvh * ((t * (qh / kvh) + 15) / 16);
-  if (blocks > 0x7FFFFFFF || b * t * qh > 0x7FFFFFFF || cap > 0x7FFFFFFF - 64) return 1;
-  hipLaunchKernelGGL(kv4DecodeKernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(splits)), dim3(64 * KW), 0, s, p);
+  const int64_t blocks = (t * (qh / kvh) + 15) / 16 * splits;
+  if (t * (qh / kvh) > 0x7FFFFFFF || blocks > 0x7FFFFFFF || (splits > 1 && b * t > 65535)) return 1;
+  hipLaunchKernelGGL(kv4DecodeKernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(kvh), static_cast<unsigned>(b)),
+                     dim3(64 * KW), 0, s, p);
   if (splits > 1)
-    hipLaunchKernelGGL(kv4MergeKernel, dim3(static_cast<unsigned>(b * t * qh)), dim3(128), 0, s, p);
+    hipLaunchKernelGGL(kv4MergeKernel, dim3(static_cast<unsigned>(qh), static_cast<unsigned>(b * t)), dim3(128), 0, s, p);
   return launched();
 }
 

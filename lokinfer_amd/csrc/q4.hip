@@ -529,17 +529,16 @@ unsigned gridFor(int64_t threads) { return static_cast<unsigned>(std::min<int64_
 template <int RU, int G, int W, bool F32, bool RMS>
 void launchFew(const lkd::W4Params& p, hipStream_t s) {
   const int64_t tiles = (p.n + 15) / 16, lds = p.m * (p.kb * 128 + lkd::kStreamPad) * 2;
-  const char* f = getenv("LKQ4");
-  const int mode = f ? atoi(f) : 0;
-  const int64_t most = getenv("LKWG") ? atoi(getenv("LKWG")) : 1024;
-  if ((mode == 0 ? tiles >= 2048 : mode == 2) && lds <= 64 << 10) {
-    hipLaunchKernelGGL((lkd::w4StreamKernel<RU, G, W, F32, RMS>), dim3(static_cast<unsigned>(std::min<int64_t>((tiles + 3) / 4, most))),
+  // us, split over 4 / 8 waves against streamed (M = 1, G = 64): K = 2048, N = 4096 3.9 / 4.2 / 6.9; 16384 7.4 / 8.5 / 7.6;
+  // 32768 11.2 / 14.2 / 10.3; 65536 19.2 / 27.0 / 16.6; K = 6144, N = 2048 7.3 / 6.2 / 15.4; 8192 9.8 / 10.0 / 15.3; 32768
+  // 27.4 / 30.1 / 22.1
+  if (tiles >= 1536 && lds <= 128 << 10)
+    hipLaunchKernelGGL((lkd::w4StreamKernel<RU, G, W, F32, RMS>), dim3(static_cast<unsigned>(std::min<int64_t>((tiles + 3) / 4, 1024))),
                        dim3(256), static_cast<size_t>(lds), s, p);
-  } else if (mode == 8) {
+  else if (p.kb >= 32 && tiles <= 512)
     hipLaunchKernelGGL((lkd::w4SplitKernel<RU, G, W, F32, RMS, 8>), dim3(static_cast<unsigned>(tiles)), dim3(512), 0, s, p);
-  } else {
+  else
     hipLaunchKernelGGL((lkd::w4SplitKernel<RU, G, W, F32, RMS, 4>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, s, p);
-  }
 }
 
 template <int BM, int NW, int KG, int G, int W, bool F32>
@@ -553,7 +552,7 @@ template <int G, int W, bool F32>
 void launchW4(const lkd::W4Params& p, hipStream_t s) {
   if (p.gamma) launchFew<1, G, W, F32, true>(p, s);
   else if (p.m <= 4) launchFew<1, G, W, F32, false>(p, s);
-  else if (p.m <= 16 && !(getenv("LKQ4") && atoi(getenv("LKQ4")) == 9)) launchFew<4, G, W, F32, false>(p, s);
+  else if (p.m <= 16) launchFew<4, G, W, F32, false>(p, s);
   else if (((p.m + 127) / 128) * ((p.n * W + 255) / 256) >= 256) launchGemm<128, 4, 1, G, W, F32>(p, s);
   else launchGemm<64, 1, 8, G, W, F32>(p, s);
 }

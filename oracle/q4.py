@@ -5,37 +5,29 @@ from __future__ import annotations
 import numpy as np
 
 
-def scale_of(hi: float, lo: float) -> float:
-    """The smallest f16 of at most 8 significant bits with 7 s >= hi and 8 s >= -lo, at most 8128 (hi >= 0 >= lo), found by
-    search from the exact conditions."""
-    if hi == 0 and lo == 0:
-        return 0.0
-    a = max(hi / 7, -lo / 8)
-    e = max(int(np.floor(np.log2(a))) - 8, -24)  # one bit lower than needed: the search walks up
-    m = max(int(np.floor(a / 2.0 ** e)) - 2, 0)
-    while True:
-        s = m * 2.0 ** e
-        odd = m
-        while odd and odd % 2 == 0:
-            odd //= 2
-        if odd < 256 and 7 * s >= hi and 8 * s >= -lo:
-            return min(s, 8128.0)
-        m += 1
+def scale_of(hi, lo):
+    """The smallest f16 of at most 8 significant bits with 7 s >= hi and 8 s >= -lo, at most 8128 (hi >= 0 >= lo, f64
+    arrays): the first of a few neighbours of max(hi / 7, -lo / 8) on that grid that meets the conditions, which f64
+    products decide exactly."""
+    a = np.maximum(hi / 7, -lo / 8)
+    step = np.exp2(np.maximum(np.floor(np.log2(np.where(a > 0, a, 1.0))) - 7, -24))
+    s = np.full(a.shape, np.inf)
+    for m in range(2, -3, -1):  # the last that holds is the smallest
+        t = (np.ceil(a / step) + m) * step
+        odd = t / step <= 256  # 256 steps are 128 of the next size
+        s = np.where((t >= 0) & odd & (7 * t >= hi) & (8 * t >= -lo), t, s)
+    return np.where(a > 0, np.minimum(s, 8128.0), 0.0)
 
 
 def quantize(x: np.ndarray):
     """x f16[..., G] -> (codes int[..., G], scales f64[...]); a group that is not finite: scale NaN, codes 8."""
-    flat = np.asarray(x, np.float64).reshape(-1, x.shape[-1])
-    codes = np.full(flat.shape, 8, np.int64)
-    scales = np.zeros(len(flat))
-    for i, g in enumerate(flat):
-        if not np.isfinite(g).all():
-            scales[i] = np.nan
-            continue
-        s = scales[i] = scale_of(max(g.max(), 0.0), min(g.min(), 0.0))
-        if s > 0:
-            codes[i] = 8 + np.clip(np.floor(g / s + 0.5), -8, 7).astype(np.int64)
-    return codes.reshape(x.shape), scales.reshape(x.shape[:-1])
+    x = np.asarray(x, np.float64)
+    ok = np.isfinite(x).all(-1)
+    g = np.where(ok[..., None], x, 0.0)
+    s = scale_of(np.maximum(g.max(-1), 0.0), np.minimum(g.min(-1), 0.0))
+    c = np.floor(g / np.where(s > 0, s, 1.0)[..., None] + 0.5)
+    codes = 8 + np.where(s[..., None] > 0, np.clip(c, -8, 7), 0).astype(np.int64)
+    return codes, np.where(ok, s, np.nan)
 
 
 def weight_values(w: np.ndarray, group: int) -> np.ndarray:

@@ -111,3 +111,21 @@ def test_oracle_quantizer_is_exact_in_f16_and_off_by_half_a_step():
     assert (v.astype(np.float16).astype(np.float64) == v).all()
     over = np.abs(x.astype(np.float64)) > 56896
     assert (np.abs(v - x.astype(np.float64))[~over] <= (np.broadcast_to(s[:, None], v.shape) / 2)[~over]).all()
+
+
+def test_oracle_scale_is_the_smallest_that_holds():
+    """Against every f16 of at most 8 significant bits."""
+    every = np.arange(0x7C00, dtype=np.uint16).view(np.float16).astype(np.float64)
+    m = np.round(every * 2.0 ** 24).astype(np.int64)
+    odd = m // np.maximum(m & -m, 1)
+    grid = every[(odd < 256) & (every <= 8128)]
+    r = np.random.default_rng(2)
+    hi = (np.abs(r.standard_normal(4000)) * np.exp2(r.uniform(-26, 15, 4000))).clip(0, 65504).astype(np.float16)
+    lo = (-np.abs(r.standard_normal(4000)) * np.exp2(r.uniform(-26, 15, 4000))).clip(-65504, 0).astype(np.float16)
+    lo[::5] = 0
+    hi[::7] = (grid[r.integers(0, len(grid), len(hi[::7]))] * 7).clip(0, 65504).astype(np.float16)  # scales that fit exactly
+    hi, lo = hi.astype(np.float64), lo.astype(np.float64)
+    got = O.scale_of(hi, lo)
+    for h, l, s in zip(hi, lo, got):
+        fits = grid[(7 * grid >= h) & (8 * grid >= -l)]
+        assert s == (fits[0] if len(fits) else 8128.0), (h, l, s)

@@ -90,7 +90,9 @@ def product(x, w):
 W4_CASES = [(1, 2048, 4096, 64), (1, 8, 1, 32), (1, 136, 17, 128), (1, 6144, 48, 128), (2, 2048, 96, 64), (4, 72, 40, 32),
             (5, 1000, 777, 32), (16, 264, 33, 64), (17, 2048, 31, 128), (33, 512, 65, 32), (64, 640, 200, 64),
             (65, 520, 200, 128), (100, 200, 300, 32), (130, 1032, 130, 64), (257, 2048, 96, 32), (409, 384, 515, 128),
-            (1030, 136, 260, 64)]
+            (1030, 136, 260, 64),
+            # many columns: weights streamed by persistent waves, x in LDS; 2048 x 16 rows of it are more than 64 KiB
+            (1, 264, 32770, 64), (3, 40, 24600, 32), (7, 136, 25000, 128), (16, 2048, 24583, 128)]
 
 
 @pytest.mark.parametrize("m,k,n,group", W4_CASES)
@@ -122,11 +124,10 @@ def test_no_rows_give_no_rows(gpu):
     assert q4.gemm_w4_f16_gpu(G(lk, np.zeros((0, 64), np.float16)), p).shape == (0, 20)
 
 
-@pytest.mark.parametrize("m", [1, 4, 70])
-def test_rmsnorm_in_front_is_the_norm_and_the_product(gpu, m):
+@pytest.mark.parametrize("m,k,n", [(1, 2048, 112), (4, 2048, 112), (70, 2048, 112), (1, 6144, 40), (1, 520, 33000)])
+def test_rmsnorm_in_front_is_the_norm_and_the_product(gpu, m, k, n):
     lk, q4, F = gpu, gpu.ops.q4_gpu, gpu.ops.f16_gpu
     r = rng_of(4, m)
-    k, n = 2048, 112
     x, g = G(lk, r.standard_normal((m, k)).astype(np.float16)), G(lk, (1 + r.standard_normal(k) / 9).astype(np.float16))
     a, b = (q4.pack_w4((r.standard_normal((k, n)) / 45).astype(np.float16)) for _ in range(2))
     h = F.rmsnorm_f16_gpu(x, g)
