@@ -343,8 +343,10 @@ int64_t lk_hip_w4_scales_bytes(int64_t n, int64_t k, int group);
 /* w f16[K, N] (nt: [N, K]) -> q, s: the smallest scale with 7 s >= the group's largest and 8 s >= minus its smallest value
  * (at most 8128), codes rounded to nearest, halves up. A group with a value that is not finite becomes NaN. */
 int lk_hip_w4_quantize(const void* w, void* q, void* s, int64_t n, int64_t k, int group, int nt, void* stream);
-/* codes u8[K, N] (low 4 bits), scales f16[ceil(K / group), N] -> q, s */
-int lk_hip_w4_pack(const void* codes, const void* scales, void* q, void* s, int64_t n, int64_t k, int group, void* stream);
+/* codes u8[K, N], scales f16[ceil(K / group), N] -> q, s; flag (device, zero before): | 1 where a code is over 15 (its low 4
+ * bits are taken), | 2 where a scale is negative, over 8128, not a number or of more than 8 significant bits */
+int lk_hip_w4_pack(const void* codes, const void* scales, void* q, void* s, int* flag, int64_t n, int64_t k, int group,
+                   void* stream);
 /* q, s -> w f16[K, N], exact */
 int lk_hip_w4_unpack(const void* q, const void* s, void* w, int64_t n, int64_t k, int group, void* stream);
 /* out [M, N] = x f16[M, K] @ W (f32 sums): f16, + bias f16[N], + res f16[M, N]; silu(x @ W) * (x @ W2) with q2, s2; f32

@@ -24,10 +24,10 @@ struct W4Layout {
   int group;
 };
 
-// one thread per (column of a tile, group): MODE 0 from w f16[K, N], 1 from w f16[N, K], 2 from codes u8[K, N] and scales
-template <int MODE>
-__global__ __launch_bounds__(256) void w4PackKernel(const void* __restrict__ src, const h16* __restrict__ scales,
-                                                    unsigned* __restrict__ q, h16* __restrict__ s, W4Layout p) {
+// one thread per (column of a tile, group): from w f16[K, N], or NT f16[N, K]
+template <bool NT>
+__global__ __launch_bounds__(256) void w4QuantizeKernel(const h16* __restrict__ w, unsigned* __restrict__ q,
+                                                        h16* __restrict__ s, W4Layout p) {
   const int per = 128 / p.group;
   const int64_t cols = (p.n + 15) / 16 * 16, total = cols * p.kb * per;
   for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
@@ -36,37 +36,63 @@ __global__ __launch_bounds__(256) void w4PackKernel(const void* __restrict__ src
     const int gb = static_cast<int>(gi - kb * per);
     const int64_t k0 = gi * p.group;
     const int live = n < p.n ? static_cast<int>(max<int64_t>(0, min<int64_t>(p.group, p.k - k0))) : 0;
-    const h16* w = static_cast<const h16*>(src);
-    float sc = 0.0f;
-    if (MODE == 2) {
-      if (live) sc = static_cast<float>(scales[gi * p.n + n]);
-    } else {
-      float hi = 0.0f, lo = 0.0f;
-      bool bad = false;
-      for (int j = 0; j < live; ++j) {
-        const float v = static_cast<float>(MODE == 0 ? w[(k0 + j) * p.n + n] : w[n * p.k + k0 + j]);
-        hi = fmaxf(hi, v);
-        lo = fminf(lo, v);
-        bad = bad || !(fabsf(v) < INFINITY);
-      }
-      sc = bad ? __builtin_nanf("") : q4Scale(hi, lo);
+    const auto at = [&](int j) { return static_cast<float>(NT ? w[n * p.k + k0 + j] : w[(k0 + j) * p.n + n]); };
+    float hi = 0.0f, lo = 0.0f;
+    bool bad = false;
+    for (int j = 0; j < live; ++j) {
+      const float v = at(j);
+      hi = fmaxf(hi, v);
+      lo = fminf(lo, v);
+      bad = bad || !(fabsf(v) < INFINITY);
     }
+    const float sc = bad ? __builtin_nanf("") : q4Scale(hi, lo);
     const int64_t tile = (n >> 4) * p.kb + kb;
     s[(tile * 16 + (n & 15)) * per + gb] = static_cast<h16>(sc);
     for (int o = 0; o < p.group / 8; ++o) {
       unsigned word = 0;
-      for (int j = 0; j < 8; ++j) {
-        const int at = 8 * o + j;
-        unsigned c = 8u;
-        if (at < live) {
-          const int64_t k = k0 + at;
-          if (MODE == 2) c = static_cast<const uint8_t*>(src)[k * p.n + n] & 15u;
-          else c = q4Code(static_cast<float>(MODE == 0 ? w[k * p.n + n] : w[n * p.k + k]), sc);
-        }
-        word |= c << q4Shift(j);
-      }
+      for (int j = 0; j < 8; ++j) word |= (8 * o + j < live ? q4Code(at(8 * o + j), sc) : 8u) << q4Shift(j);
       const int in = gb * p.group + 8 * o;  // k within the tile
       q[(tile * 64 + (n & 15) + 16 * ((in >> 3) & 3)) * 4 + (in >> 5)] = word;
+    }
+  }
+}
+
+// Given codes and scales: one thread per (column, 8 of each 32 k of a tile), grid columns / 64, k blocks. What is no code or no
+// scale sets a flag: 1 a code over 15, 2 a scale that is negative, over 8128 or not a number, or has more than 8 bits.
+__global__ __launch_bounds__(256) void w4PackKernel(const uint8_t* __restrict__ codes, const h16* __restrict__ scales,
+                                                    uint4* __restrict__ q, h16* __restrict__ s, int* __restrict__ flag,
+                                                    W4Layout p) {
+  const int per = 128 / p.group, kq = threadIdx.x >> 6;
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 64 + (threadIdx.x & 63), tiles = (p.n + 15) / 16;
+  if (n >= tiles * 16) return;
+  for (int64_t kb = blockIdx.y; kb < p.kb; kb += gridDim.y) {
+    unsigned c[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t k = kb * 128 + 32 * i + 8 * kq + j;
+        c[i][j] = n < p.n && k < p.k ? codes[k * p.n + n] : 8u;
+      }
+    unsigned word[4] = {0u, 0u, 0u, 0u}, all = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        word[i] |= (c[i][j] & 15u) << q4Shift(j);
+        all |= c[i][j];
+      }
+    if (all > 15u) atomicOr(flag, 1);
+    const int64_t tile = (n >> 4) * p.kb + kb;
+    q[tile * 64 + (n & 15) + 16 * kq] = make_uint4(word[0], word[1], word[2], word[3]);
+    if (kq < per) {
+      const int64_t g = kb * per + kq;
+      const h16 sc = n < p.n && g * p.group < p.k ? scales[g * p.n + n] : static_cast<h16>(0.0f);
+      const unsigned bits = __builtin_bit_cast(unsigned short, sc), sub = bits & 0x3FFu;
+      // normal: the last 3 of 11 bits; subnormal: an odd part under 256
+      const bool fine = bits <= 0x6FF0u && (bits >= 0x400u ? (bits & 7u) == 0u : sub == 0u || (sub >> (__ffs(sub) - 1)) < 256u);
+      if (!fine) atomicOr(flag, 2);
+      s[(tile * 16 + (n & 15)) * per + kq] = sc;
     }
   }
 }
@@ -578,21 +604,20 @@ int lk_hip_w4_quantize(const void* w, void* q, void* s, int64_t n, int64_t k, in
   const lkd::W4Layout p{n, k, (k + 127) / 128, group};
   const unsigned grid = gridFor((n + 15) / 16 * 16 * p.kb * (128 / group));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (nt)
-    hipLaunchKernelGGL(lkd::w4PackKernel<1>, dim3(grid), dim3(256), 0, st, w, nullptr, static_cast<unsigned*>(q),
-                       static_cast<lkd::h16*>(s), p);
-  else
-    hipLaunchKernelGGL(lkd::w4PackKernel<0>, dim3(grid), dim3(256), 0, st, w, nullptr, static_cast<unsigned*>(q),
-                       static_cast<lkd::h16*>(s), p);
+  const auto kernel = nt ? lkd::w4QuantizeKernel<true> : lkd::w4QuantizeKernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, static_cast<const lkd::h16*>(w), static_cast<unsigned*>(q),
+                     static_cast<lkd::h16*>(s), p);
   return launched();
 }
 
-int lk_hip_w4_pack(const void* codes, const void* scales, void* q, void* s, int64_t n, int64_t k, int group, void* stream) {
-  if (n <= 0 || k <= 0 || !groupOk(group) || !al16(q) || !al16(s)) return 1;
+int lk_hip_w4_pack(const void* codes, const void* scales, void* q, void* s, int* flag, int64_t n, int64_t k, int group,
+                   void* stream) {
+  if (n <= 0 || k <= 0 || !groupOk(group) || !al16(q) || !al16(s) || n > (int64_t{1} << 36)) return 1;
   const lkd::W4Layout p{n, k, (k + 127) / 128, group};
-  hipLaunchKernelGGL(lkd::w4PackKernel<2>, dim3(gridFor((n + 15) / 16 * 16 * p.kb * (128 / group))), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), codes, static_cast<const lkd::h16*>(scales),
-                     static_cast<unsigned*>(q), static_cast<lkd::h16*>(s), p);
+  const dim3 grid(static_cast<unsigned>((n + 63) / 64), static_cast<unsigned>(std::min<int64_t>(p.kb, 65535)));
+  hipLaunchKernelGGL(lkd::w4PackKernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream),
+                     static_cast<const uint8_t*>(codes), static_cast<const lkd::h16*>(scales), static_cast<uint4*>(q),
+                     static_cast<lkd::h16*>(s), flag, p);
   return launched();
 }
 
@@ -647,14 +672,15 @@ void runQuantizeW4(ExecCtx& ctx, const KernelArgs& a) {
          "quantize_w4: launch failed");
 }
 
-// pack_w4_u8_gpu: codes u8[K, N], scales f16[ceil(K / G), N] -> q, s; attr group
+// pack_w4_u8_gpu: codes u8[K, N], scales f16[ceil(K / G), N], flag i32[1] (zero; in place) -> q, s; attr group
 void runPackW4(ExecCtx& ctx, const KernelArgs& a) {
-  const int64_t k = a.ints[0], n = a.ints[1], group = a.ints[11];
-  LK_REQUIRE(ctx, w4Shapes(a.ints[4], a.ints[5], a.ints[10], n, k, group) && a.ints[6] == 256 && a.ints[9] == 16 &&
-                      a.ints[3] == n && a.ints[2] == (k + group - 1) / group && a.ints[7] == a.ints[4] &&
-                      a.ints[8] == a.ints[5],
-             "pack_w4: codes u8[K, N], scales f16[ceil(K / group), N], group 32, 64 or 128");
-  status(ctx, lk_hip_w4_pack(a.ptrs[0], a.ptrs[1], a.ptrs[2], a.ptrs[3], n, k, static_cast<int>(group), ctx.stream),
+  const int64_t k = a.ints[0], n = a.ints[1], group = a.ints[12];
+  LK_REQUIRE(ctx, w4Shapes(a.ints[5], a.ints[6], a.ints[11], n, k, group) && a.ints[7] == 256 && a.ints[10] == 16 &&
+                      a.ints[3] == n && a.ints[2] == (k + group - 1) / group && a.ints[8] == a.ints[5] &&
+                      a.ints[9] == a.ints[6] && a.ints[4] == 1,
+             "pack_w4: codes u8[K, N], scales f16[ceil(K / group), N], flag i32[1], group 32, 64 or 128");
+  status(ctx, lk_hip_w4_pack(a.ptrs[0], a.ptrs[1], a.ptrs[3], a.ptrs[4], P<int>(a, 2), n, k, static_cast<int>(group),
+                             ctx.stream),
          "pack_w4: launch failed");
 }
 
@@ -718,7 +744,7 @@ void runGemmW4(ExecCtx& ctx, const KernelArgs& a) {
 void registerQ4Kernels() {
   const Device G = Device::Gpu;
   registerKernel({"quantize_w4_f16_gpu", G, runQuantizeW4, 1, 2});
-  registerKernel({"pack_w4_u8_gpu", G, runPackW4, 2, 2});
+  registerKernel({"pack_w4_u8_gpu", G, runPackW4, 3, 2});
   registerKernel({"unpack_w4_f16_gpu", G, runUnpackW4, 2, 1});
   registerKernel({"gemm_w4_f16_gpu", G, runGemmW4<W4_PLAIN, false>, 3, 1});
   registerKernel({"gemm_w4_bias_f16_gpu", G, runGemmW4<W4_BIAS, false>, 4, 1});

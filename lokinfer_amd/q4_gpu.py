@@ -112,15 +112,6 @@ def quantize_w4_f16_gpu(w, group: int = 64, nt: bool = False) -> PackedWeight4:
     return PackedWeight4(Tensor(q), Tensor(s), (k, n), group)
 
 
-def _scales_ok(s: torch.Tensor) -> bool:
-    """Whether every f16 scale is finite, >= 0, at most 8128 and has at most 8 significant bits."""
-    bits = s.contiguous().view(torch.int16).to(torch.int32)
-    low = torch.where(bits >= 0x400, bits & 7, 0)  # a normal number: the last 3 of its 11 bits
-    sub = bits & 0x3FF                             # a subnormal one: an odd part below 256
-    odd = torch.where((bits < 0x400) & (sub > 0), sub // (sub & -sub).clamp(min=1), 0)
-    return bool(((bits >= 0) & (bits <= 0x6FF0) & (low == 0) & (odd < 256)).all())
-
-
 def pack_w4(w, scales=None, group: int = 64, nt: bool = False) -> PackedWeight4:
     """A weight into the kernels' layout: w f16[K, N] (numpy array or lk.Tensor; nt: f16[N, K]), quantised here, or its
     codes u8[K, N] (0 .. 15) with scales f16[ceil(K / group), N] (>= 0, at most 8 significant bits and 8128)."""
@@ -136,9 +127,11 @@ def pack_w4(w, scales=None, group: int = 64, nt: bool = False) -> PackedWeight4:
     k, n = codes.shape
     q, s = _w4_empty(k, n, group)
     check(tuple(scales.shape) == (-(-k // group), n), "scales must be f16[ceil(K / group), N]")
-    check(bool((codes < 16).all()), "codes must be 0 .. 15")
-    check(_scales_ok(scales), "scales must be >= 0, at most 8128, of at most 8 significant bits")
-    _call("pack_w4_u8_gpu", [codes, scales, q, s], [group])
+    flag = torch.zeros(1, dtype=_I32, device=codes.device)
+    _call("pack_w4_u8_gpu", [codes, scales, flag, q, s], [group])
+    bad = int(flag)  # waits for the layout: once per weight
+    check(not bad & 1, "codes must be 0 .. 15")
+    check(not bad, "scales must be >= 0, at most 8128, of at most 8 significant bits")
     return PackedWeight4(Tensor(q), Tensor(s), (k, n), group)
 
 

@@ -1,5 +1,5 @@
-"""4-bit serving without a GPU: the registry's and the Python ops' refusals, the check of given scales, and the oracle's
-quantiser against its definition."""
+"""4-bit serving without a GPU: the registry's and the Python ops' refusals, and the oracle's quantiser against its
+definition."""
 import ctypes as C
 
 import numpy as np
@@ -31,7 +31,8 @@ P32 = 72 * 32
 REFUSED = [
     ("quantize_w4_f16_gpu", [64, 16, 1, 1, 256, 1, 1, 16, 4, 48, 0], "group"),          # no such group
     ("quantize_w4_f16_gpu", [64, 17, 1, 1, 256, 1, 1, 16, 4, 32, 0], "ceil"),           # 17 columns need 2 tiles
-    ("pack_w4_u8_gpu", [64, 16, 1, 16, 1, 1, 256, 1, 1, 16, 4, 32], "ceil"),            # 2 groups of 32
+    ("pack_w4_u8_gpu", [64, 16, 1, 16, 1, 1, 1, 256, 1, 1, 16, 4, 32], "ceil"),         # 2 groups of 32
+    ("pack_w4_u8_gpu", [64, 16, 2, 16, 2, 1, 1, 256, 1, 1, 16, 4, 32], "flag"),
     ("unpack_w4_f16_gpu", [1, 1, 256, 1, 1, 16, 4, 129, 16, 32], "out"),                # K = 129 needs 2 k blocks
     ("gemm_w4_f16_gpu", [1, 64, 1, 1, 256, 1, 1, 16, 4, 1, 17, 32], "weight"),          # N = 17
     ("gemm_w4_f16_gpu", [1, 64, 1, 1, 256, 1, 1, 16, 4, 2, 16, 32], "out"),             # out rows
@@ -82,25 +83,6 @@ def test_python_ops_refuse_host_tensors_and_bad_handles():
     with pytest.raises(ops.OpError, match="s does not fit"):
         q4.PackedWeight4(lk.Tensor(torch.zeros(1, 1, 256, dtype=torch.int32)),
                          lk.Tensor(torch.zeros(1, 1, 16, 2, dtype=torch.float16)), (64, 16), 32)
-
-
-def test_scales_of_more_than_8_bits_are_refused():
-    every = np.arange(0x7C01, dtype=np.uint16).view(np.float16)  # all f16 >= 0 and infinity
-
-    def fits(h):
-        if not np.isfinite(h) or h > 8128:
-            return False
-        m = int(round(float(h) * 2.0 ** 24))
-        while m and m % 2 == 0:
-            m //= 2
-        return m < 256
-
-    want = np.array([fits(h) for h in every])
-    got = np.array([q4._scales_ok(torch.tensor([float(h)], dtype=torch.float16)) for h in every[::7]])
-    assert (got == want[::7]).all()
-    assert q4._scales_ok(torch.from_numpy(every[want].copy()))
-    for bad in (-1.0, float("nan"), float("inf"), 8192.0, 1 + 2.0 ** -8):
-        assert not q4._scales_ok(torch.tensor([1.0, bad], dtype=torch.float16))
 
 
 def test_oracle_quantizer_is_exact_in_f16_and_off_by_half_a_step():

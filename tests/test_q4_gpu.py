@@ -87,6 +87,31 @@ def product(x, w):
     return x @ w, 2.0 ** -22 * np.sqrt(x.shape[1]) * np.sqrt((x * x) @ (w * w))
 
 
+def test_scales_that_do_not_fit_are_refused(gpu):
+    """Every f16 as a scale, and codes over 15."""
+    lk, q4 = gpu, gpu.ops.q4_gpu
+    every = np.arange(0x10000, dtype=np.uint32).astype(np.uint16).view(np.float16)
+
+    def fits(h):
+        if not (0 <= h <= 8128) or np.signbit(h):
+            return False
+        m = int(float(h) * 2.0 ** 24)
+        return (m & -m) * 256 > m or m == 0
+
+    want = np.array([fits(h) for h in every])
+    codes = np.full((32, int(want.sum())), 9, np.uint8)
+    p = q4.pack_w4(codes, every[want][None, :], 32)
+    assert np.array_equal(q4.unpack_w4_f16_gpu(p).numpy(), np.repeat(every[want][None, :], 32, 0))
+    one = np.full((32, 1), 9, np.uint8)
+    for h in np.concatenate([every[~want][::199], np.float16([8192, -1, np.nan, np.inf, 1 + 2.0 ** -8, 2.0 ** -15 * (1 + 2.0 ** -8)])]):
+        with pytest.raises(OpError, match="scales"):
+            q4.pack_w4(one, np.array([[h]], np.float16), 32)
+    codes = np.zeros((200, 70), np.uint8)
+    codes[199, 69] = 16
+    with pytest.raises(OpError, match="codes"):
+        q4.pack_w4(codes, np.ones((2, 70), np.float16), 128)
+
+
 W4_CASES = [(1, 2048, 4096, 64), (1, 8, 1, 32), (1, 136, 17, 128), (1, 6144, 48, 128), (2, 2048, 96, 64), (4, 72, 40, 32),
             (5, 1000, 777, 32), (16, 264, 33, 64), (17, 2048, 31, 128), (33, 512, 65, 32), (64, 640, 200, 64),
             (65, 520, 200, 128), (100, 200, 300, 32), (130, 1032, 130, 64), (257, 2048, 96, 32), (409, 384, 515, 128),
@@ -237,6 +262,8 @@ ATTN = [  # b, t, qh, kvh, cap, pos
     (1, 2, 16, 8, 64, [0]), (1, 5, 6, 2, 96, [61]), (2, 3, 4, 4, 64, [61, 0]), (1, 33, 4, 2, 96, [0]),
     (1, 64, 8, 2, 128, [64]), (2, 70, 4, 2, 160, [0, 83]), (1, 100, 3, 3, 128, [27]), (1, 129, 16, 8, 512, [300]),
     (1, 40, 16, 1, 64, [20]),
+    # key ranges over workgroups, most of them empty; rows past 16 a kv head; f16 tiles of a long cache
+    (1, 1, 4, 2, 8192, [5]), (3, 1, 16, 8, 4096, [0, 4095, 64]), (1, 3, 24, 2, 4096, [2500]), (2, 20, 4, 2, 2080, [2060, 30]),
 ]
 
 
