@@ -146,14 +146,14 @@ struct Kv4Params {
   h16* out;
   float* part;  // [B T qh, splits, 130]: (max, sum, out[128]) of each workgroup's keys
   int64_t cap;
-  unsigned t;
+  unsigned t, blocks;          // blocks: row blocks of a kv head
   int qh, kvh, group, splits;  // group = qh / kvh
   float scale;  // log2(e) / sqrt(128)
   unsigned long long* err;
 };
 
-// Up to 16 rows a kv head per workgroup of 8 waves: row r = i group + h (query i's q heads side by side). A wave takes 64 keys
-// at a time, four tiles of 16, on 16x16x32 MFMAs:
+// 16 RB rows of a kv head per workgroup of KW waves: row r = i group + h (query i's q heads side by side). A wave takes 64 keys
+// at a time, four tiles of 16, on 16x16x32 MFMAs, each operand of the cache made once for the RB blocks of 16 rows:
 // S = K Q^T: lane (key l % 16, kq = l / 16) loads 16 bytes of its key's row, the codes of scale group kq; its word w, scaled
 // (exact in f16), is the A operand of step w, dims 32 kq + 8 w .., the B operand row l % 16's same dims. Its accumulators are
 // then row l % 16's scores of keys 4 kq + 0 .. 3, on which the softmax runs in f32 (log2 units).
@@ -161,74 +161,93 @@ struct Kv4Params {
 // hi, so that p keeps some 22 bits). The A operand is 8 keys of one dim: lane (db = l % 16, kq) loads those keys' words
 // db, dims 8 db .. 8 db + 7; the low halves of two keys' words put side by side hold the even dims' codes as pairs, the high
 // halves the odd ones', so each dim's operand is masked out of them as a row's codes are out of a word.
-// Chunks are dealt over the waves of all of a head's workgroups (grid y: splits); the waves' sums meet in LDS.
+// Chunks are dealt over the waves of all workgroups of a row block (splits); the waves' sums meet in LDS.
 // Keys from the longest row's end on have their weight and their value's scale set to zero, whatever the memory holds there.
-constexpr int KW = 8;
-__global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
+// The sums are rescaled to a new maximum only where it exceeds the one they stand at by 2^8: until then weights reach 2^8,
+// which changes no relative precision, and nearly every tile brings some row a slightly larger score.
+constexpr float kGrowth = 8.0f;
+template <int RB, int KW>
+__global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1 ? 4 : 2))) void kv4AttnKernel(Kv4Params p) {
   const Q4Masks masks;
-  __shared__ __attribute__((aligned(16))) float os[KW][16][KHD + 4];
-  __shared__ float ms[KW][16], ls[KW][16];
+  constexpr int ROWS = 16 * RB;
+  __shared__ __attribute__((aligned(16))) float os[KW][ROWS][KHD + 4];
+  __shared__ float ms[KW][ROWS], ls[KW][ROWS];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lc = lane & 15, kq = lane >> 4;
   const unsigned group = static_cast<unsigned>(p.group), rowsHead = p.t * group;
-  const unsigned split = blockIdx.x % static_cast<unsigned>(p.splits), rb = blockIdx.x / static_cast<unsigned>(p.splits);
-  const unsigned kvHead = blockIdx.y;
-  const int64_t seq = blockIdx.z;
+  // with 8 kv heads one XCD's L2 each; the last rows, which see the most keys, first
+  const unsigned kvHead = blockIdx.x % static_cast<unsigned>(p.kvh), rest = blockIdx.x / static_cast<unsigned>(p.kvh);
+  const unsigned split = rest % static_cast<unsigned>(p.splits), rb = p.blocks - 1 - rest / static_cast<unsigned>(p.splits);
+  const int64_t seq = blockIdx.y;
   const int64_t p0 = p.pos[seq];
-  const unsigned rowIn = min(rb * 16 + lc, rowsHead - 1), qi = rowIn / group;
-  const int64_t qAt = (seq * p.t + qi) * p.qh + kvHead * group + (rowIn - qi * group);  // of q and out, in heads
-  half8 qf[4];
-#pragma unroll
-  for (int w = 0; w < 4; ++w) qf[w] = ld8(p.q + qAt * KHD + 32 * kq + 8 * w);
   const int cap = static_cast<int>(p.cap);
-  // rows of the cache that the lane's row, and the block's last and first row, see
-  const auto sees = [&](int64_t i) { return p0 < 0 ? 0 : static_cast<int>(min<int64_t>(p0 + i + 1, p.cap)); };
-  const int nkRow = sees(qi), nk = sees(min(rb * 16 + 15, rowsHead - 1) / group), nkAll = sees(rb * 16 / group);
-  if (split == 0 && rb == 0 && kvHead == 0 && threadIdx.x == 0 && (p0 < 0 || p0 + p.t > p.cap))
-    raiseDeviceError(p.err, LK_DEVERR_POSITION, p0 < 0 ? p0 : p0 + p.t - 1);
+  // rows of the cache that query i sees; the block's last and first row's
+  const auto sees = [&](int64_t i) { return p0 < 0 ? 0 : static_cast<int>(p0 < p.cap ? min<int64_t>(p0 + i + 1, p.cap) : p.cap); };
+  const int nk = sees(min(rb * ROWS + ROWS - 1, rowsHead - 1) / group), nkAll = sees(rb * ROWS / group);
+  half8 qf[RB][4];
+  int nkRow[RB];
+#pragma unroll
+  for (int k = 0; k < RB; ++k) {
+    const unsigned row = min(rb * ROWS + 16 * k + lc, rowsHead - 1), qi = row / group;
+    nkRow[k] = sees(qi);
+    const h16* q = p.q + ((seq * p.t + qi) * p.qh + kvHead * group + (row - qi * group)) * KHD + 32 * kq;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) qf[k][w] = ld8(q + 8 * w);
+  }
+  if (rest == 0 && kvHead == 0 && threadIdx.x == 0 && (p0 < 0 || p0 > p.cap - p.t))
+    raiseDeviceError(p.err, LK_DEVERR_POSITION, p0 < 0 || p0 > p.cap ? p0 : p0 + p.t - 1);
   const int64_t block = 72 * p.cap;
   const char* kb = p.kv + (seq * 2 * p.kvh + kvHead) * block;
   const char* vb = kb + p.kvh * block;
-  const h16* ksc = reinterpret_cast<const h16*>(kb + 64 * p.cap) + kq * p.cap;
-  const h16* vsc = reinterpret_cast<const h16*>(vb + 64 * p.cap) + (lc >> 2) * p.cap;
+  // a chunk's base is uniform, a lane's place in it a 32-bit offset in bytes: codes and scales of keys and values
+  const unsigned kOff = lc * 64 + 16 * kq, vOff = 4 * kq * 64 + 4 * lc;
+  const unsigned ksOff = kq * static_cast<unsigned>(cap) * 2 + lc * 2, vsOff = (lc >> 2) * static_cast<unsigned>(cap) * 2 + 8 * kq;
   const int chunks = (nk + 63) / 64, step = p.splits * KW;
-  f32x4 acc[8];
+  f32x4 acc[RB][8];
+  float m[RB];   // a running maximum times the scale, rounded once and taken off everywhere as it is
+  f32x4 l[RB];   // the weights' sum, four times: a product with ones
+  const h16 one = static_cast<h16>(1.0f);
+  const half8 ones{one, one, one, one, one, one, one, one};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  // m: the running maximum times the scale, rounded once and taken off everywhere as it is
-  float m = -INFINITY, l = 0.0f;
-  struct Chunk {
-    uint4 k[4];
+  for (int k = 0; k < RB; ++k) {
+    m[k] = -INFINITY;
+    l[k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[k][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  for (int c = static_cast<int>(split) * KW + wave; c < chunks; c += step) {
+    // Rows behind the last key are read as they lie, and masked below; the cache ends with a chunk or in its middle, where
+    // the second half reads the first's rows.
+    const int64_t half = c * 64 + 32 < cap ? 32 : 0, c0 = static_cast<int64_t>(c) * 64;
+    uint4 kw[4];
     h16 ks[4];
-    unsigned v[4][4];
+    unsigned vw[4][4];
     half4 vs[4];
-  };
-  const auto load = [&](int c) {
-    Chunk x;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t at = min(c * 64 + 16 * u + lc, nk - 1);
-      x.k[u] = *reinterpret_cast<const uint4*>(kb + at * 64 + 16 * kq);
-      x.ks[u] = ksc[at];
+      const int64_t r0 = c0 + (u >> 1) * half;
+      kw[u] = *reinterpret_cast<const uint4*>(kb + r0 * 64 + kOff + 1024 * (u & 1));
+      ks[u] = *reinterpret_cast<const h16*>(kb + 64 * p.cap + r0 * 2 + ksOff + 32 * (u & 1));
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t at = min(c * 64 + 16 * u + 4 * kq, cap - 4);
+      const int64_t r0 = c0 + (u >> 1) * half;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) x.v[u][r] = *reinterpret_cast<const unsigned*>(vb + (at + r) * 64 + 4 * lc);
-      x.vs[u] = *reinterpret_cast<const half4*>(vsc + at);
+      for (int r = 0; r < 4; ++r) vw[u][r] = *reinterpret_cast<const unsigned*>(vb + r0 * 64 + vOff + 1024 * (u & 1) + 64 * r);
+      vs[u] = *reinterpret_cast<const half4*>(vb + 64 * p.cap + r0 * 2 + vsOff + 32 * (u & 1));
     }
-    return x;
-  };
-  const auto compute = [&](int c, Chunk& x) {
-    f32x4 s[4];
+    f32x4 s[RB][4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const unsigned w4[4] = {x.k[u].x, x.k[u].y, x.k[u].z, x.k[u].w};
-      const h16 f = x.ks[u];
-      s[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      const unsigned w4[4] = {kw[u].x, kw[u].y, kw[u].z, kw[u].w};
+      const h16 f = ks[u];
 #pragma unroll
-      for (int w = 0; w < 4; ++w)
-        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(q4Ints(w4[w], masks) * half8{f, f, f, f, f, f, f, f}, qf[w], s[u], 0, 0, 0);
+      for (int k = 0; k < RB; ++k) s[k][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const half8 a = q4Ints(w4[w], masks) * half8{f, f, f, f, f, f, f, f};
+#pragma unroll
+        for (int k = 0; k < RB; ++k) s[k][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[k][w], s[k][u], 0, 0, 0);
+      }
     }
     if (c * 64 + 64 > nkAll) {  // keys past some row's
 #pragma unroll
@@ -236,48 +255,61 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int key = c * 64 + 16 * u + 4 * kq + r;
-          if (key >= nkRow) s[u][r] = -INFINITY;
-          if (key >= nk) x.vs[u][r] = static_cast<h16>(0.0f);
+#pragma unroll
+          for (int k = 0; k < RB; ++k)
+            if (key >= nkRow[k]) s[k][u][r] = -INFINITY;
+          if (key >= nk) vs[u][r] = static_cast<h16>(0.0f);
         }
     }
-    float mx = s[0][0];
+    half8 ph[RB][2], pl[RB][2];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int k = 0; k < RB; ++k) {
+      float mx = s[k][0][0];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[u][r]);
-    mx = crossRowMax(mx) * p.scale;
-    if (__any(mx > m)) {  // some row's maximum grew
-      const float to = fmaxf(m, mx), corr = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - to);
-      l *= corr;
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] *= corr;
-      m = to;
-    }
-    const float base = m == -INFINITY ? 0.0f : m;  // no key so far: every weight 0 (or a NaN kept)
+        for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[k][u][r]);
+      mx = crossRowMax(mx) * p.scale;
+      if (__any(mx > m[k] + kGrowth)) {
+        const float to = fmaxf(m[k], mx), corr = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[k] - to);
+        l[k] *= corr;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], p.scale, -base));
-        l += s[u][r];
+        for (int e = 0; e < 8; ++e) acc[k][e] *= corr;
+        m[k] = to;
       }
+      const float base = m[k] == -INFINITY ? 0.0f : m[k];  // no key so far: every weight 0 (or a NaN kept)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          typedef float f32x2 __attribute__((ext_vector_type(2)));
+          const f32x2 e = {__builtin_amdgcn_exp2f(fmaf(s[k][u][r], p.scale, -base)),
+                           __builtin_amdgcn_exp2f(fmaf(s[k][u][r + 1], p.scale, -base))};
+          const half2v hi = __builtin_convertvector(e, half2v);
+          const half2v lo = __builtin_convertvector((f32x2{fmaf(static_cast<float>(hi[0]), -1.0f, e[0]),
+                                                           fmaf(static_cast<float>(hi[1]), -1.0f, e[1])}), half2v);
+          const int at = 4 * (u & 1) + r;
+          ph[k][u >> 1][at] = hi[0];
+          ph[k][u >> 1][at + 1] = hi[1];
+          pl[k][u >> 1][at] = lo[0];
+          pl[k][u >> 1][at + 1] = lo[1];
+        }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        l[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[k][t], l[k], 0, 0, 0);
+        l[k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[k][t], l[k], 0, 0, 0);
+      }
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {  // keys 32 t ..: tiles 2 t, 2 t + 1
-      half8 ph, pl;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = s[2 * t + (j >> 2)][j & 3];
-        ph[j] = static_cast<h16>(v);
-        pl[j] = static_cast<h16>(v - static_cast<float>(ph[j]));
-      }
       unsigned even[4], odd[4];
       half2v sc[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {  // keys 2 j, 2 j + 1 of the lane's 8
-        const unsigned a = x.v[2 * t + (j >> 1)][2 * (j & 1)], b = x.v[2 * t + (j >> 1)][2 * (j & 1) + 1];
+        const unsigned a = vw[2 * t + (j >> 1)][2 * (j & 1)], b = vw[2 * t + (j >> 1)][2 * (j & 1) + 1];
         even[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
         odd[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-        sc[j] = half2v{x.vs[2 * t + (j >> 1)][2 * (j & 1)], x.vs[2 * t + (j >> 1)][2 * (j & 1) + 1]};
+        sc[j] = half2v{vs[2 * t + (j >> 1)][2 * (j & 1)], vs[2 * t + (j >> 1)][2 * (j & 1) + 1]};
       }
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
@@ -292,29 +324,31 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
         for (int i = 0; i < 4; ++i) {
           const half8 a{dims[i][0][0], dims[i][0][1], dims[i][1][0], dims[i][1][1],
                         dims[i][2][0], dims[i][2][1], dims[i][3][0], dims[i][3][1]};
-          acc[2 * i + o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, acc[2 * i + o], 0, 0, 0);
-          acc[2 * i + o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, acc[2 * i + o], 0, 0, 0);
+#pragma unroll
+          for (int k = 0; k < RB; ++k) {
+            acc[k][2 * i + o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph[k][t], acc[k][2 * i + o], 0, 0, 0);
+            acc[k][2 * i + o] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl[k][t], acc[k][2 * i + o], 0, 0, 0);
+          }
         }
       }
     }
-  };
-  for (int c = static_cast<int>(split) * KW + wave; c < chunks; c += step) {
-    Chunk x = load(c);
-    compute(c, x);
   }
   // accumulator r of dim e: dim 8 (4 kq + r) + e of row l % 16
-  l = crossRowSum(l);
-  const int rows = static_cast<int>(min(rowsHead - rb * 16, 16u));
-  if (lc < rows) {
-    if (kq == 0) {
-      ms[wave][lc] = m;
-      ls[wave][lc] = l;
-    }
+  const int rows = static_cast<int>(min(rowsHead - rb * ROWS, static_cast<unsigned>(ROWS)));
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      float* o = &os[wave][lc][8 * (4 * kq + r)];
-      *reinterpret_cast<f32x4*>(o) = f32x4{acc[0][r], acc[1][r], acc[2][r], acc[3][r]};
-      *reinterpret_cast<f32x4*>(o + 4) = f32x4{acc[4][r], acc[5][r], acc[6][r], acc[7][r]};
+  for (int k = 0; k < RB; ++k) {
+    const int row = 16 * k + lc;
+    if (row < rows) {
+      if (kq == 0) {
+        ms[wave][row] = m[k];
+        ls[wave][row] = l[k][0];
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float* o = &os[wave][row][8 * (4 * kq + r)];
+        *reinterpret_cast<f32x4*>(o) = f32x4{acc[k][0][r], acc[k][1][r], acc[k][2][r], acc[k][3][r]};
+        *reinterpret_cast<f32x4*>(o + 4) = f32x4{acc[k][4][r], acc[k][5][r], acc[k][6][r], acc[k][7][r]};
+      }
     }
   }
   __syncthreads();
@@ -330,10 +364,10 @@ __global__ __launch_bounds__(64 * KW, 2) void kv4DecodeKernel(Kv4Params p) {
       ll = fmaf(f, ls[w][r], ll);
       y = fmaf(f, os[w][r][d], y);
     }
-    const unsigned i = (rb * 16 + r) / group;
-    const int64_t at = (seq * p.t + i) * p.qh + kvHead * group + (rb * 16 + r - i * group);
+    const unsigned i = (rb * ROWS + r) / group;
+    const int64_t at = (seq * p.t + i) * p.qh + kvHead * group + (rb * ROWS + r - i * group);
     if (p.splits == 1) {
-      const bool noRow = p0 < 0 || p0 + i >= p.cap;
+      const bool noRow = p0 < 0 || p0 >= p.cap - i;
       p.out[at * KHD + d] = noRow ? static_cast<h16>(__builtin_nanf("")) : toH16(y / ll);
     } else {
       float* pp = p.part + (at * p.splits + split) * (KHD + 2);
@@ -351,7 +385,7 @@ __global__ __launch_bounds__(128) void kv4MergeKernel(Kv4Params p) {
   const int d = threadIdx.x;
   const unsigned qi = blockIdx.y, seq = qi / p.t;
   const int64_t at = static_cast<int64_t>(qi) * p.qh + blockIdx.x, p0 = p.pos[seq];
-  const bool noRow = p0 < 0 || p0 + (qi - seq * p.t) >= p.cap;
+  const bool noRow = p0 < 0 || p0 >= p.cap - (qi - seq * p.t);
   const float* part = p.part + at * p.splits * (KHD + 2);
   float m = -INFINITY, l = 0.0f, o = 0.0f;
   for (int s0 = 0; s0 < p.splits; s0 += 32) {
@@ -378,25 +412,6 @@ __global__ __launch_bounds__(128) void kv4MergeKernel(Kv4Params p) {
     m = mb;
   }
   p.out[at * KHD + d] = noRow ? static_cast<h16>(__builtin_nanf("")) : toH16(o / l);
-}
-
-// Many rows: the rows 0 .. pos + T - 1 of one sequence as f16 [P, kvh 128], keys then values, for the f16 tiles of
-// lk_hip_f16_attention_gqa: they are dequantised once instead of by every block of queries. 8 values per thread, grid
-// rows 16 / 256, kv heads, 2.
-__global__ __launch_bounds__(256) void kv4ExpandKernel(const char* __restrict__ kv, const int64_t* __restrict__ pos,
-                                                       h16* __restrict__ out, unsigned t, int kvh, unsigned cap) {
-  const Q4Masks masks;
-  const int64_t p0 = *pos;
-  const unsigned rows = p0 < 0 ? 0 : static_cast<unsigned>(min<int64_t>(p0 + t, cap));
-  const unsigned h = blockIdx.y;
-  const char* at = kv + (static_cast<int64_t>(blockIdx.z) * kvh + h) * 72 * cap;
-  h16* o = out + static_cast<int64_t>(blockIdx.z) * cap * kvh * KHD + h * KHD;
-  for (unsigned id = blockIdx.x * 256 + threadIdx.x; id < rows * 16; id += gridDim.x * 256) {
-    const unsigned row = id >> 4, w = id & 15;
-    const h16 s = *reinterpret_cast<const h16*>(at + static_cast<int64_t>(cap) * (64 + (w >> 2) * 2) + 2 * row);
-    const half8 v = q4Ints(*reinterpret_cast<const unsigned*>(at + static_cast<int64_t>(id) * 4), masks);
-    st8(o + static_cast<int64_t>(row) * kvh * KHD + 8 * w, v * half8{s, s, s, s, s, s, s, s});
-  }
 }
 
 // ---- moving caches between sequences ------------------------------------------------------------------------------
@@ -465,14 +480,25 @@ bool kvOk(const void* kv, int64_t b, int kvh, int64_t cap) {
 // rows of a call: they are counted in 32 bits
 bool rowsOk(int64_t b, int64_t t) { return t >= 0 && t <= 0x7FFFFFFF && b <= 65535 && b * t <= 0x7FFFFFFF; }
 
-// Many rows: expanded to f16 once
-bool kv4Expands(int64_t t, int64_t group) { return t > 1 && t * group > 32; }
+// Row blocks and waves of a workgroup. us of (1, 8) / (1, 4) / (2, 8) / (2, 4) by T queries over P rows, 16 / 8 heads:
+// 256, 512: 9.1 / 9.1 / 13 / 13; 512, 512: 12.7 / 10.6 / 13.4 / 13.4; 600, 2048: 40 / 39 / 43 / 39; 1024, 2048: 51 / 48 / 45 / 41;
+// 2048, 2048: 75 / 63 / 69 / 55; 2048, 8192: 344 / 337 / 268 / 253; 256, 32768: 204 / 240 / 246 / 302; 409, 32768: 338 / 345 /
+// 254 / 302. (Expanded once to f16 and run through the f16 op's tiles: 15, 15, 49, 46, 55, 269, 277 and 310.)
+struct Kv4Shape {
+  int rb, kw;
+};
+Kv4Shape kv4Shape(int64_t b, int64_t rows, int kvh, int64_t cap) {
+  const int64_t groups = b * kvh * ((rows + 15) / 16);
+  if (groups <= 256) return {1, 8};
+  if (groups <= 640 && cap <= 2048) return {1, 4};
+  return groups <= 640 ? Kv4Shape{2, 8} : Kv4Shape{2, 4};
+}
 
+// Workgroups over a row block's keys: one for up to 1024 rows (a launch more costs 4 us), else the chip's 256 in all, of at
+// least 512 rows each. p32768 at 16 / 8 heads, 16 / 32 / 64 of them: 21 / 17 / 20 us with the joining launch.
 int kv4Splits(int64_t b, int64_t t, int qh, int kvh, int64_t cap) {
   const int64_t groups = b * kvh * ((t * (qh / kvh) + 15) / 16);
-
-
-  if (cap <= 2048 || groups >= 256) return 1;
+  if (cap <= 1024 || groups >= 256) return 1;
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((cap + 511) / 512, 256 / groups)));
 }
 
@@ -518,7 +544,6 @@ int lk_hip_kv4_read(const void* kv, void* out, int64_t blocks, int64_t cap, void
 
 int64_t lk_hip_kv4_attention_workspace_bytes(int64_t b, int64_t t, int qh, int kvh, int64_t cap) {
   if (b <= 0 || t <= 0 || qh <= 0 || kvh <= 0 || qh % kvh != 0 || cap <= 0) return 0;
-  if (kv4Expands(t, qh / kvh)) return 2 * cap * kvh * lkd::KHD * 2;
   const int64_t s = kv4Splits(b, t, qh, kvh, cap);
   return s > 1 ? s * b * t * qh * (lkd::KHD + 2) * 4 : 0;
 }
@@ -531,27 +556,18 @@ int lk_hip_kv4_attention(const void* q, const void* kv, const int64_t* pos, void
   const int64_t need = lk_hip_kv4_attention_workspace_bytes(b, t, qh, kvh, cap);
   if (need > 0 && (!workspace || workspace_bytes < need || !al16(workspace))) return 3;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (kv4Expands(t, qh / kvh)) {
-    h16* rows = static_cast<h16*>(workspace);
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(cap / 16, 256)), static_cast<unsigned>(kvh), 2);
-    for (int64_t i = 0; i < b; ++i) {  // one sequence after the other through the same rows
-      hipLaunchKernelGGL(kv4ExpandKernel, grid, dim3(256), 0, s, static_cast<const char*>(kv) + i * 2 * kvh * 72 * cap, pos + i,
-                         rows, static_cast<unsigned>(t), kvh, static_cast<unsigned>(cap));
-      const int rc = lk_hip_f16_attention_gqa(static_cast<const h16*>(q) + i * t * qh * KHD, rows, rows + cap * kvh * KHD,
-                                              pos + i, static_cast<h16*>(out) + i * t * qh * KHD, t, qh, kvh, cap, nullptr, 0,
-                                              stream);
-      if (rc) return rc;
-    }
-    return launched();
-  }
   const int splits = kv4Splits(b, t, qh, kvh, cap);
+  const int64_t rows = t * (qh / kvh);
+  const Kv4Shape shape = kv4Shape(b, rows, kvh, cap);
+  const int64_t blocks = (rows + 16 * shape.rb - 1) / (16 * shape.rb);
+  if (rows > 0x7FFFFFFF || blocks * splits * kvh > 0x7FFFFFFF || (splits > 1 && b * t > 65535)) return 1;
   const Kv4Params p{static_cast<const h16*>(q), static_cast<const char*>(kv), pos, static_cast<h16*>(out),
-                    static_cast<float*>(workspace), cap, static_cast<unsigned>(t), qh, kvh, qh / kvh, splits,
-                    kLog2e / std::sqrt(static_cast<float>(KHD)), lkh::deviceErrorRecord()};
-  const int64_t blocks = (t * (qh / kvh) + 15) / 16 * splits;
-  if (t * (qh / kvh) > 0x7FFFFFFF || blocks > 0x7FFFFFFF || (splits > 1 && b * t > 65535)) return 1;
-  hipLaunchKernelGGL(kv4DecodeKernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(kvh), static_cast<unsigned>(b)),
-                     dim3(64 * KW), 0, s, p);
+                    static_cast<float*>(workspace), cap, static_cast<unsigned>(t), static_cast<unsigned>(blocks), qh, kvh,
+                    qh / kvh, splits, kLog2e / std::sqrt(static_cast<float>(KHD)), lkh::deviceErrorRecord()};
+  const dim3 grid(static_cast<unsigned>(blocks * splits * kvh), static_cast<unsigned>(b));
+  const auto kernel = shape.rb == 1 ? (shape.kw == 8 ? kv4AttnKernel<1, 8> : kv4AttnKernel<1, 4>)
+                                    : (shape.kw == 8 ? kv4AttnKernel<2, 8> : kv4AttnKernel<2, 4>);
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * shape.kw), 0, s, p);
   if (splits > 1)
     hipLaunchKernelGGL(kv4MergeKernel, dim3(static_cast<unsigned>(qh), static_cast<unsigned>(b * t)), dim3(128), 0, s, p);
   return launched();
@@ -578,12 +594,12 @@ namespace lkh {
 
 namespace {
 
-bool kv4Shape(int64_t two, int64_t bytes) { return two == 2 && bytes > 0 && bytes % (72 * 32) == 0; }
+bool kv4Layout(int64_t two, int64_t bytes) { return two == 2 && bytes > 0 && bytes % (72 * 32) == 0; }
 
 // kv4_write_f16_gpu: kv u8[B, 2, kvh, 72 P], k, v f16[B T, kvh 128], pos i64[B] (in place)
 void runKv4Write(ExecCtx& ctx, const KernelArgs& a) {
   const int64_t b = a.ints[0], kvh = a.ints[2], cap = a.ints[3] / 72, rows = a.ints[4];
-  LK_REQUIRE(ctx, b > 0 && kvh > 0 && kv4Shape(a.ints[1], a.ints[3]) && rows % b == 0 && a.ints[5] == kvh * 128 &&
+  LK_REQUIRE(ctx, b > 0 && kvh > 0 && kv4Layout(a.ints[1], a.ints[3]) && rows % b == 0 && a.ints[5] == kvh * 128 &&
                       a.ints[6] == rows && a.ints[7] == a.ints[5] && a.ints[8] == b,
              "kv4_write: kv u8[B, 2, kvh, 72 P] with P % 32 == 0, k and v f16[B T, kvh 128], pos i64[B]");
   status(ctx, lk_hip_kv4_write(a.ptrs[0], a.ptrs[1], a.ptrs[2], P<int64_t>(a, 3), b, rows / b, static_cast<int>(kvh), cap,
@@ -595,7 +611,7 @@ void runKv4Write(ExecCtx& ctx, const KernelArgs& a) {
 // floats eps, theta
 void runKv4Qkr(ExecCtx& ctx, const KernelArgs& a) {
   const int64_t rows = a.ints[0], b = a.ints[4], kvh = a.ints[7], cap = a.ints[8] / 72, qw = a.ints[10];
-  LK_REQUIRE(ctx, b > 0 && kvh > 0 && kv4Shape(a.ints[6], a.ints[8]) && a.ints[5] == b && rows % b == 0 &&
+  LK_REQUIRE(ctx, b > 0 && kvh > 0 && kv4Layout(a.ints[6], a.ints[8]) && a.ints[5] == b && rows % b == 0 &&
                       a.ints[2] == 128 && a.ints[3] == 128 && qw > 0 && qw % 128 == 0 &&
                       a.ints[1] == qw + 2 * kvh * 128 && a.ints[9] == rows,
              "qknorm_rope_kv4: qkv f16[B T, (qh + 2 kvh) 128], gains f16[128], pos i64[B], kv u8[B, 2, kvh, 72 P]");
@@ -607,7 +623,7 @@ void runKv4Qkr(ExecCtx& ctx, const KernelArgs& a) {
 
 // kv4_read_f16_gpu: kv u8[blocks, 72 P] -> f16[blocks, P, 128]
 void runKv4Read(ExecCtx& ctx, const KernelArgs& a) {
-  LK_REQUIRE(ctx, kv4Shape(2, a.ints[1]) && a.ints[2] == a.ints[0] && a.ints[3] == a.ints[1] / 72 && a.ints[4] == 128,
+  LK_REQUIRE(ctx, kv4Layout(2, a.ints[1]) && a.ints[2] == a.ints[0] && a.ints[3] == a.ints[1] / 72 && a.ints[4] == 128,
              "kv4_read: kv u8[blocks, 72 P] with P % 32 == 0, out f16[blocks, P, 128]");
   status(ctx, lk_hip_kv4_read(a.ptrs[0], a.ptrs[1], a.ints[0], a.ints[3], ctx.stream), "kv4_read: launch failed");
 }
@@ -615,7 +631,7 @@ void runKv4Read(ExecCtx& ctx, const KernelArgs& a) {
 // attention_kv4_f16_gpu: q f16[B T, qh 128], kv u8[B, 2, kvh, 72 P], pos i64[B] -> out f16[B T, qh 128], work f32[n]
 void runKv4Attention(ExecCtx& ctx, const KernelArgs& a) {
   const int64_t rows = a.ints[0], width = a.ints[1], b = a.ints[2], kvh = a.ints[4], cap = a.ints[5] / 72;
-  LK_REQUIRE(ctx, b > 0 && kvh > 0 && kv4Shape(a.ints[3], a.ints[5]) && rows % b == 0 && width > 0 &&
+  LK_REQUIRE(ctx, b > 0 && kvh > 0 && kv4Layout(a.ints[3], a.ints[5]) && rows % b == 0 && width > 0 &&
                       width % (128 * kvh) == 0 && a.ints[6] == b && a.ints[7] == rows && a.ints[8] == width,
              "attention_kv4: q f16[B T, qh 128], kv u8[B, 2, kvh, 72 P], qh a multiple of kvh, pos i64[B]");
   const int rc = lk_hip_kv4_attention(a.ptrs[0], a.ptrs[1], P<int64_t>(a, 2), a.ptrs[3], b, rows / b,
@@ -626,7 +642,7 @@ void runKv4Attention(ExecCtx& ctx, const KernelArgs& a) {
 
 // kv4_reorder_gpu: kv u8[L, B, 2, kvh, 72 P], parents i64[B], n i64[1] (in place)
 void runKv4Reorder(ExecCtx& ctx, const KernelArgs& a) {
-  LK_REQUIRE(ctx, kv4Shape(a.ints[2], a.ints[4]) && a.ints[5] == a.ints[1] && a.ints[6] == 1 && a.ints[1] > 0 &&
+  LK_REQUIRE(ctx, kv4Layout(a.ints[2], a.ints[4]) && a.ints[5] == a.ints[1] && a.ints[6] == 1 && a.ints[1] > 0 &&
                       a.ints[1] <= lkd::kMaxBeams && a.ints[3] > 0 && a.ints[0] * 2 * a.ints[3] <= 65535,
              "kv4_reorder: kv u8[L, B, 2, kvh, 72 P] with B <= 32 and L kvh <= 32767, parents i64[B], n i64[1]");
   status(ctx, lk_hip_kv4_reorder(a.ptrs[0], P<int64_t>(a, 1), P<int64_t>(a, 2), a.ints[0], a.ints[1],

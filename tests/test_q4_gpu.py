@@ -262,8 +262,10 @@ ATTN = [  # b, t, qh, kvh, cap, pos
     (1, 2, 16, 8, 64, [0]), (1, 5, 6, 2, 96, [61]), (2, 3, 4, 4, 64, [61, 0]), (1, 33, 4, 2, 96, [0]),
     (1, 64, 8, 2, 128, [64]), (2, 70, 4, 2, 160, [0, 83]), (1, 100, 3, 3, 128, [27]), (1, 129, 16, 8, 512, [300]),
     (1, 40, 16, 1, 64, [20]),
-    # key ranges over workgroups, most of them empty; rows past 16 a kv head; f16 tiles of a long cache
+    # key ranges over workgroups, most of them empty; rows past 16 a kv head
     (1, 1, 4, 2, 8192, [5]), (3, 1, 16, 8, 4096, [0, 4095, 64]), (1, 3, 24, 2, 4096, [2500]), (2, 20, 4, 2, 2080, [2060, 30]),
+    # more rows: 4 waves a workgroup; 32 rows of 8 waves over a longer cache; 32 rows of 4 waves
+    (2, 150, 16, 8, 512, [0, 361]), (1, 300, 16, 8, 2112, [1801]), (2, 401, 16, 8, 448, [0, 40]), (1, 165, 32, 4, 192, [20]),
 ]
 
 
@@ -297,7 +299,7 @@ def test_large_scores_and_one_key_taking_all(gpu, t):
     close(got, o.reshape(t, -1), np.repeat(top * (2.0 ** -22 * (8 + np.sqrt(128)) + 4 * 2.0 ** -22 * term), 128, 1))
 
 
-@pytest.mark.parametrize("t,qh,kvh", [(1, 4, 2), (1, 16, 1), (48, 4, 2)])
+@pytest.mark.parametrize("t,qh,kvh", [(1, 4, 2), (1, 16, 1), (48, 4, 2), (89, 64, 8), (90, 128, 16)])
 def test_rows_that_are_not_finite_reach_only_queries_that_see_them(gpu, t, qh, kvh):
     lk, q4 = gpu, gpu.ops.q4_gpu
     r = rng_of(10, t, qh)
@@ -338,6 +340,10 @@ def test_positions_outside_the_cache_are_nan_and_reported(gpu):
         assert np.isnan(got[t - 1]).all() and np.isfinite(got[: t - 1]).all()  # the last query of sequence 0
         assert np.array_equal(got[t:2 * t], want[t:2 * t])
         assert np.isnan(got[2 * t:]).all()
+        got = q4.attention_kv4_f16_gpu(q, kv, I(lk, 2 ** 63 - 1, 20, 2 ** 63 - t)).t.cpu().numpy()
+        with pytest.raises(LokinferError, match="position"):
+            check_device_errors()
+        assert np.isnan(got[: t]).all() and np.isnan(got[2 * t:]).all() and np.array_equal(got[t:2 * t], want[t:2 * t])
 
 
 def test_qknorm_rope_is_the_f16_ops(gpu):

@@ -31,7 +31,7 @@ def step(lk, d, kv):
     q = q4.qknorm_rope_kv4_f16_gpu(d["qkv"], d["g"], d["g"], d["pos"], kv)
     a = q4.attention_kv4_f16_gpu(q, kv, d["pos"])
     s, parent, tok, done = lk.ops.beam_select_f32_gpu(d["logits"], d["scores"], d["done"], 3, (7, 11))
-    wide = q4.attention_kv4_f16_gpu(T(d["q"].t.repeat(20, 1)), kv, T(d["pos"].t.clamp(max=500)))  # through f16 tiles
+    wide = q4.attention_kv4_f16_gpu(T(d["q"].t.repeat(20, 1)), kv, T(d["pos"].t.clamp(max=500)))  # rows of many workgroups
     q4.kv4_reorder_gpu(T(kv.t.unsqueeze(0)), parent, d["n"])
     return [x.t for x in (y, q, a, s, parent, tok, done, wide)] + [kv.t]
 
@@ -120,7 +120,7 @@ def test_caches_past_4_gib(gpu):
     held = O.cache_values(k, v, kvh)
     read = q4.kv4_read_f16_gpu(lk.Tensor(kv.t[0, 1, kvh - 1])).t[torch.tensor(at)].cpu().numpy()
     assert np.array_equal(read.astype(np.float64), held[1][:, kvh - 1])
-    for t in (1, 40):  # 40 rows go through f16 tiles
+    for t in (1, 40):
         q = np.tile((4 * k.astype(np.float32).reshape(3, kvh, 128).sum(0)).reshape(1, -1), (t, 1)).astype(np.float16)
         got = q4.attention_kv4_f16_gpu(G(q), kv, pos(cap - t)).t[-1].cpu().numpy().reshape(kvh, 128).astype(np.float64)
         for h in range(kvh):
