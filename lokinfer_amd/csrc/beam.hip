@@ -9,10 +9,10 @@
 // their k best, maximum and sum of exponentials. At least k of a wave's 64 lane maxima, so k of its logits, are not below the
 // k-th largest of them (found by counting); the logits not below the largest such bound of the four waves, k and some
 // more, go to LDS and are ranked by counting. Where they are more than fit (thousands of equal logits), each wave takes
-// its k best one after the other instead. beamPickKernel, one workgroup, joins a row's lists with one wave (lane i at the
-// head of list i), adds up its log-sum, and takes the k best of the rows' heads. Within a row the order is that of the
-// logits (exact); between beams that of the candidates in 64 bits, the sums of exponentials of 8192 logits each (32
-// bits) added in 64 bits.
+// its k best one after the other instead. beamPickKernel, one workgroup, joins a row's lists with one wave (what is not
+// below a bound from the lists' heads, ranked by counting), adds up its log-sum, and joins the rows' candidates likewise.
+// Within a row the order is that of the logits (exact); between beams that of the candidates in 64 bits, the sums of
+// exponentials of 8192 logits each (32 bits) added in 64 bits.
 #include <algorithm>
 
 #include "common.h"
@@ -71,6 +71,14 @@ __device__ __forceinline__ unsigned waveMaxU32(unsigned v) {
 __device__ __forceinline__ u64 waveMaxU64(unsigned hi, unsigned lo) {
   const unsigned top = waveMaxU32(hi);
   return pairOf(top, waveMaxU32(hi == top ? lo : 0u));
+}
+
+// how many of n keys come before the i-th, key: larger ones, and equal ones in front of it
+__device__ __forceinline__ int beamRank(const u64* keys, int n, u64 key, int i) {
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) rank += keys[j] > key || (keys[j] == key && j < i);
+  return rank;
 }
 
 __global__ __launch_bounds__(64 * kBeamWaves) void beamScanKernel(BeamParams p) {
@@ -143,10 +151,9 @@ __global__ __launch_bounds__(64 * kBeamWaves) void beamScanKernel(BeamParams p) 
     __syncthreads();
     n = kBeamWaves * p.k;
   }
-  if (static_cast<int>(threadIdx.x) < n) {  // entries without a logit (key 0) are distinct by their index
+  if (static_cast<int>(threadIdx.x) < n) {  // (places without a logit can be equal: key 0)
     const u64 mine = fit[threadIdx.x];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += fit[j] > mine;
+    const int rank = beamRank(fit, n, mine, static_cast<int>(threadIdx.x));
     if (rank < p.k)
       p.lists[(static_cast<int64_t>(beam) * p.tiles + tile) * p.k + rank] =
           make_uint2(static_cast<unsigned>(mine >> 32), ~static_cast<unsigned>(mine));
@@ -160,21 +167,63 @@ __global__ __launch_bounds__(64 * kBeamWaves) void beamScanKernel(BeamParams p) 
   }
 }
 
-// Row `beam`'s k candidates, best first, by one wave: the best heads of its lists one after the other.
-__device__ __forceinline__ void beamRow(const BeamParams& p, int beam, uint2* heads, double* cand, int* tok) {
+// the wave's own LDS, between its lanes' writes and reads
+__device__ __forceinline__ void waveFence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Of `lists` lists of k keys each, best first, one wave keeps, in place and in order, those not below a bound that k of them
+// reach, and returns their number. With d = ceil(k / lists) - 1, the J = ceil(k / (d + 1)) lists of the largest keys at
+// place d have d + 1 keys each that are not below the smallest of these.
+__device__ __forceinline__ int beamKeep(u64* keys, int lists, int k) {
+  const int lane = threadIdx.x & 63, d = (k + lists - 1) / lists - 1, n = lists * k;
+  waveFence();
+  const u64 mine = lane < lists ? keys[lane * k + d] : 0;
+  int above = 0;
+#pragma unroll 4
+  for (int i = 0; i < lists; ++i) above += keys[i * k + d] > mine;
+  const u64 least = lane < lists && above * (d + 1) < k ? ~mine : 0;
+  const u64 bound = ~waveMaxU64(static_cast<unsigned>(least >> 32), static_cast<unsigned>(least));
+  int kept = 0;
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const u64 key = i0 + lane < n ? keys[i0 + lane] : 0;
+    const bool in = i0 + lane < n && key >= bound;
+    const u64 all = __ballot(in);
+    waveFence();  // places at or in front of those just read
+    if (in) keys[kept + static_cast<int>(__popcll(all & ((u64{1} << lane) - 1)))] = key;
+    kept += static_cast<int>(__popcll(all));
+  }
+  waveFence();
+  return kept;
+}
+
+// an order-preserving key of a candidate; never 0
+__device__ __forceinline__ u64 orderOf(double c) {
+  const u64 u = static_cast<u64>(__double_as_longlong(c == 0.0 ? 0.0 : c));
+  return (u >> 63) ? ~u : u | 0x8000000000000000ull;
+}
+__device__ __forceinline__ double valueOf(u64 key) {
+  return __longlong_as_double(static_cast<long long>((key >> 63) ? key ^ 0x8000000000000000ull : ~key));
+}
+
+// Row `beam`'s k candidates, best first, by one wave: cand their keys (0: none left), tok their tokens.
+__device__ __forceinline__ void beamRow(const BeamParams& p, int beam, u64* heads, u64* cand, int* tok) {
   const int lane = threadIdx.x & 63;
   const int64_t at = static_cast<int64_t>(beam) * p.tiles;
   const float score = p.scores[beam];
   const float2 mine = lane < p.tiles ? p.sums[at + lane] : make_float2(-INFINITY, 0.0f);
   const uint2* lists = p.lists + at * p.k;
   const int entries = p.tiles * p.k;
+  waveFence();  // the row before
   for (int i0 = lane; i0 < entries; i0 += 64 * 8) {  // 8 loads in flight
     uint2 e[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[i] = lists[min(i0 + 64 * i, entries - 1)];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i0 + 64 * i < entries) heads[i0 + 64 * i] = e[i];
+      if (i0 + 64 * i < entries) heads[i0 + 64 * i] = pairOf(e[i].x, ~e[i].y);
   }
   const float m = waveMaxDpp(mine.x);
   double sum = mine.x == -INFINITY ? (mine.y == mine.y ? 0.0 : mine.y)
@@ -186,70 +235,53 @@ __device__ __forceinline__ void beamRow(const BeamParams& p, int beam, uint2* he
     const bool one = done && live;
     for (int j = lane; j < p.k; j += 64) {
       const int t = one ? (j == 0 ? p.eos[0] : j - 1 + (j - 1 >= p.eos[0])) : j;
-      tok[j] = t < p.v ? t : -1;
-      cand[j] = one && j == 0 ? static_cast<double>(score) : -INFINITY;
+      tok[j] = t;
+      cand[j] = t < p.v ? orderOf(one && j == 0 ? static_cast<double>(score) : -INFINITY) : 0;
     }
     return;
   }
   const double lse = static_cast<double>(m) + log(sum);
-  // the wave's own slice of LDS, written above by its other lanes
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  int next = 0;
-  uint2 h = lane < p.tiles ? heads[lane * p.k] : make_uint2(0u, 0u), mineOf{0u, 0u};  // lane j keeps the j-th best
-  for (int j = 0; j < p.k; ++j) {
-    const u64 top = waveMaxU64(h.x, ~h.y);
-    const unsigned bk = static_cast<unsigned>(top >> 32), bi = ~static_cast<unsigned>(top);
-    if (lane == j) mineOf = make_uint2(bk, bi);
-    if (bk != 0u && h.x == bk && h.y == bi) {
-      ++next;
-      h = next < p.k ? heads[lane * p.k + next] : make_uint2(0u, 0u);
-    }
-  }
-  if (lane < p.k) {
-    const double c = static_cast<double>(score) + (static_cast<double>(valueOf(mineOf.x)) - lse);
-    cand[lane] = mineOf.x != 0u && c == c ? c : -INFINITY;
-    tok[lane] = mineOf.x != 0u ? static_cast<int>(mineOf.y) : -1;  // fewer than k logits: none left
+  const int n = beamKeep(heads, p.tiles, p.k);
+  for (int i = lane; i < n; i += 64) {
+    const u64 key = heads[i];
+    const int rank = beamRank(heads, n, key, i);
+    if (rank >= p.k) continue;
+    const unsigned order = static_cast<unsigned>(key >> 32);  // 0: fewer than k logits, none left
+    const double c = static_cast<double>(score) + (static_cast<double>(valueOf(order)) - lse);
+    cand[rank] = order == 0u ? 0 : orderOf(c == c ? c : -INFINITY);
+    tok[rank] = static_cast<int>(~static_cast<unsigned>(key));
   }
 }
 
-// one workgroup: a wave per row (rows w, w + waves, ...), then the first wave, lane b at the head of row b's candidates
+// one workgroup: a wave per row (rows w, w + waves, ...), then a thread per candidate of the rows
 __global__ __launch_bounds__(1024) void beamPickKernel(BeamParams p) {
-  extern __shared__ uint2 heads[];  // [waves, tiles, k]
-  __shared__ double cand[kBeamMost][kBeamMost];
-  __shared__ int tok[kBeamMost][kBeamMost];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  extern __shared__ u64 heads[];  // [waves, tiles, k]
+  __shared__ u64 cand[kBeamMost * kBeamMost];
+  __shared__ int tok[kBeamMost * kBeamMost];
+  const int wave = threadIdx.x >> 6;
   for (int beam = wave; beam < p.b; beam += blockDim.x / 64)
-    beamRow(p, beam, heads + static_cast<int64_t>(wave) * p.tiles * p.k, cand[beam], tok[beam]);
+    beamRow(p, beam, heads + static_cast<int64_t>(wave) * p.tiles * p.k, cand + beam * p.k, tok + beam * p.k);
   __syncthreads();
-  if (wave != 0) return;
-  // (candidate, beam) as keys: an order-preserving map of the double; 0 where nothing is left
-  const bool over = lane < p.b && p.done[lane] != 0;
-  int next = 0;
-  double c = 0.0;
-  int t = -1;
-  u64 key = 0;
-  const auto head = [&] {
-    t = lane < p.b && next < p.k ? tok[lane][next] : -1;
-    c = t >= 0 ? cand[lane][next] : 0.0;
-    const u64 u = static_cast<u64>(__double_as_longlong(c == 0.0 ? 0.0 : c));
-    key = t < 0 ? 0 : (u >> 63) ? ~u : u | 0x8000000000000000ull;
-  };
-  head();
-  for (int j = 0; j < p.k; ++j) {
-    const u64 top = waveMaxU64(static_cast<unsigned>(key >> 32), static_cast<unsigned>(key));
-    const int who = __ffsll(static_cast<unsigned long long>(__ballot(key == top))) - 1;  // the lowest beam
-    if (lane == who) {
-      p.outScores[j] = static_cast<float>(c);
-      p.outParents[j] = who;
-      p.outTokens[j] = t;
-      bool end = over;
-      for (int e = 0; e < 4; ++e) end = end || t == p.eos[e];
-      p.outDone[j] = end ? 1 : 0;
-      ++next;
-      head();
+  for (int i = threadIdx.x; i < p.b * p.k; i += blockDim.x) {
+    const u64 key = cand[i];
+    const int beam = i / p.k;
+    // in front of it: those of its own row, and of each other row from the best on what is larger or, of a lower beam, equal
+    int rank = i - beam * p.k, l = beam == 0 ? 1 : 0, at = 0;
+    while (rank < p.k && l < p.b) {
+      const u64 other = at < p.k ? cand[l * p.k + at] : 0;
+      const bool more = at < p.k && (other > key || (other == key && l < beam));
+      rank += more;
+      at = more ? at + 1 : 0;
+      l = more ? l : l + 1 + (l + 1 == beam);
     }
+    if (rank >= p.k) continue;  // at least k are candidates: k <= B V
+    const int t = tok[i];
+    p.outScores[rank] = static_cast<float>(valueOf(key));
+    p.outParents[rank] = beam;
+    p.outTokens[rank] = t;
+    bool end = p.done[beam] != 0;
+    for (int e = 0; e < 4; ++e) end = end || t == p.eos[e];
+    p.outDone[rank] = end ? 1 : 0;
   }
 }
 

@@ -13,6 +13,8 @@ are traced values (or captured lk.Tensors), shapes may hold symbolic dims, and t
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import winograd as _wino
@@ -923,6 +925,11 @@ def argmax_f32_gpu(x):
     return _launch("argmax_f32_gpu", [x], [(x.shape[0],)], out_dtypes=[i64])
 
 
+@functools.lru_cache(maxsize=1024)
+def _beam_work(b, v, k) -> int:
+    return GpuContext.shared().lib.lk_hip_beam_select_workspace_bytes(b, v, k)
+
+
 def beam_select_f32_gpu(logits, scores, done, k, eos):
     """(MI355X backend) A beam search's step over logits f32[B, V], the beams' scores f32[B] and done i64[B]: the k best of
     the candidates scores[b] + logits[b, t] - log sum exp logits[b] (a beam with done[b] != 0 has one, its score at eos[0]),
@@ -945,7 +952,7 @@ def beam_select_f32_gpu(logits, scores, done, k, eos):
         raise OpError("scores must be f32[B], done i64[B]")
     if not (1 <= len(eos) <= 4 and all(0 <= e < v for e in eos)):
         raise OpError("eos must be 1 to 4 ids below V")
-    work = ctx.lib.lk_hip_beam_select_workspace_bytes(b, v, k) // 4
+    work = _beam_work(b, v, k) // 4
     best = torch.empty(k, dtype=torch.float32, device=ctx.device)
     picks = torch.empty((3, k), dtype=torch.int64, device=ctx.device)
     scratch = torch.empty(work, dtype=torch.float32, device=ctx.device)
