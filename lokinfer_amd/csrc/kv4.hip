@@ -22,49 +22,67 @@ namespace lkd {
 constexpr int KHD = 128;
 
 // ---- writing ----------------------------------------------------------------------------------------------------
-// One wave quantises a row's key (lanes 0..31) and value (lanes 32..63), 4 values per lane: x of the lane's
-// values 4 (lane % 32) ... kvBlock: the (sequence, kv head)'s key block; its value block lies valueOff bytes further.
-__device__ __forceinline__ void kv4PutRow(half4 x, char* kvBlock, int64_t valueOff, int64_t cap, int64_t row) {
-  const int lane = threadIdx.x & 63, l = lane & 31;
-  float v[4], hi = 0.0f, lo = 0.0f;
+// 32 lanes quantise a row's key (the first 16, 8 values per lane) and value: the lane's word of codes and its group's scale.
+struct Kv4Word {
+  unsigned word;
+  h16 scale;
+};
+__device__ __forceinline__ Kv4Word kv4Quantise(half8 x) {
+  const int lane = threadIdx.x & 63;
+  float v[8], hi = 0.0f, lo = 0.0f;
   bool bad = false;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < 8; ++e) {
     v[e] = static_cast<float>(x[e]);
     hi = fmaxf(hi, v[e]);
     lo = fminf(lo, v[e]);
     bad = bad || !(fabsf(v[e]) < INFINITY);
   }
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {  // the 8 lanes of a group
+  for (int o = 1; o < 4; o <<= 1) {  // the 4 lanes of a group
     hi = fmaxf(hi, __shfl_xor(hi, o, 64));
     lo = fminf(lo, __shfl_xor(lo, o, 64));
   }
-  const bool rowBad = __any(bad);
+  const bool rowBad = static_cast<unsigned>(__ballot(bad) >> (lane & 32)) != 0u;
   float s = q4Scale(hi, lo);
-  if (rowBad) s = lane < 32 ? __builtin_nanf("") : 0.0f;
-  unsigned word = 0;
+  if (rowBad) s = (lane & 16) ? 0.0f : __builtin_nanf("");
+  Kv4Word out{0u, static_cast<h16>(s)};
 #pragma unroll
-  for (int e = 0; e < 4; ++e) word |= q4Code(v[e], s) << q4Shift(4 * (l & 1) + e);
-  word |= __shfl_xor(word, 1, 64);
-  char* at = kvBlock + (lane < 32 ? 0 : valueOff);
-  if ((l & 1) == 0) *reinterpret_cast<unsigned*>(at + row * 64 + 2 * l) = word;
-  if ((l & 7) == 0) *reinterpret_cast<h16*>(at + cap * 64 + (l >> 3) * 2 * cap + 2 * row) = static_cast<h16>(s);
+  for (int e = 0; e < 8; ++e) out.word |= q4Code(v[e], s) << q4Shift(e);
+  return out;
 }
 
-// grid: rows / 4, kv heads
+// grid: T / 16, kv heads, B. A wave takes 4 rows, two at a time; the scales go through LDS, since a plane's neighbours are
+// neighbouring rows'.
+constexpr int kWriteRows = 16;
 __global__ __launch_bounds__(256) void kv4WriteKernel(char* __restrict__ kv, const h16* __restrict__ k,
-                                                      const h16* __restrict__ v, const int64_t* __restrict__ pos,
-                                                      unsigned rows, unsigned t, int kvh, int64_t cap) {
-  const int lane = threadIdx.x & 63, h = blockIdx.y;
-  const unsigned r = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (r >= rows) return;
-  const unsigned seq = r / t;
-  const int64_t row = pos[seq] + (r - seq * t);
-  if (row < 0 || row >= cap) return;  // uniform over the wave
-  const h16* src = (lane < 32 ? k : v) + (static_cast<int64_t>(r) * kvh + h) * KHD + 4 * (lane & 31);
-  const int64_t block = 72 * cap;
-  kv4PutRow(*reinterpret_cast<const half4*>(src), kv + (static_cast<int64_t>(seq) * 2 * kvh + h) * block, kvh * block, cap, row);
+                                                      const h16* __restrict__ v, const int64_t* __restrict__ pos, int t,
+                                                      int kvh, int64_t cap) {
+  __shared__ h16 scales[8][kWriteRows];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, h = blockIdx.y, seq = blockIdx.z;
+  const int first = blockIdx.x * kWriteRows;
+  const int64_t p0 = pos[seq];
+  char* kb = kv + (static_cast<int64_t>(seq) * 2 * kvh + h) * 72 * cap;
+  char* vb = kb + static_cast<int64_t>(kvh) * 72 * cap;
+  const auto inside = [&](int i) { return i < t && p0 >= -i && p0 < cap - i; };
+  half8 x[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int in = first + wave * 4 + 2 * i + (lane >> 5);
+    x[i] = half8{};
+    if (in < t) x[i] = ld8(((lane & 16) ? v : k) + ((static_cast<int64_t>(seq) * t + in) * kvh + h) * KHD + 8 * l);
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int in = wave * 4 + 2 * i + (lane >> 5);
+    const Kv4Word y = kv4Quantise(x[i]);
+    if (inside(first + in)) *reinterpret_cast<unsigned*>(((lane & 16) ? vb : kb) + (p0 + first + in) * 64 + 4 * l) = y.word;
+    if ((l & 3) == 0) scales[(lane & 16) / 4 + (l >> 2)][in] = y.scale;
+  }
+  __syncthreads();
+  const int in = threadIdx.x % kWriteRows, plane = threadIdx.x / kWriteRows;
+  if (plane < 8 && inside(first + in))
+    *reinterpret_cast<h16*>((plane >= 4 ? vb : kb) + cap * (64 + (plane & 3) * 2) + 2 * (p0 + first + in)) = scales[plane][in];
 }
 
 struct Kv4QkrParams {
@@ -117,8 +135,12 @@ __global__ __launch_bounds__(256) void kv4QkRopeKernel(Kv4QkrParams p) {
   __builtin_amdgcn_wave_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   const int64_t block = 72 * p.cap;
-  kv4PutRow(*reinterpret_cast<const half4*>(mine + 4 * lane), p.kv + (static_cast<int64_t>(seq) * 2 * p.kvh + (slot - p.qh)) * block,
-            p.kvh * block, p.cap, row);
+  const Kv4Word y = kv4Quantise(ld8(mine + 8 * (lane & 31)));  // the upper lanes as the lower ones
+  if (lane >= 32) return;
+  char* at = p.kv + (static_cast<int64_t>(seq) * 2 * p.kvh + (slot - p.qh) + (lane < 16 ? 0 : p.kvh)) * block;
+  const int l = lane & 15;
+  *reinterpret_cast<unsigned*>(at + row * 64 + 4 * l) = y.word;
+  if ((l & 3) == 0) *reinterpret_cast<h16*>(at + p.cap * 64 + (l >> 2) * 2 * p.cap + 2 * row) = y.scale;
 }
 
 // ---- reading ----------------------------------------------------------------------------------------------------
@@ -471,7 +493,6 @@ __global__ __launch_bounds__(256) void kv4ReorderKernel(char* __restrict__ kv, c
 namespace {
 
 bool al16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
-bool al8(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 7) == 0; }
 int launched() { return hipGetLastError() == hipSuccess ? 0 : 2; }
 constexpr int64_t kMostRows = int64_t{1} << 27;  // of a cache: a row's 16 words and a chunk of 64 rows fit 32 bits
 bool kvOk(const void* kv, int64_t b, int kvh, int64_t cap) {
@@ -509,11 +530,11 @@ extern "C" {
 int lk_hip_kv4_write(void* kv, const void* k, const void* v, const int64_t* pos, int64_t b, int64_t t, int kvh, int64_t cap,
                      void* stream) {
   using namespace lkd;
-  if (!kvOk(kv, b, kvh, cap) || !rowsOk(b, t) || !al8(k) || !al8(v)) return 1;
+  if (!kvOk(kv, b, kvh, cap) || !rowsOk(b, t) || !al16(k) || !al16(v)) return 1;
   if (t == 0) return 0;
-  hipLaunchKernelGGL(kv4WriteKernel, dim3(static_cast<unsigned>((b * t + 3) / 4), static_cast<unsigned>(kvh)), dim3(256), 0,
-                     static_cast<hipStream_t>(stream), static_cast<char*>(kv), static_cast<const h16*>(k),
-                     static_cast<const h16*>(v), pos, static_cast<unsigned>(b * t), static_cast<unsigned>(t), kvh, cap);
+  const dim3 grid(static_cast<unsigned>((t + kWriteRows - 1) / kWriteRows), static_cast<unsigned>(kvh), static_cast<unsigned>(b));
+  hipLaunchKernelGGL(kv4WriteKernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<char*>(kv),
+                     static_cast<const h16*>(k), static_cast<const h16*>(v), pos, static_cast<int>(t), kvh, cap);
   return launched();
 }
 
@@ -604,7 +625,7 @@ void runKv4Write(ExecCtx& ctx, const KernelArgs& a) {
              "kv4_write: kv u8[B, 2, kvh, 72 P] with P % 32 == 0, k and v f16[B T, kvh 128], pos i64[B]");
   status(ctx, lk_hip_kv4_write(a.ptrs[0], a.ptrs[1], a.ptrs[2], P<int64_t>(a, 3), b, rows / b, static_cast<int>(kvh), cap,
                                ctx.stream),
-         "kv4_write: kv must be 16-byte, k and v 8-byte aligned");
+         "kv4_write: kv, k and v must be 16-byte aligned");
 }
 
 // qknorm_rope_kv4_f16_gpu: qkv f16[B T, (qh + 2 kvh) 128], qg, kg f16[128], pos i64[B], kv (in place) -> q f16[B T, qh 128];
