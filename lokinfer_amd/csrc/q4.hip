@@ -315,6 +315,68 @@ __global__ __launch_bounds__(256) void w4StreamKernel(W4Params p) {
   }
 }
 
+// Some more rows: as w4SplitKernel, 32 rows by 16 columns per workgroup of 8 waves. A weight's operand, scaled before the
+// products (exact), serves both blocks of 16 rows, and the sums run through all of the wave's k.
+template <int G, int W, bool F32>
+__global__ __launch_bounds__(512) void w4RowsKernel(W4Params p) {
+  const Q4Masks masks;
+  constexpr int RB = 2, WAVES = 8, PER = 128 / G;
+  __shared__ float red[WAVES][W][RB][4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, a = lane & 15, kq = lane >> 4;
+  const int64_t tile = blockIdx.x, m0 = static_cast<int64_t>(blockIdx.y) * 16 * RB;
+  const h16* xr[RB];  // rows past M read the last one: their sums are not used
+#pragma unroll
+  for (int r = 0; r < RB; ++r) xr[r] = p.x + min<int64_t>(m0 + 16 * r + a, p.m - 1) * p.k;
+  f32x4 acc[W][RB];
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int r = 0; r < RB; ++r) acc[w][r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t kb = wave; kb < p.kb; kb += WAVES) {
+    W4Block<G, W> blk;
+    blk.load(p, tile, kb, lane);
+    half8 x[RB][4];
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t k = kb * 128 + 32 * i + 8 * kq;
+        x[r][i] = half8{};
+        if (k < p.k) x[r][i] = ld8(xr[r] + k);
+      }
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const unsigned word[4] = {blk.q[w].x, blk.q[w].y, blk.q[w].z, blk.q[w].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const h16 f = blk.s[w][i * PER / 4];
+        const half8 b = q4Ints(word[i], masks) * half8{f, f, f, f, f, f, f, f};
+#pragma unroll
+        for (int r = 0; r < RB; ++r) acc[w][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[r][i], b, acc[w][r], 0, 0, 0);
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w)
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) red[wave][w][r][e][lane] = acc[w][r][e];
+  __syncthreads();
+  // accumulator e of block r: row 16 r + 4 (l / 16) + e, column l % 16
+  for (int o = threadIdx.x; o < RB * 256; o += 64 * WAVES) {
+    const int l = o & 63, e = (o >> 6) & 3, r = o >> 8;
+    float y[W];
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      y[w] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v) y[w] += red[v][w][r][e][l];
+    }
+    w4Put<F32, W>(p, m0 + 16 * r + 4 * (l >> 4) + e, tile * 16 + (l & 15), y);
+  }
+}
+
 // More rows: workgroup of NW x KG waves, tile BM rows x NW 64 columns (SwiGLU: 32 of the gate's and the up weight's same 32).
 // Wave (nw, kg) takes all BM rows of its 64 columns over the k blocks kg, kg + KG, ... of 128 k; the KG sums meet in LDS. x goes
 // through LDS, a block ahead in registers; the weights go from memory straight into the registers of the one wave that
@@ -509,7 +571,7 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
     }
   } else {
     // 4 columns of a row per item
-    constexpr int COLS = W == 2 ? 32 : 64, ITEMS = NW * BM * COLS / 4 / THREADS;
+    constexpr int COLS = W == 2 ? 32 : 64, ALL = NW * BM * COLS / 4, ITEMS = (ALL + THREADS - 1) / THREADS;
     h16 add[ITEMS][4];
 #pragma unroll
     for (int t = 0; t < ITEMS; ++t) {
@@ -530,6 +592,7 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
     for (int t = 0; t < ITEMS; ++t) {
       const int o = threadIdx.x + t * THREADS, c = o % (COLS / 4) * 4, row = o / (COLS / 4) % BM, v = o / (COLS / 4 * BM);
       f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f}, u = y;
+      if (ALL % THREADS != 0 && o >= ALL) break;
 #pragma unroll
       for (int g = 0; g < KG; ++g) {
         const float* at = red + ((g * NW + v) * BM + row) * 64 + c;
@@ -575,12 +638,33 @@ void launchGemm(const lkd::W4Params& p, hipStream_t s) {
 }
 
 template <int G, int W, bool F32>
+void launchRows(const lkd::W4Params& p, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((p.n + 15) / 16), static_cast<unsigned>((p.m + 31) / 32));
+  hipLaunchKernelGGL((lkd::w4RowsKernel<G, W, F32>), grid, dim3(512), 0, s, p);
+}
+
+// A product of M rows by `cols` columns (both weights') on tiles of bm x bn: rounds of the chip's 256 workgroups, each about
+// a + K / b us. One round's us at K = 512, 2048, 6144: 32 x 64 5.3, 7.4, 13; 64 x 64 8.0, 10.6, 19; 128 x 256 14, 33, 88.
+double w4Us(int64_t m, int64_t cols, int64_t k, int bm, int bn, double a, double b) {
+  const int64_t groups = ((m + bm - 1) / bm) * ((cols + bn - 1) / bn);
+  return static_cast<double>((groups + 255) / 256) * (a + static_cast<double>(k) / b);
+}
+
+// Over 16 rows: the rows kernel against 32 x 64 tiles, us at 32 rows: K, N = 512, 2048 3.2 / 5.3; 2048, 4096 6.5 / 7.3; 6144,
+// 2048 13.8 / 12.6; 2048, 12288 15 / 8.7. The tiles against each other, us of 32 x 64 / 64 x 64 / 128 x 256: M, K, N = 128,
+// 2048, 4096 8.1 / 11 / 33; 256, 6144, 2048 14 / 20 / 81; 409, 2048, 2048 14 / 11 / 33; 409, 6144, 2048 26 / 21 / 89; 409,
+// 2048, 12288 61 / 57 / 38; 2048, 2048, 2048 57 / 56 / 39; 2048, 2048, 12288 297 / 274 / 109.
+template <int G, int W, bool F32>
 void launchW4(const lkd::W4Params& p, hipStream_t s) {
-  if (p.gamma) launchFew<1, G, W, F32, true>(p, s);
-  else if (p.m <= 4) launchFew<1, G, W, F32, false>(p, s);
-  else if (p.m <= 16) launchFew<4, G, W, F32, false>(p, s);
-  else if (((p.m + 127) / 128) * ((p.n * W + 255) / 256) >= 256) launchGemm<128, 4, 1, G, W, F32>(p, s);
-  else launchGemm<64, 1, 8, G, W, F32>(p, s);
+  if (p.gamma) return launchFew<1, G, W, F32, true>(p, s);
+  if (p.m <= 4) return launchFew<1, G, W, F32, false>(p, s);
+  if (p.m <= 16) return launchFew<4, G, W, F32, false>(p, s);
+  if ((p.m + 31) / 32 * ((p.n + 15) / 16) <= 256 && p.k <= 2048) return launchRows<G, W, F32>(p, s);
+  const double t32 = w4Us(p.m, p.n * W, p.k, 32, 64, 3.0, 400.0), t64 = w4Us(p.m, p.n * W, p.k, 64, 64, 6.6, 350.0),
+               t128 = w4Us(p.m, p.n * W, p.k, 128, 256, 6.0, 65.0);
+  if (t32 <= t64 && t32 <= t128) launchGemm<32, 1, 8, G, W, F32>(p, s);
+  else if (t64 <= t128) launchGemm<64, 1, 8, G, W, F32>(p, s);
+  else launchGemm<128, 4, 1, G, W, F32>(p, s);
 }
 
 template <int G>
@@ -638,7 +722,7 @@ int lk_hip_w4_gemm(const void* x, const void* gamma, const void* q, const void* 
   if (f32_out && (bias || res)) return 1;
   if (gamma && (m > 1 || !al16(gamma))) return 1;
   if (m == 0) return 0;
-  if (m > 64 * int64_t{65535} || k > (int64_t{1} << 23)) return 1;  // the grid; 32-bit offsets within 128 rows
+  if (m > 32 * int64_t{65535} || k > (int64_t{1} << 23)) return 1;  // the grid; 32-bit offsets within 128 rows
   const W4Params p{static_cast<const h16*>(x), static_cast<const h16*>(gamma),
                    {static_cast<const uint4*>(q), static_cast<const uint4*>(q2)},
                    {static_cast<const h16*>(s), static_cast<const h16*>(s2)},
