@@ -24,34 +24,58 @@ struct W4Layout {
   int group;
 };
 
-// one thread per (column of a tile, group): from w f16[K, N], or NT f16[N, K]
-template <bool NT>
+// One thread per (column of a tile, group), from w f16[K, N] (neighbouring threads on neighbouring columns) or NT f16[N, K]
+// (on neighbouring groups). The group's values stay in registers between the search for its scale and the codes.
+template <bool NT, int G>
 __global__ __launch_bounds__(256) void w4QuantizeKernel(const h16* __restrict__ w, unsigned* __restrict__ q,
-                                                        h16* __restrict__ s, W4Layout p) {
-  const int per = 128 / p.group;
-  const int64_t cols = (p.n + 15) / 16 * 16, total = cols * p.kb * per;
+                                                        h16* __restrict__ s, W4Layout p, bool wide) {
+  constexpr int PER = 128 / G;
+  const int64_t cols = (p.n + 15) / 16 * 16, groups = p.kb * PER, total = cols * groups;
   for (int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; id < total;
        id += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t n = id % cols, gi = id / cols, kb = gi / per;  // neighbouring threads on neighbouring columns
-    const int gb = static_cast<int>(gi - kb * per);
-    const int64_t k0 = gi * p.group;
-    const int live = n < p.n ? static_cast<int>(max<int64_t>(0, min<int64_t>(p.group, p.k - k0))) : 0;
-    const auto at = [&](int j) { return static_cast<float>(NT ? w[n * p.k + k0 + j] : w[(k0 + j) * p.n + n]); };
+    const int64_t major = id / (NT ? groups : cols), minor = id - major * (NT ? groups : cols);
+    const int64_t n = NT ? major : minor, gi = NT ? minor : major, kb = gi / PER, k0 = gi * G;
+    const int gb = static_cast<int>(gi - kb * PER);
+    const int live = n < p.n ? static_cast<int>(max<int64_t>(0, min<int64_t>(G, p.k - k0))) : 0;
+    half8 v[G / 8];
+#pragma unroll
+    for (int o = 0; o < G / 8; ++o) v[o] = half8{};
+    const auto at = [&](int j) { return NT ? w[n * p.k + k0 + j] : w[(k0 + j) * p.n + n]; };
+#pragma unroll
+    for (int o = 0; o < G / 8; ++o) {
+      if (live == G) {
+        if (NT && wide) {
+          v[o] = ld8(w + n * p.k + k0 + 8 * o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[o][e] = at(8 * o + e);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (8 * o + e < live) v[o][e] = at(8 * o + e);
+      }
+    }
     float hi = 0.0f, lo = 0.0f;
     bool bad = false;
-    for (int j = 0; j < live; ++j) {
-      const float v = at(j);
-      hi = fmaxf(hi, v);
-      lo = fminf(lo, v);
-      bad = bad || !(fabsf(v) < INFINITY);
-    }
+#pragma unroll
+    for (int o = 0; o < G / 8; ++o)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = static_cast<float>(v[o][e]);
+        hi = fmaxf(hi, x);
+        lo = fminf(lo, x);
+        bad = bad || !(fabsf(x) < INFINITY);
+      }
     const float sc = bad ? __builtin_nanf("") : q4Scale(hi, lo);
     const int64_t tile = (n >> 4) * p.kb + kb;
-    s[(tile * 16 + (n & 15)) * per + gb] = static_cast<h16>(sc);
-    for (int o = 0; o < p.group / 8; ++o) {
+    s[(tile * 16 + (n & 15)) * PER + gb] = static_cast<h16>(sc);
+#pragma unroll
+    for (int o = 0; o < G / 8; ++o) {
       unsigned word = 0;
-      for (int j = 0; j < 8; ++j) word |= (8 * o + j < live ? q4Code(at(8 * o + j), sc) : 8u) << q4Shift(j);
-      const int in = gb * p.group + 8 * o;  // k within the tile
+#pragma unroll
+      for (int e = 0; e < 8; ++e) word |= q4Code(static_cast<float>(v[o][e]), sc) << q4Shift(e);  // past K: 0, code 8
+      const int in = gb * G + 8 * o;  // k within the tile
       q[(tile * 64 + (n & 15) + 16 * ((in >> 3) & 3)) * 4 + (in >> 5)] = word;
     }
   }
@@ -688,9 +712,12 @@ int lk_hip_w4_quantize(const void* w, void* q, void* s, int64_t n, int64_t k, in
   const lkd::W4Layout p{n, k, (k + 127) / 128, group};
   const unsigned grid = gridFor((n + 15) / 16 * 16 * p.kb * (128 / group));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const auto kernel = nt ? lkd::w4QuantizeKernel<true> : lkd::w4QuantizeKernel<false>;
+  using lkd::w4QuantizeKernel;
+  const auto kernel = group == 32   ? (nt ? w4QuantizeKernel<true, 32> : w4QuantizeKernel<false, 32>)
+                      : group == 64 ? (nt ? w4QuantizeKernel<true, 64> : w4QuantizeKernel<false, 64>)
+                                    : (nt ? w4QuantizeKernel<true, 128> : w4QuantizeKernel<false, 128>);
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, static_cast<const lkd::h16*>(w), static_cast<unsigned*>(q),
-                     static_cast<lkd::h16*>(s), p);
+                     static_cast<lkd::h16*>(s), p, al16(w) && k % 8 == 0);
   return launched();
 }
 
