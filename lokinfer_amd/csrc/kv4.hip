@@ -374,30 +374,34 @@ __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1
     }
   }
   __syncthreads();
-  for (int o = threadIdx.x; o < rows * KHD; o += 64 * KW) {
-    const int r = o / KHD, d = o % KHD;
-    float mm = -INFINITY;
+  // 4 dims of a row per item
+  for (int o = threadIdx.x; o < rows * (KHD / 4); o += 64 * KW) {
+    const int r = o / (KHD / 4), d = o % (KHD / 4) * 4;
+    float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
     for (int w = 0; w < KW; ++w) mm = fmaxf(mm, ms[w][r]);
-    float ll = 0.0f, y = 0.0f;
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < KW; ++w) {
       const float f = ms[w][r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms[w][r] - mm);  // no key: zeros, or a NaN
       ll = fmaf(f, ls[w][r], ll);
-      y = fmaf(f, os[w][r][d], y);
+      const f32x4 part = *reinterpret_cast<const f32x4*>(&os[w][r][d]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fmaf(f, part[e], y[e]);
     }
     const unsigned i = (rb * ROWS + r) / group;
     const int64_t at = (seq * p.t + i) * p.qh + kvHead * group + (rb * ROWS + r - i * group);
     if (p.splits == 1) {
       const bool noRow = p0 < 0 || p0 >= p.cap - i;
-      p.out[at * KHD + d] = noRow ? static_cast<h16>(__builtin_nanf("")) : toH16(y / ll);
+      half4 out;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = noRow ? static_cast<h16>(__builtin_nanf("")) : toH16(y[e] / ll);
+      *reinterpret_cast<half4*>(p.out + at * KHD + d) = out;
     } else {
       float* pp = p.part + (at * p.splits + split) * (KHD + 2);
-      pp[2 + d] = y;
-      if (d == 0) {
-        pp[0] = mm;
-        pp[1] = ll;
-      }
+      *reinterpret_cast<float2*>(pp + 2 + d) = make_float2(y[0], y[1]);
+      *reinterpret_cast<float2*>(pp + 4 + d) = make_float2(y[2], y[3]);
+      if (d == 0) *reinterpret_cast<float2*>(pp) = make_float2(mm, ll);
     }
   }
 }
@@ -572,7 +576,7 @@ int64_t lk_hip_kv4_attention_workspace_bytes(int64_t b, int64_t t, int qh, int k
 int lk_hip_kv4_attention(const void* q, const void* kv, const int64_t* pos, void* out, int64_t b, int64_t t, int qh, int kvh,
                          int64_t cap, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace lkd;
-  if (!kvOk(kv, b, kvh, cap) || !rowsOk(b, t) || qh <= 0 || qh % kvh != 0 || !al16(q)) return 1;
+  if (!kvOk(kv, b, kvh, cap) || !rowsOk(b, t) || qh <= 0 || qh % kvh != 0 || !al16(q) || !al16(out)) return 1;
   if (t == 0) return 0;
   const int64_t need = lk_hip_kv4_attention_workspace_bytes(b, t, qh, kvh, cap);
   if (need > 0 && (!workspace || workspace_bytes < need || !al16(workspace))) return 3;
