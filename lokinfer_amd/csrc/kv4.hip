@@ -53,7 +53,8 @@ __device__ __forceinline__ Kv4Word kv4Quantise(half8 x) {
 }
 
 // grid: T / 16, kv heads, B. A wave takes 4 rows, two at a time; the scales go through LDS, since a plane's neighbours are
-// neighbouring rows'.
+// neighbouring rows'. 32768 rows of 8 heads 65 us (172 MB, 2.7 TB/s; one row per wave and single scales: 108); 409 rows 4.2 us,
+// of which 2.5 are a launch's.
 constexpr int kWriteRows = 16;
 __global__ __launch_bounds__(256) void kv4WriteKernel(char* __restrict__ kv, const h16* __restrict__ k,
                                                       const h16* __restrict__ v, const int64_t* __restrict__ pos, int t,
@@ -99,8 +100,9 @@ struct Kv4QkrParams {
   RopeTable tab;
 };
 
-// One wave per (row, q head) and (row, kv head), grid rows / 4, heads: a q head is normalized and rotated to q, a kv head's key likewise and
-// quantised with its value. Arithmetic and roundings of the norm and the rotation as qkRopeKvKernel's.
+// One wave per (row, q head) and (row, kv head), grid rows / 4, heads: a q head is normalized and rotated to q, a kv head's key
+// likewise and quantised with its value. Arithmetic and roundings of the norm and the rotation as qkRopeKvKernel's. 16 / 8 heads: 1 row 4.4
+// us, 409 8.5, 2048 27 (instructions: a rotation's sine and cosine, 4 values per lane).
 __global__ __launch_bounds__(256) void kv4QkRopeKernel(Kv4QkrParams p) {
   __shared__ __attribute__((aligned(16))) h16 rows[4][2 * KHD];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -144,7 +146,8 @@ __global__ __launch_bounds__(256) void kv4QkRopeKernel(Kv4QkrParams p) {
 }
 
 // ---- reading ----------------------------------------------------------------------------------------------------
-// one thread per 8 values, grid cap 16 / 256, blocks: blocks of 72 cap bytes -> f16 [blocks, cap, 128]
+// one thread per 8 values, grid cap 16 / 256, blocks: blocks of 72 cap bytes -> f16 [blocks, cap, 128]; HBM-bound, 512 blocks of
+// 1216 rows 35 us (204 MB, 5.8 TB/s)
 __global__ __launch_bounds__(256) void kv4ReadKernel(const char* __restrict__ kv, h16* __restrict__ out, int64_t blocks,
                                                      unsigned cap) {
   const Q4Masks masks;
@@ -187,6 +190,10 @@ struct Kv4Params {
 // Keys from the longest row's end on have their weight and their value's scale set to zero, whatever the memory holds there.
 // The sums are rescaled to a new maximum only where it exceeds the one they stand at by 2^8: until then weights reach 2^8,
 // which changes no relative precision, and nearly every tile brings some row a slightly larger score.
+// 16 / 8 heads: one query over 417 rows 6.6 us and over 32768 12.6 + 4.1 of the joining launch (38 MB, 2.3 TB/s): latency, of one
+// chunk in the first. 2048 queries over as many rows 46 us, 370 TFLOP/s: bound by VALU (some 70% of the cycles, MFMA 30%), half of it
+// the codes' conversion, which 32 rows share, half the softmax. Tiles of f16 made once per call and shared through LDS took
+// 6 + 50; more rows a wave leave one wave a SIMD (61 us).
 constexpr float kGrowth = 8.0f;
 template <int RB, int KW>
 __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1 ? 4 : 2))) void kv4AttnKernel(Kv4Params p) {
@@ -406,7 +413,8 @@ __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1
   }
 }
 
-// one workgroup per (q head, query): the splits' partials, 32 at a time
+// one workgroup per (q head, query): the splits' partials, 32 at a time, all loads in flight together: 4 us, a launch and one
+// latency
 __global__ __launch_bounds__(128) void kv4MergeKernel(Kv4Params p) {
   const int d = threadIdx.x;
   const unsigned qi = blockIdx.y, seq = qi / p.t;
@@ -442,9 +450,9 @@ __global__ __launch_bounds__(128) void kv4MergeKernel(Kv4Params p) {
 
 // ---- moving caches between sequences ------------------------------------------------------------------------------
 // One thread per 16 bytes of codes or of a scale plane (2 bytes behind its last whole 8 rows) of a (layer, key or value, kv
-// head)'s live rows: it reads the piece of the
-// parent of every sequence whose parent is another, then writes them, so that no write comes before a read of the same
-// bytes. MB: B rounded up, so that the pieces stay in registers, all reads in flight together.
+// head)'s live rows: it reads the piece of the parent of every sequence whose parent is another, then writes them, so that no
+// write comes before a read of the same bytes. MB: B rounded up, so that the pieces stay in registers, all reads in flight
+// together. HBM-bound: 2 layers of 16 sequences of 1100 rows 20 us (81 MB read and written, 4.0 TB/s), of 4 of 448 rows 4.3.
 constexpr int kMaxBeams = 32;
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 template <int MB, typename T>
@@ -505,17 +513,17 @@ bool kvOk(const void* kv, int64_t b, int kvh, int64_t cap) {
 // rows of a call: they are counted in 32 bits
 bool rowsOk(int64_t b, int64_t t) { return t >= 0 && t <= 0x7FFFFFFF && b <= 65535 && b * t <= 0x7FFFFFFF; }
 
-// Row blocks and waves of a workgroup. us of (1, 8) / (1, 4) / (2, 8) / (2, 4) by T queries over P rows, 16 / 8 heads:
-// 256, 512: 9.1 / 9.1 / 13 / 13; 512, 512: 12.7 / 10.6 / 13.4 / 13.4; 600, 2048: 40 / 39 / 43 / 39; 1024, 2048: 51 / 48 / 45 / 41;
-// 2048, 2048: 75 / 63 / 69 / 55; 2048, 8192: 344 / 337 / 268 / 253; 256, 32768: 204 / 240 / 246 / 302; 409, 32768: 338 / 345 /
-// 254 / 302. (Expanded once to f16 and run through the f16 op's tiles: 15, 15, 49, 46, 55, 269, 277 and 310.)
+// Row blocks and waves of a workgroup. us of (1, 8) / (1, 4) / (2, 8) / (2, 4) by T queries over P rows, 16 / 8 heads: 256, 512
+// 8.1 / 8.1 / 11 / 10; 512, 512 11 / 9.9 / 11 / 11; 1024, 1024 24 / 23 / 23 / 20; 300, 2048 27 / 28 / 22 / 23; 600, 2048 37 / 37 /
+// 37 / 35; 2048, 2048 61 / 60 / 57 / 46; 2048, 8192 307 / 316 / 244 / 235; 256, 32768 194 / 237 / 241 / 294; 409, 32768 329 /
+// 350 / 250 / 295.
 struct Kv4Shape {
   int rb, kw;
 };
 Kv4Shape kv4Shape(int64_t b, int64_t rows, int kvh, int64_t cap) {
   const int64_t groups = b * kvh * ((rows + 15) / 16);
   if (groups <= 256) return {1, 8};
-  if (groups <= 640 && cap <= 2048) return {1, 4};
+  if (groups <= 640 && cap <= 1024) return {1, 4};
   return groups <= 640 ? Kv4Shape{2, 8} : Kv4Shape{2, 4};
 }
 
