@@ -350,14 +350,16 @@ int lk_hip_w4_pack(const void* codes, const void* scales, void* q, void* s, int*
 /* q, s -> w f16[K, N], exact */
 int lk_hip_w4_unpack(const void* q, const void* s, void* w, int64_t n, int64_t k, int group, void* stream);
 /* out [M, N] = x f16[M, K] @ W (f32 sums): f16, + bias f16[N], + res f16[M, N]; silu(x @ W) * (x @ W2) with q2, s2; f32
- * with f32_out. gamma f16[K] (M = 1, else null): x is rmsnorm(x, gamma, eps) first. K % 8 == 0; x, gamma 16-byte aligned. */
+ * with f32_out. gamma f16[K] (M = 1, else null): x is rmsnorm(x, gamma, eps) first. K % 8 == 0;
+ * K <= 2^23, M <= 2097120; x, gamma 16-byte aligned. */
 int lk_hip_w4_gemm(const void* x, const void* gamma, const void* q, const void* s, const void* q2, const void* s2,
                    const void* bias, const void* res, void* out, int64_t m, int64_t n, int64_t k, int group, int f32_out,
                    float eps, void* stream);
 
 /* ---- key / value caches in 4 bits (MI355X backend): u8 [B, 2, kvh, 72 P], P rows (a multiple of 32) per (sequence, keys
  *      or values, kv head): first 64 bytes of codes a row, then the scales, f16 [4, P] (groups of 32 of the head's 128 values);
- *      16-byte aligned. pos: a device i64[B], the position of each sequence's first row of the call. ---- */
+ *      16-byte aligned, as are q, k, v and qkv; B <= 65535, P <= 2^27. pos: a device i64[B], the position of each sequence's
+ *      first row of the call. ---- */
 /* k, v f16[B T, kvh 128] -> rows pos[b] .. of sequence b; rows outside the cache are dropped. A row whose key or value is not
  * finite is held so that a query that sees it gets NaN. */
 int lk_hip_kv4_write(void* kv, const void* k, const void* v, const int64_t* pos, int64_t b, int64_t t, int kvh, int64_t cap,

@@ -637,7 +637,7 @@ void runKv4Write(ExecCtx& ctx, const KernelArgs& a) {
              "kv4_write: kv u8[B, 2, kvh, 72 P] with P % 32 == 0, k and v f16[B T, kvh 128], pos i64[B]");
   status(ctx, lk_hip_kv4_write(a.ptrs[0], a.ptrs[1], a.ptrs[2], P<int64_t>(a, 3), b, rows / b, static_cast<int>(kvh), cap,
                                ctx.stream),
-         "kv4_write: kv, k and v must be 16-byte aligned");
+         "kv4_write: kv, k and v must be 16-byte aligned, B at most 65535, P at most 2^27");
 }
 
 // qknorm_rope_kv4_f16_gpu: qkv f16[B T, (qh + 2 kvh) 128], qg, kg f16[128], pos i64[B], kv (in place) -> q f16[B T, qh 128];
@@ -651,14 +651,14 @@ void runKv4Qkr(ExecCtx& ctx, const KernelArgs& a) {
   status(ctx, lk_hip_kv4_qknorm_rope(a.ptrs[0], a.ptrs[1], a.ptrs[2], P<int64_t>(a, 3), a.ptrs[4], a.ptrs[5], b, rows / b,
                                      static_cast<int>(qw / 128), static_cast<int>(kvh), cap, F(a, 0, 1e-6f), F(a, 1, 1e6f),
                                      ctx.stream),
-         "qknorm_rope_kv4: qkv and kv must be 16-byte aligned");
+         "qknorm_rope_kv4: qkv and kv must be 16-byte aligned, B and heads at most 65535, P at most 2^27");
 }
 
 // kv4_read_f16_gpu: kv u8[blocks, 72 P] -> f16[blocks, P, 128]
 void runKv4Read(ExecCtx& ctx, const KernelArgs& a) {
   LK_REQUIRE(ctx, kv4Layout(2, a.ints[1]) && a.ints[2] == a.ints[0] && a.ints[3] == a.ints[1] / 72 && a.ints[4] == 128,
              "kv4_read: kv u8[blocks, 72 P] with P % 32 == 0, out f16[blocks, P, 128]");
-  status(ctx, lk_hip_kv4_read(a.ptrs[0], a.ptrs[1], a.ints[0], a.ints[3], ctx.stream), "kv4_read: launch failed");
+  status(ctx, lk_hip_kv4_read(a.ptrs[0], a.ptrs[1], a.ints[0], a.ints[3], ctx.stream), "kv4_read: kv must be 16-byte aligned, P at most 2^27");
 }
 
 // attention_kv4_f16_gpu: q f16[B T, qh 128], kv u8[B, 2, kvh, 72 P], pos i64[B] -> out f16[B T, qh 128], work f32[n]
@@ -670,7 +670,7 @@ void runKv4Attention(ExecCtx& ctx, const KernelArgs& a) {
   const int rc = lk_hip_kv4_attention(a.ptrs[0], a.ptrs[1], P<int64_t>(a, 2), a.ptrs[3], b, rows / b,
                                       static_cast<int>(width / 128), static_cast<int>(kvh), cap, a.ptrs[4], a.ints[9] * 4,
                                       ctx.stream);
-  status(ctx, rc, rc == 3 ? "attention_kv4: work is too small" : "attention_kv4: q and kv must be 16-byte aligned");
+  status(ctx, rc, rc == 3 ? "attention_kv4: work is too small" : "attention_kv4: q and kv must be 16-byte aligned, B at most 65535, P at most 2^27");
 }
 
 // kv4_reorder_gpu: kv u8[L, B, 2, kvh, 72 P], parents i64[B], n i64[1] (in place)

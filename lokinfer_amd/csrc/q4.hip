@@ -857,7 +857,7 @@ void runGemmW4(ExecCtx& ctx, const KernelArgs& a) {
              "gemm_w4: out [M, N], bias f16[N], res f16[M, N]");
   status(ctx, lk_hip_w4_gemm(x, g, q[0], s[0], q[1], s[1], bias, res, a.ptrs[ptr], m, n, k, static_cast<int>(group),
                              EPI == W4_LOGITS, F(a, 0, 1e-6f), ctx.stream),
-         "gemm_w4: K must be a multiple of 8 and the operands 16-byte aligned");
+         "gemm_w4: K must be a multiple of 8 and at most 2^23, M at most 2097120, the operands 16-byte aligned");
 }
 
 }  // namespace

@@ -308,7 +308,7 @@ def beam_search(model: Qwen3Lm, ids: np.ndarray, audio: np.ndarray, beams: int, 
         raise ValueError(f"kv must hold {beams} sequences of {T + max_new - 1} positions")
     logits, _ = _prefill(model, ids, audio, chunk, kv)
     scores, done = (Tensor(torch.zeros(1, dtype=t, device=dev)) for t in (torch.float32, torch.int64))
-    dummy = model._dev(np.zeros((1, model.cfg.d), np.float16), np.float16)
+    dummy = model._dev(np.zeros((beams, model.cfg.d), np.float16), np.float16)  # a row each, if all take the audio token
     tokens = torch.full((beams, max_new), eos[0], dtype=torch.int64, device=dev)
     length = torch.zeros(beams, dtype=torch.int64, device=dev)
     for n in range(max_new):

@@ -132,6 +132,22 @@ def test_caches_past_4_gib(gpu):
             assert np.abs(got[h] - ref).max() <= 2.0 ** -11 * np.abs(ref).max() + 2.0 ** -22 * (8 + np.sqrt(cap))
 
 
+def test_reorder_past_4_gib(gpu):
+    """Two layers of two sequences of 8 heads and 2 Mi rows (9.7 GB): the last head's values of the last sequence."""
+    q4 = gpu.ops.q4_gpu
+    cap = 1 << 21
+    kv = q4.kv4_cache(2, 8, cap, layers=2)
+    assert kv.nbytes > 1 << 33
+    kv.t[:, 0].fill_(7)
+    n = 45
+    i64 = lambda *v: gpu.Tensor(torch.tensor(v, device="cuda"))  # noqa: E731
+    q4.kv4_reorder_gpu(kv, i64(0, 0), i64(n))
+    codes = kv.t[..., : 64 * cap].unflatten(-1, (cap, 64))
+    scales = kv.t[..., 64 * cap:].unflatten(-1, (4, cap, 2))
+    for part, rows in ((codes[:, 1], -2), (scales[:, 1], -2)):
+        assert (part.narrow(rows, 0, n) == 7).all() and (part.narrow(rows, n, 200) == 0).all()
+
+
 def test_weights_past_4_gib(gpu):
     """K = 4096, N = 2.2 million: 4.5 GB of codes; the last columns against the same columns as a weight of their own."""
     lk, q4 = gpu, gpu.ops.q4_gpu

@@ -105,6 +105,26 @@ def test_beam_search(small, beams, max_new, penalty):
             assert got[0] == greedy[:max_new]
 
 
+def test_beams_that_take_the_audio_token(small, monkeypatch):
+    """An audio id among the generated ones is embedded as a row of zeros for every beam that took it."""
+    from lokinfer_amd.f16_gpu import PAD_ID
+    from lokinfer_amd.runtime import check_device_errors
+
+    M, _, _, ids = small
+    cfg = M.Qwen3Config(layers=1, d=256, qh=2, kvh=1, ffn=256, vocab=PAD_ID + 1)
+    lm = M.Qwen3Lm(M.random_weights(cfg, 5), cfg, variant="q4")
+    select = M.ops.beam_select_f32_gpu
+
+    def pads(*args):
+        s, parents, tok, done = select(*args)
+        return s, parents, type(tok)(torch.full_like(tok.t, PAD_ID)), done
+
+    monkeypatch.setattr(M.ops, "beam_select_f32_gpu", pads)
+    got = M.beam_search(lm, ids, np.zeros((0, cfg.d), np.float16), 3, 4, eos=(1999,))
+    check_device_errors()
+    assert got[0] == [PAD_ID] * 4 and np.isfinite(got[1])
+
+
 def test_refusals(small):
     M, cfg, sd, ids = small
     lm = M.Qwen3Lm(sd, cfg, variant="q4")
