@@ -56,15 +56,24 @@ struct RopeTable {
   float invf[64];
 };
 
-__device__ __forceinline__ void ropePair(float lo, float hi, int64_t p, float invf, h16& olo, h16& ohi) {
+__device__ __forceinline__ void ropeAngle(int64_t p, float invf, float& c, float& s) {
   const float ang = static_cast<float>(p) * invf;
   double sd, cd;
   sincos(static_cast<double>(ang), &sd, &cd);  // one routine in every kernel (the compiler may merge sin + cos)
-  const float c = static_cast<float>(cd), s = static_cast<float>(sd);
+  c = static_cast<float>(cd), s = static_cast<float>(sd);
+}
+
+__device__ __forceinline__ void ropeRotate(float lo, float hi, float c, float s, h16& olo, h16& ohi) {
   // explicit fma forms: every kernel that rotates computes the same bits (no contraction choice left to the
   // compiler, which could fuse either product)
   olo = toH16(fmaf(lo, c, -(hi * s)));
   ohi = toH16(fmaf(hi, c, lo * s));
+}
+
+__device__ __forceinline__ void ropePair(float lo, float hi, int64_t p, float invf, h16& olo, h16& ohi) {
+  float c, s;
+  ropeAngle(p, invf, c, s);
+  ropeRotate(lo, hi, c, s, olo, ohi);
 }
 
 __device__ __forceinline__ float siluMul(float g, float u) { return g / (1.0f + expf(-g)) * u; }

@@ -116,22 +116,33 @@ __global__ __launch_bounds__(256) void kv4QkRopeKernel(Kv4QkrParams p) {
   if (!isQ && (row < 0 || row >= p.cap)) return;
   const h16* x = p.qkv + r * width + slot * KHD;
   const h16* g = isQ ? p.qg : p.kg;
-  const float f = rmsFactor(rowSumSq(x, KHD, lane), KHD, p.eps);
+  // the loads first, the angle while they are on their way
+  const half8 own = lane < KHD / 8 ? ld8(x + 8 * lane) : half8{};  // rowSumSq's piece of a head
+  const h16 lo = x[lane], hi = x[lane + 64], glo = g[lane], ghi = g[lane + 64];
+  h16 vlo{}, vhi{};
+  if (!isQ) {
+    const h16* v = x + static_cast<int64_t>(p.kvh) * KHD;
+    vlo = v[lane];
+    vhi = v[lane + 64];
+  }
+  float c, s, sum = 0.0f;
+  ropeAngle(row, p.tab.invf[lane], c, s);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum = fmaf(static_cast<float>(own[e]), static_cast<float>(own[e]), sum);
+  const float f = rmsFactor(waveSum(sum), KHD, p.eps);
   h16 a, b;
-  ropePair(static_cast<float>(rmsElem(x[lane], g[lane], f)), static_cast<float>(rmsElem(x[lane + 64], g[lane + 64], f)),
-           row, p.tab.invf[lane], a, b);
+  ropeRotate(static_cast<float>(rmsElem(lo, glo, f)), static_cast<float>(rmsElem(hi, ghi, f)), c, s, a, b);
   if (isQ) {
     h16* o = p.q + r * p.qh * KHD + slot * KHD;
     o[lane] = a;
     o[lane + 64] = b;
     return;
   }
-  const h16* v = x + static_cast<int64_t>(p.kvh) * KHD;
   h16* mine = rows[wave];
   mine[lane] = a;
   mine[lane + 64] = b;
-  mine[KHD + lane] = v[lane];
-  mine[KHD + lane + 64] = v[lane + 64];
+  mine[KHD + lane] = vlo;
+  mine[KHD + lane + 64] = vhi;
   // this wave's own slice: its LDS operations complete in order
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();

@@ -223,32 +223,63 @@ __global__ __launch_bounds__(64 * WAVES) void w4SplitKernel(W4Params p) {
   for (int w = 0; w < W; ++w)
 #pragma unroll
     for (int r = 0; r < RU; ++r) acc[w][r] = 0.0f;
+  // With a norm in front (one row): the row, the gains and the weights are all loaded before the first is waited for; a lane
+  // normalizes one 16-byte piece of the wave's U blocks and the wave's LDS hands them round. Rows 1 .. of the operand repeat
+  // row 0: their sums are not stored.
+  constexpr int AHEAD = RMS ? 4 : 0;  // the lane's first pieces of the sum of squares, which has rowSumSq's order
+  __shared__ __attribute__((aligned(16))) h16 normed[RMS ? WAVES : 1][U * 128];
+  half8 sq[AHEAD + 1];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    sq[j] = half8{};
+    if (lane + 64 * j < p.k / 8) sq[j] = ld8(p.x + 8 * (lane + 64 * j));
+  }
   float rf = 1.0f;
   for (int64_t k0 = wave; k0 < p.kb; k0 += U * WAVES) {
     W4Block<G, W> blk[U];
-    half8 x[U][4];
+    half8 x[U][4], piece{}, gain{};
+    if constexpr (RMS) {
+      const int64_t k = (k0 + (lane >> 4) * WAVES) * 128 + 8 * (lane & 15);
+      if (lane < 16 * U && k < p.k) {
+        piece = ld8(p.x + k);
+        gain = ld8(p.gamma + k);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) blk[u].load(p, tile, min<int64_t>(k0 + u * WAVES, p.kb - 1), lane);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t k = (k0 + u * WAVES) * 128 + 32 * i + 8 * kq;
-        x[u][i] = half8{};
-        if (row < p.m && k < p.k) x[u][i] = ld8(p.x + row * p.k + k);
-      }
     if constexpr (RMS) {
-      if (k0 == wave) rf = rmsFactor(rowSumSq(p.x, p.k, lane), p.k, p.eps);
+      if (k0 == wave) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum = fmaf(static_cast<float>(sq[j][e]), static_cast<float>(sq[j][e]), sum);
+        for (int64_t c = lane + 64 * AHEAD; c < p.k / 8; c += 64) {
+          const half8 v = ld8(p.x + 8 * c);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sum = fmaf(static_cast<float>(v[e]), static_cast<float>(v[e]), sum);
+        }
+        rf = rmsFactor(waveSum(sum), p.k, p.eps);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) piece[e] = rmsElem(piece[e], gain[e], rf);
+      __builtin_amdgcn_wave_barrier();
+      if (lane < 16 * U) st8(&normed[wave][8 * lane], piece);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[u][i] = ld8(&normed[wave][128 * u + 32 * i + 8 * kq]);
+    } else {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int64_t k = (k0 + u * WAVES) * 128 + 32 * i + 8 * kq;
-          if (row < p.m && k < p.k) {
-            const half8 gv = ld8(p.gamma + k);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[u][i][e] = rmsElem(x[u][i][e], gv[e], rf);
-          }
+          x[u][i] = half8{};
+          if (row < p.m && k < p.k) x[u][i] = ld8(p.x + row * p.k + k);
         }
     }
 #pragma unroll
