@@ -950,18 +950,18 @@ def beam_select_f32_gpu(logits, scores, done, k, eos):
         raise OpError("B and k at most 32, V at most 262144, k <= B V")
     if s.shape != (b,) or d.shape != (b,):
         raise OpError("scores must be f32[B], done i64[B]")
-    if not (1 <= len(eos) <= 4 and all(0 <= e < v for e in eos)):
+    if not (1 <= len(eos) <= 4 and min(eos) >= 0 and max(eos) < v):
         raise OpError("eos must be 1 to 4 ids below V")
     work = _beam_work(b, v, k) // 4
-    best = torch.empty(k, dtype=torch.float32, device=ctx.device)
-    picks = torch.empty((3, k), dtype=torch.int64, device=ctx.device)
-    scratch = torch.empty(work, dtype=torch.float32, device=ctx.device)
+    best = x.new_empty(k)
+    picks = d.new_empty((3, k))
+    scratch = x.new_empty(work)
     at = picks.data_ptr()
     ctx.run("beam_select_f32_gpu",
             (x.data_ptr(), s.data_ptr(), d.data_ptr(), best.data_ptr(), at, at + 8 * k, at + 16 * k, scratch.data_ptr()),
             (b, v, b, b, k, k, k, k, work, *(int(e) for e in eos)), ())
-    picks = picks.unbind(0)
-    return (Tensor(best), *(Tensor(t) for t in picks))
+    parents, tokens, ended = picks.unbind(0)
+    return Tensor(best), Tensor(parents), Tensor(tokens), Tensor(ended)
 
 
 def lstm_bidir_t_f32_gpu(x, w_ih, w_hh_t, b):

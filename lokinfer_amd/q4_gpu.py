@@ -93,7 +93,16 @@ class PackedWeight4:
         check(isinstance(s, Tensor) and s.dtype == f16 and tuple(s.shape) == tiles + (16, 128 // group),
               "s does not fit the shape and group")
         check(q.t.is_cuda and q.t.device == s.t.device, "q and s must be on one GPU")
-        self.q, self.s, self.shape, self.group = q, s, (k, n), group
+        self._q, self._s, self.shape, self.group = q.t, s.t, (k, n), group
+        self._dims = (*q.shape, *s.shape)
+
+    @property
+    def q(self) -> Tensor:
+        return Tensor(self._q)
+
+    @property
+    def s(self) -> Tensor:
+        return Tensor(self._s)
 
 
 def _w4_empty(k, n, group):
@@ -138,14 +147,15 @@ def pack_w4(w, scales=None, group: int = 64, nt: bool = False) -> PackedWeight4:
 def unpack_w4_f16_gpu(w: PackedWeight4):
     """The weight's values, f16[K, N] (exact)."""
     out = _empty(_w(w).shape)
-    _call("unpack_w4_f16_gpu", [w.q.t, w.s.t, out], [w.group])
+    _call("unpack_w4_f16_gpu", [w._q, w._s, out], [w.group])
     return Tensor(out)
 
 
 def _w(w) -> PackedWeight4:
     if not isinstance(w, PackedWeight4):
         raise OpError("the weight must be a PackedWeight4 (pack_w4)")
-    _arg(w.q, _I32, 3, "the weight")
+    if w._q.get_device() != _index:
+        _arg(w.q, _I32, 3, "the weight")
     return w
 
 
@@ -158,26 +168,31 @@ def _gemm(name, x, w, w2=None, extra=None, norm=None, dtype=_F16):
         raise OpError(f"x [M, K] and w [K, N]: inner dims differ: {tuple(xt.shape)}, {w.shape}")
     if k % 8:
         raise OpError("K must be a multiple of 8")
-    ops, floats = [xt], ()
+    out = xt.new_empty((m, n), dtype=dtype)
+    ptrs, ints, floats = [xt.data_ptr()], [m, k], ()
     if norm is not None:
         g = _arg(norm[0], _F16, 1, "g")
         if g.shape[0] != k:
             raise OpError("g must be f16[K]")
-        ops.append(g)
+        ptrs.append(g.data_ptr())
+        ints.append(k)
         floats = (float(norm[1]),)
-    ops += [w.q.t, w.s.t]
+    ptrs += (w._q.data_ptr(), w._s.data_ptr())
+    ints += w._dims
     if w2 is not None:
         if _w(w2).shape != w.shape or w2.group != w.group:
             raise OpError("both weights must have one shape and group")
-        ops += [w2.q.t, w2.s.t]
+        ptrs += (w2._q.data_ptr(), w2._s.data_ptr())
+        ints += w2._dims
     if extra is not None:
         t = _arg(extra[0], _F16, extra[1], extra[2])
-        if tuple(t.shape) != ((m, n) if extra[1] == 2 else (n,)):
+        if t.shape != ((m, n) if extra[1] == 2 else (n,)):
             raise OpError(f"{extra[2]} must be f16{'[M, N]' if extra[1] == 2 else '[N]'}")
-        ops.append(t)
-    out = _empty((m, n), dtype)
-    ops.append(out)
-    _call(name, ops, (w.group,), floats)
+        ptrs.append(t.data_ptr())
+        ints += t.shape
+    ptrs.append(out.data_ptr())
+    ints += (m, n, w.group)
+    _run(name, ptrs, ints, floats)
     return Tensor(out)
 
 
@@ -274,7 +289,10 @@ def kv4_write_f16_gpu(kv, k, v, pos):
     key, val = _rows(k, kt.shape[0], "k"), _arg(v, _F16, 2, "v")
     if val.shape != key.shape or key.shape[1] != HD * kt.shape[2]:
         raise OpError("k, v must be f16[B T, kvh 128]")
-    _call("kv4_write_f16_gpu", [kt, key, val, pt])
+    b, two, kvh, row = kt.shape
+    rows, width = key.shape
+    _run("kv4_write_f16_gpu", (kt.data_ptr(), key.data_ptr(), val.data_ptr(), pt.data_ptr()),
+         (b, two, kvh, row, rows, width, rows, width, b))
 
 
 def qknorm_rope_kv4_f16_gpu(qkv, qg, kg, pos, kv, eps=1e-6, theta=1e6):
@@ -298,7 +316,7 @@ def kv4_read_f16_gpu(kv):
     """The values that a cache (or any u8[..., 72 P] part of one) holds: f16[..., P, 128]."""
     cap = kv4_capacity(kv)
     kt = _arg(kv, _U8, kv.t.dim(), "kv")
-    out = _empty((*kt.shape[:-1], cap, HD))
+    out = kt.new_empty((*kt.shape[:-1], cap, HD), dtype=_F16)
     blocks = kt.numel() // (ROW * cap)
     _run("kv4_read_f16_gpu", (kt.data_ptr(), out.data_ptr()), (blocks, ROW * cap, blocks, cap, HD))
     return Tensor(out)
@@ -316,8 +334,11 @@ def attention_kv4_f16_gpu(q, kv, pos):
     if width <= 0 or width % (HD * kvh):
         raise OpError("q must be f16[B T, qh 128], qh a multiple of kvh")
     need = _attention_bytes(b, rows // b, width // HD, kvh, row // ROW)
-    out = _empty((rows, width))
-    _call("attention_kv4_f16_gpu", [qt, kt, pt, out, _empty((-(-need // 4),), _F32) if need else _NO_WORK])
+    out = qt.new_empty((rows, width))
+    words = -(-need // 4)
+    work = qt.new_empty((words,), dtype=_F32) if need else _NO_WORK
+    _run("attention_kv4_f16_gpu", (qt.data_ptr(), kt.data_ptr(), pt.data_ptr(), out.data_ptr(), work.data_ptr()),
+         (rows, width, b, 2, kvh, row, b, rows, width, words))
     return Tensor(out)
 
 
@@ -332,7 +353,7 @@ def kv4_reorder_gpu(kv, parents, n):
         raise OpError("L kvh must be at most 32767")
     if pt.shape[0] != b or nt.shape[0] != 1:
         raise OpError("parents must be i64[B], n i64[1]")
-    _call("kv4_reorder_gpu", [kt, pt, nt])
+    _run("kv4_reorder_gpu", (kt.data_ptr(), pt.data_ptr(), nt.data_ptr()), (layers, b, two, kvh, row, b, 1))
 
 
 __all__ = [n for n in dir() if n.endswith(("_f16_gpu", "_reorder_gpu"))] + ["pack_w4", "PackedWeight4", "kv4_cache",

@@ -15,6 +15,7 @@ from ._lib import LokinferError, check_device_errors, lib
 from .graph import current_graph
 
 WORKSPACE_BYTES = 64 << 20
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 class GpuContext:
@@ -27,6 +28,7 @@ class GpuContext:
         # First 64 KiB: ticket counters (must start at zero; kernels restore them), rest: partials.
         self.workspace = torch.zeros(WORKSPACE_BYTES // 4, dtype=torch.float32, device=self.device)
         self.lib = lib()
+        self._run_kernel, self._index = self.lib.lk_run_kernel, self.device.index
         self._handles: dict[str, int] = {}
         self._ws_by_slot: dict[int, torch.Tensor] = {0: self.workspace}
         self.slot = 0
@@ -105,16 +107,18 @@ class GpuContext:
         return h
 
     def run(self, name: str, ptrs, ints, floats) -> None:
-        L = self.lib
-        pa, ia, fa = array("Q", ptrs), array("q", ints), array("d", floats)
+        n = len(ptrs)
+        words = array("q", (*ptrs, *ints))  # both arrays of lk_run_kernel: one buffer is cheaper to make than two
+        at = words.buffer_info()[0]
+        fa = array("d", floats) if floats else None
         ws = self._ws_by_slot.get(self.slot)
         if ws is None:
             ws = self.workspace_for(self.slot)
-        rc = L.lk_run_kernel(self._handles.get(name) or self.handle(name), pa.buffer_info()[0], len(pa),
-                             ia.buffer_info()[0], len(ia), fa.buffer_info()[0], len(fa), ws.data_ptr(), WORKSPACE_BYTES,
-                             torch._C._cuda_getCurrentRawStream(self.device.index))
+        rc = self._run_kernel(self._handles.get(name) or self.handle(name), at, n, at + 8 * n, len(words) - n,
+                              fa.buffer_info()[0] if floats else None, len(floats), ws.data_ptr(), WORKSPACE_BYTES,
+                              _raw_stream(self._index))
         if rc != 0:
-            raise LokinferError(L.lk_last_error().decode())
+            raise LokinferError(self.lib.lk_last_error().decode())
 
 
 def synchronize() -> None:
