@@ -358,7 +358,7 @@ int lk_hip_w4_gemm(const void* x, const void* gamma, const void* q, const void* 
 
 /* ---- key / value caches in 4 bits (MI355X backend): u8 [B, 2, kvh, 72 P], P rows (a multiple of 32) per (sequence, keys
  *      or values, kv head): first 64 bytes of codes a row, then the scales, f16 [4, P] (groups of 32 of the head's 128 values);
- *      16-byte aligned, as are q, k, v and qkv; B <= 65535, P <= 2^27. pos: a device i64[B], the position of each sequence's
+ *      16-byte aligned, as are q, k, v, qkv and out; B <= 65535, P <= 2^27. pos: a device i64[B], the position of each sequence's
  *      first row of the call. ---- */
 /* k, v f16[B T, kvh 128] -> rows pos[b] .. of sequence b; rows outside the cache are dropped. A row whose key or value is not
  * finite is held so that a query that sees it gets NaN. */

@@ -681,7 +681,7 @@ void runKv4Attention(ExecCtx& ctx, const KernelArgs& a) {
   const int rc = lk_hip_kv4_attention(a.ptrs[0], a.ptrs[1], P<int64_t>(a, 2), a.ptrs[3], b, rows / b,
                                       static_cast<int>(width / 128), static_cast<int>(kvh), cap, a.ptrs[4], a.ints[9] * 4,
                                       ctx.stream);
-  status(ctx, rc, rc == 3 ? "attention_kv4: work is too small" : "attention_kv4: q and kv must be 16-byte aligned, B at most 65535, P at most 2^27");
+  status(ctx, rc, rc == 3 ? "attention_kv4: work is too small" : "attention_kv4: q, kv and out must be 16-byte aligned, B at most 65535, P at most 2^27");
 }
 
 // kv4_reorder_gpu: kv u8[L, B, 2, kvh, 72 P], parents i64[B], n i64[1] (in place)
