@@ -680,15 +680,18 @@ bool groupOk(int g) { return g == 32 || g == 64 || g == 128; }
 int launched() { return hipGetLastError() == hipSuccess ? 0 : 2; }
 unsigned gridFor(int64_t threads) { return static_cast<unsigned>(std::min<int64_t>((threads + 255) / 256, 65536)); }
 
+int64_t streamLds(const lkd::W4Params& p) { return p.m * (p.kb * 128 + lkd::kStreamPad) * 2; }
+bool streamed(const lkd::W4Params& p) { return (p.n + 15) / 16 >= 1536 && streamLds(p) <= 128 << 10; }
+
 template <int RU, int G, int W, bool F32, bool RMS>
 void launchFew(const lkd::W4Params& p, hipStream_t s) {
-  const int64_t tiles = (p.n + 15) / 16, lds = p.m * (p.kb * 128 + lkd::kStreamPad) * 2;
+  const int64_t tiles = (p.n + 15) / 16;
   // us, split over 4 / 8 waves against streamed (M = 1, G = 64): K = 2048, N = 4096 3.9 / 4.2 / 6.9; 16384 7.4 / 8.5 / 7.6;
   // 32768 11.2 / 14.2 / 10.3; 65536 19.2 / 27.0 / 16.6; K = 6144, N = 2048 7.3 / 6.2 / 15.4; 8192 9.8 / 10.0 / 15.3; 32768
   // 27.4 / 30.1 / 22.1
-  if (tiles >= 1536 && lds <= 128 << 10)
+  if (streamed(p))
     hipLaunchKernelGGL((lkd::w4StreamKernel<RU, G, W, F32, RMS>), dim3(static_cast<unsigned>(std::min<int64_t>((tiles + 3) / 4, 1024))),
-                       dim3(256), static_cast<size_t>(lds), s, p);
+                       dim3(256), static_cast<size_t>(streamLds(p)), s, p);
   else if (p.kb >= 32 && tiles <= 512)
     hipLaunchKernelGGL((lkd::w4SplitKernel<RU, G, W, F32, RMS, 8>), dim3(static_cast<unsigned>(tiles)), dim3(512), 0, s, p);
   else
@@ -715,16 +718,19 @@ double w4Us(int64_t m, int64_t cols, int64_t k, int bm, int bn, double a, double
   return static_cast<double>((groups + 255) / 256) * (a + static_cast<double>(k) / b);
 }
 
-// Over 16 rows: the rows kernel against 32 x 64 tiles, us at 32 rows: K, N = 512, 2048 3.2 / 5.3; 2048, 4096 6.5 / 7.3; 6144,
-// 2048 13.8 / 12.6; 2048, 12288 15 / 8.7. The tiles against each other, us of 32 x 64 / 64 x 64 / 128 x 256: M, K, N = 128,
+// 5 to 16 rows that are not streamed: the split kernel, whose workgroups each read all of x, against 32 x 64 tiles, us at M, K, N
+// = 8, 6144, 16384 20 / 16; 16, 6144, 16384 30 / 16; 16, 2048, 12288 9.4 / 8.1; 8, 2048, 12288 6.7 / 8.1; 16, 6144, 2048 9.6 / 12.8.
+// Over 16 rows: the rows kernel against 32 x 64 tiles, 32 rows, K, N = 512, 2048 3.2 / 5.3; 2048, 4096 6.5 / 7.3; 4096, 2048
+// 9.7 / 9.9 (17 rows 7.3 / 10); 6144, 2048 13.8 / 12.6; 2048, 12288 15 / 8.7.
+// The tiles against each other, us of 32 x 64 / 64 x 64 / 128 x 256: M, K, N = 128,
 // 2048, 4096 8.1 / 11 / 33; 256, 6144, 2048 14 / 20 / 81; 409, 2048, 2048 14 / 11 / 33; 409, 6144, 2048 26 / 21 / 89; 409,
 // 2048, 12288 61 / 57 / 38; 2048, 2048, 2048 57 / 56 / 39; 2048, 2048, 12288 297 / 274 / 109.
 template <int G, int W, bool F32>
 void launchW4(const lkd::W4Params& p, hipStream_t s) {
   if (p.gamma) return launchFew<1, G, W, F32, true>(p, s);
   if (p.m <= 4) return launchFew<1, G, W, F32, false>(p, s);
-  if (p.m <= 16) return launchFew<4, G, W, F32, false>(p, s);
-  if ((p.m + 31) / 32 * ((p.n + 15) / 16) <= 256 && p.k <= 2048) return launchRows<G, W, F32>(p, s);
+  if (p.m <= 16 && (streamed(p) || p.m * ((p.n + 15) / 16) < 8192)) return launchFew<4, G, W, F32, false>(p, s);
+  if (p.m > 16 && (p.m + 31) / 32 * ((p.n + 15) / 16) <= 256 && p.k <= 4096) return launchRows<G, W, F32>(p, s);
   const double t32 = w4Us(p.m, p.n * W, p.k, 32, 64, 3.0, 400.0), t64 = w4Us(p.m, p.n * W, p.k, 64, 64, 6.6, 350.0),
                t128 = w4Us(p.m, p.n * W, p.k, 128, 256, 6.0, 65.0);
   if (t32 <= t64 && t32 <= t128) launchGemm<32, 1, 8, G, W, F32>(p, s);

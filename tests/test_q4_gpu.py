@@ -118,6 +118,8 @@ W4_CASES = [(1, 2048, 4096, 64), (1, 8, 1, 32), (1, 136, 17, 128), (1, 6144, 48,
             (1030, 136, 260, 64),
             # many columns: weights streamed by persistent waves, x in LDS; 2048 x 16 rows of it are more than 64 KiB
             (1, 264, 32770, 64), (3, 40, 24600, 32), (7, 136, 25000, 128), (16, 2048, 24583, 128),
+            # few rows, many columns: tiles, not streamed (x is too long for LDS, or not enough columns for it)
+            (6, 200, 22000, 64), (16, 520, 8200, 32), (13, 5128, 24580, 128),
             # tiles of 32 x 64, 64 x 64 and 128 x 256
             (17, 4104, 70, 32), (40, 6152, 200, 64), (100, 2184, 515, 128), (20, 72, 8200, 32), (405, 2056, 2050, 64),
             (450, 3080, 1990, 128), (450, 3080, 1990, 32), (1025, 264, 2100, 32), (700, 1032, 4100, 128), (700, 1032, 4100, 64)]
