@@ -349,8 +349,8 @@ int lk_hip_w4_pack(const void* codes, const void* scales, void* q, void* s, int*
                    void* stream);
 /* q, s -> w f16[K, N], exact */
 int lk_hip_w4_unpack(const void* q, const void* s, void* w, int64_t n, int64_t k, int group, void* stream);
-/* out [M, N] = x f16[M, K] @ W (f32 sums): f16, + bias f16[N], + res f16[M, N]; silu(x @ W) * (x @ W2) with q2, s2; f32
- * with f32_out. gamma f16[K] (M = 1, else null): x is rmsnorm(x, gamma, eps) first. K % 8 == 0;
+/* out [M, N] = x f16[M, K] @ W (f32 sums): f16, + bias f16[N], + res f16[M, N] (either, both or none); silu(x @ W) * (x @ W2)
+ * with q2, s2; f32 with f32_out. gamma f16[K] (M = 1, else null): x is rmsnorm(x, gamma, eps) first. K % 8 == 0;
  * K <= 2^23, M <= 2097120; x, gamma 16-byte aligned. */
 int lk_hip_w4_gemm(const void* x, const void* gamma, const void* q, const void* s, const void* q2, const void* s2,
                    const void* bias, const void* res, void* out, int64_t m, int64_t n, int64_t k, int group, int f32_out,

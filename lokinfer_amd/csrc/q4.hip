@@ -603,10 +603,15 @@ __global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
     if (F32 || !in(row, col)) return static_cast<h16>(0.0f);
     return p.res ? p.res[row * p.n + col] : p.bias ? p.bias[col] : static_cast<h16>(0.0f);
   };
+  // Of a bias and a residual together, `added` is the residual; the bias is loaded at its store. They are added in w4Put's order.
   const auto put = [&](int64_t row, int64_t col, float y, h16 add) {
     if (!in(row, col)) return;
-    if constexpr (F32) static_cast<float*>(p.out)[row * p.n + col] = y;
-    else static_cast<h16*>(p.out)[row * p.n + col] = toH16(y + static_cast<float>(add));
+    if constexpr (F32) {
+      static_cast<float*>(p.out)[row * p.n + col] = y;
+    } else {
+      if (W == 1 && p.bias && p.res) y += static_cast<float>(p.bias[col]);
+      static_cast<h16*>(p.out)[row * p.n + col] = toH16(y + static_cast<float>(add));
+    }
   };
   const bool adds = W == 1 && (p.res || p.bias);
   if constexpr (KG == 1) {

@@ -1,0 +1,58 @@
+"""4-bit serving and beam selection on the GPU where a call's arguments meet: epilogues together, long flat tails of keys, values
+that f16 holds as subnormals, weights used on other streams, candidates that 64 bits do not tell apart. Tolerances as in
+test_q4_gpu, whose terms are repeated where they apply."""
+import ctypes as C
+
+import numpy as np
+import pytest
+import torch
+
+from lokinfer_amd._lib import lib
+
+from oracle import q4 as O
+
+pytestmark = pytest.mark.gpu
+
+U, SUB = 2.0 ** -11, 2.0 ** -25
+
+
+def G(lk, a):
+    return lk.from_numpy(np.ascontiguousarray(a), device="gpu", copy=True)
+
+
+def I(lk, *v):
+    return G(lk, np.array(v, np.int64))
+
+
+def product(x, w):
+    """x @ w and the f32 term of its tolerance."""
+    x = np.asarray(x, np.float64)
+    return x @ w, 2.0 ** -22 * np.sqrt(x.shape[1]) * np.sqrt((x * x) @ (w * w))
+
+
+# one shape for each kernel a product can take: k split over 4 or 8 waves, streamed, 32 rows, tiles of 32 x 64, 64 x 64, 128 x 256
+SHAPES = [(2, 264, 40, 32), (3, 4104, 64, 128), (3, 40, 24600, 32), (20, 264, 70, 64), (17, 4104, 70, 32), (405, 2056, 2050, 64),
+          (700, 1032, 4100, 128)]
+
+
+@pytest.mark.parametrize("m,k,n,group", SHAPES)
+def test_bias_and_residual_together(gpu, m, k, n, group):
+    """The C entry point takes both: (x @ w + bias) + res, whichever kernel runs."""
+    lk, q4 = gpu, gpu.ops.q4_gpu
+    r = np.random.default_rng([31, m, k, n])
+    x = r.standard_normal((m, k)).astype(np.float16)
+    w = (r.standard_normal((k, n)) / np.sqrt(k)).astype(np.float16)
+    bias, res = r.standard_normal(n).astype(np.float16), r.standard_normal((m, n)).astype(np.float16)
+    p = q4.pack_w4(w, group=group)
+    gx, gb, gr = G(lk, x), G(lk, bias), G(lk, res)
+    out = torch.zeros(m, n, dtype=torch.float16, device="cuda")
+    at = [C.c_void_p(t.data_ptr()) for t in (gx.t, p.q.t, p.s.t, gb.t, gr.t, out)]
+    call = lib().lk_hip_w4_gemm
+    rc = call(at[0], None, at[1], at[2], None, None, at[3], at[4], at[5], C.c_int64(m), C.c_int64(n), C.c_int64(k),
+              C.c_int(group), C.c_int(0), C.c_float(0.0), C.c_void_p(torch.cuda.current_stream().cuda_stream))
+    assert rc == 0
+    ref, term = product(x, O.weight_values(w, group))
+    first, ref = ref + bias, ref + bias + res
+    # two f32 sums behind the product, one rounding to f16
+    off = np.abs(out.cpu().numpy().astype(np.float64) - ref)
+    assert (off <= U * (1 + 2.0 ** -10) * np.abs(ref) + term + 2.0 ** -23 * (np.abs(first) + np.abs(ref)) + SUB).all()
