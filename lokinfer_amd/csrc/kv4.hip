@@ -311,11 +311,12 @@ __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[k][u][r]);
       mx = crossRowMax(mx) * p.scale;
       if (__any(mx > m[k] + kGrowth)) {
-        const float to = fmaxf(m[k], mx), corr = to == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[k] - to);
+        const bool grows = mx > m[k] + kGrowth;  // (each row by itself: its sums do not depend on its neighbours)
+        const float corr = grows ? __builtin_amdgcn_exp2f(m[k] - mx) : 1.0f;
         l[k] *= corr;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[k][e] *= corr;
-        m[k] = to;
+        m[k] = grows ? mx : m[k];
       }
       const float base = m[k] == -INFINITY ? 0.0f : m[k];  // no key so far: every weight 0 (or a NaN kept)
 #pragma unroll

@@ -56,3 +56,21 @@ def test_bias_and_residual_together(gpu, m, k, n, group):
     # two f32 sums behind the product, one rounding to f16
     off = np.abs(out.cpu().numpy().astype(np.float64) - ref)
     assert (off <= U * (1 + 2.0 ** -10) * np.abs(ref) + term + 2.0 ** -23 * (np.abs(first) + np.abs(ref)) + SUB).all()
+
+
+@pytest.mark.parametrize("t,qh,kvh", [(48, 4, 2), (90, 128, 16)])
+def test_a_row_does_not_depend_on_the_rows_beside_it(gpu, t, qh, kvh):
+    """Where one row's running maximum grows, the sums of the others of its workgroup stay as they are: bit for bit."""
+    lk, q4 = gpu, gpu.ops.q4_gpu
+    r = np.random.default_rng([34, t, qh])
+    n = 1000
+    k, v = (r.standard_normal((n, kvh * 128)).astype(np.float16) for _ in range(2))
+    k *= np.exp(r.standard_normal((n, 1))).astype(np.float16)  # maxima that grow along the keys
+    kv = q4.kv4_cache(1, kvh, n)
+    q4.kv4_write_f16_gpu(kv, G(lk, k), G(lk, v), I(lk, 0))
+    q = r.standard_normal((t, qh * 128)).astype(np.float16)
+    want = q4.attention_kv4_f16_gpu(G(lk, q), kv, I(lk, n - t)).numpy()
+    other = q.copy()
+    other[::2] *= 4
+    got = q4.attention_kv4_f16_gpu(G(lk, other), kv, I(lk, n - t)).numpy()
+    assert np.array_equal(got[1::2], want[1::2]) and not np.array_equal(got[::2], want[::2])
