@@ -193,19 +193,21 @@ struct Kv4Params {
 // S = K Q^T: lane (key l % 16, kq = l / 16) loads 16 bytes of its key's row, the codes of scale group kq; its word w, scaled
 // (exact in f16), is the A operand of step w, dims 32 kq + 8 w .., the B operand row l % 16's same dims. Its accumulators are
 // then row l % 16's scores of keys 4 kq + 0 .. 3, on which the softmax runs in f32 (log2 units).
-// O^T = V^T P^T over two tiles: the lane's own 8 weights are the B operand as they are, as two f16 parts (hi, and lo = p -
-// hi, so that p keeps some 22 bits). The A operand is 8 keys of one dim: lane (db = l % 16, kq) loads those keys' words
+// O^T = V^T P^T over two tiles: the lane's own 8 weights are the B operand as they are, as two f16 parts, hi and lo = p - hi.
+// f16's smallest step is 2^-24, so the pair is off by 2^-22 of p or by 2^-25, and by 2^-37 of the row's largest weight, which is
+// held at 2^12 or above (kStart). The A operand is 8 keys of one dim: lane (db = l % 16, kq) loads those keys' words
 // db, dims 8 db .. 8 db + 7; the low halves of two keys' words put side by side hold the even dims' codes as pairs, the high
 // halves the odd ones', so each dim's operand is masked out of them as a row's codes are out of a word.
 // Chunks are dealt over the waves of all workgroups of a row block (splits); the waves' sums meet in LDS.
 // Keys from the longest row's end on have their weight and their value's scale set to zero, whatever the memory holds there.
-// The sums are rescaled to a new maximum only where it exceeds the one they stand at by 2^8: until then weights reach 2^8,
-// which changes no relative precision, and nearly every tile brings some row a slightly larger score.
+// A row's weights are 2^(score - m): m is set 12 below a maximum, and again, with its sums rescaled, only where a score exceeds
+// it by 15 (2^15 fits f16), since nearly every tile brings some row a slightly larger score. m 7 below a maximum takes up to 1.6%
+// less time, m at one with room for 2^8 up to 2.3%, which loses weights under 2^-25 of the largest.
 // 16 / 8 heads: one query over 417 rows 6.6 us and over 32768 12.6 + 4.1 of the joining launch (38 MB, 2.3 TB/s): latency, of one
 // chunk in the first. 2048 queries over as many rows 46 us, 370 TFLOP/s: bound by VALU (some 70% of the cycles, MFMA 30%), half of it
 // the codes' conversion, which 32 rows share, half the softmax. Tiles of f16 made once per call and shared through LDS took
 // 6 + 50; more rows a wave leave one wave a SIMD (61 us).
-constexpr float kGrowth = 8.0f;
+constexpr float kTop = 15.0f, kStart = 12.0f;
 template <int RB, int KW>
 __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1 ? 4 : 2))) void kv4AttnKernel(Kv4Params p) {
   const Q4Masks masks;
@@ -243,7 +245,7 @@ __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1
   const unsigned ksOff = kq * static_cast<unsigned>(cap) * 2 + lc * 2, vsOff = (lc >> 2) * static_cast<unsigned>(cap) * 2 + 8 * kq;
   const int chunks = (nk + 63) / 64, step = p.splits * KW;
   f32x4 acc[RB][8];
-  float m[RB];   // a running maximum times the scale, rounded once and taken off everywhere as it is
+  float m[RB];   // what is taken off a row's scores: the maximum it was set at times the scale, rounded once, less kStart
   f32x4 l[RB];   // the weights' sum, four times: a product with ones
   const h16 one = static_cast<h16>(1.0f);
   const half8 ones{one, one, one, one, one, one, one, one};
@@ -310,13 +312,13 @@ __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1
 #pragma unroll
         for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[k][u][r]);
       mx = crossRowMax(mx) * p.scale;
-      if (__any(mx > m[k] + kGrowth)) {
-        const bool grows = mx > m[k] + kGrowth;  // (each row by itself: its sums do not depend on its neighbours)
-        const float corr = grows ? __builtin_amdgcn_exp2f(m[k] - mx) : 1.0f;
+      if (__any(mx - m[k] > kTop)) {
+        const bool grows = mx - m[k] > kTop;  // (each row by itself: its sums do not depend on its neighbours)
+        const float to = mx - kStart, corr = grows ? __builtin_amdgcn_exp2f(m[k] - to) : 1.0f;
         l[k] *= corr;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[k][e] *= corr;
-        m[k] = grows ? mx : m[k];
+        m[k] = grows ? to : m[k];
       }
       const float base = m[k] == -INFINITY ? 0.0f : m[k];  // no key so far: every weight 0 (or a NaN kept)
 #pragma unroll

@@ -74,3 +74,27 @@ def test_a_row_does_not_depend_on_the_rows_beside_it(gpu, t, qh, kvh):
     other[::2] *= 4
     got = q4.attention_kv4_f16_gpu(G(lk, other), kv, I(lk, n - t)).numpy()
     assert np.array_equal(got[1::2], want[1::2]) and not np.array_equal(got[::2], want[::2])
+
+
+@pytest.mark.parametrize("t", [4096, 8192, 10400], ids=["16x8", "32x8", "32x4"])  # rows x waves of a workgroup
+def test_few_keys_above_a_long_flat_tail(gpu, t):
+    """One key of each wave 17.5 above a million equal others: each of these has a weight of 2^-25, all of them together 0.3%
+    of the sum, and they alone have a value. The keys of a row lie in one workgroup."""
+    lk, q4 = gpu, gpu.ops.q4_gpu
+    cap = 1 << 20
+    top = 64 * torch.arange(8, device="cuda")
+    key, val = torch.zeros(cap, 128, dtype=torch.float16, device="cuda"), torch.full((cap, 128), 0.875, dtype=torch.float16, device="cuda")
+    key[top], val[top] = 1.75, 0.0
+    kv = q4.kv4_cache(1, 1, cap)
+    q4.kv4_write_f16_gpu(kv, lk.Tensor(key), lk.Tensor(val), I(lk, 0))
+    assert (q4.kv4_read_f16_gpu(kv).t[0, :, 0] == torch.stack([key, val])).all()  # exact in 4 bits
+    q = np.float16(17.5 / (1.75 * np.sqrt(128)))
+    got = q4.attention_kv4_f16_gpu(lk.Tensor(torch.full((t, 128), float(q), dtype=torch.float16, device="cuda")), kv, I(lk, cap - t))
+    got = got.t.cpu().numpy().astype(np.float64)
+    score = 128 * 1.75 * float(q) / np.sqrt(128)
+    rest = (cap - t + np.arange(t) + 1 - 8)[:, None] * np.exp(-score)
+    ref = 0.875 * rest / (8 + rest)
+    # as in test_q4_gpu: E of a score of 128 equal products; a weight is held to 2^-37 of the largest
+    e = 2.0 ** -22 * (np.sqrt(128) * score / np.sqrt(128) + score)
+    extra = 0.875 * (2.0 ** -22 * (8 + np.sqrt(cap)) + 4 * e + cap * 2.0 ** -37)
+    assert (np.abs(got - ref) <= U * (1 + 2.0 ** -10) * ref + extra).all(), (got.min(), got.max(), ref.min(), ref.max())
