@@ -202,12 +202,14 @@ struct Kv4Params {
 // Keys from the longest row's end on have their weight and their value's scale set to zero, whatever the memory holds there.
 // A row's weights are 2^(score - m): m is set 12 below a maximum, and again, with its sums rescaled, only where a score exceeds
 // it by 15 (2^15 fits f16), since nearly every tile brings some row a slightly larger score. m 7 below a maximum takes up to 1.6%
-// less time, m at one with room for 2^8 up to 2.3%, which loses weights under 2^-25 of the largest.
+// less time, m at one with room for 2^8 up to 2.3%, which loses weights under 2^-25 of the largest. A score is one fma away
+// from m, its product with the scale not rounded by itself; where f32's steps are too coarse for that, from 2^20 on (at 2^28 the
+// difference would leave f16), the product is rounded first, as the maximum's was, and m is the maximum: 1% of the time.
 // 16 / 8 heads: one query over 417 rows 6.6 us and over 32768 12.6 + 4.1 of the joining launch (38 MB, 2.3 TB/s): latency, of one
 // chunk in the first. 2048 queries over as many rows 46 us, 370 TFLOP/s: bound by VALU (some 70% of the cycles, MFMA 30%), half of it
 // the codes' conversion, which 32 rows share, half the softmax. Tiles of f16 made once per call and shared through LDS took
 // 6 + 50; more rows a wave leave one wave a SIMD (61 us).
-constexpr float kTop = 15.0f, kStart = 12.0f;
+constexpr float kTop = 15.0f, kStart = 12.0f, kCoarse = 0x1p20f;
 template <int RB, int KW>
 __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1 ? 4 : 2))) void kv4AttnKernel(Kv4Params p) {
   const Q4Masks masks;
@@ -314,11 +316,20 @@ __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1
       mx = crossRowMax(mx) * p.scale;
       if (__any(mx - m[k] > kTop)) {
         const bool grows = mx - m[k] > kTop;  // (each row by itself: its sums do not depend on its neighbours)
-        const float to = mx - kStart, corr = grows ? __builtin_amdgcn_exp2f(m[k] - to) : 1.0f;
+        const float to = fabsf(mx) > kCoarse ? mx : mx - kStart, corr = grows ? __builtin_amdgcn_exp2f(m[k] - to) : 1.0f;
         l[k] *= corr;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[k][e] *= corr;
         m[k] = grows ? to : m[k];
+      }
+      float sc = p.scale;
+      if (__any(fabsf(mx) > kCoarse)) {
+        const bool coarse = fabsf(mx) > kCoarse;
+        sc = coarse ? 1.0f : sc;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[k][u][r] = coarse ? s[k][u][r] * p.scale : s[k][u][r];
       }
       const float base = m[k] == -INFINITY ? 0.0f : m[k];  // no key so far: every weight 0 (or a NaN kept)
 #pragma unroll
@@ -326,8 +337,8 @@ __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
           typedef float f32x2 __attribute__((ext_vector_type(2)));
-          const f32x2 e = {__builtin_amdgcn_exp2f(fmaf(s[k][u][r], p.scale, -base)),
-                           __builtin_amdgcn_exp2f(fmaf(s[k][u][r + 1], p.scale, -base))};
+          const f32x2 e = {__builtin_amdgcn_exp2f(fmaf(s[k][u][r], sc, -base)),
+                           __builtin_amdgcn_exp2f(fmaf(s[k][u][r + 1], sc, -base))};
           const half2v hi = __builtin_convertvector(e, half2v);
           const half2v lo = __builtin_convertvector((f32x2{fmaf(static_cast<float>(hi[0]), -1.0f, e[0]),
                                                            fmaf(static_cast<float>(hi[1]), -1.0f, e[1])}), half2v);

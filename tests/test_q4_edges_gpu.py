@@ -98,3 +98,32 @@ def test_few_keys_above_a_long_flat_tail(gpu, t):
     e = 2.0 ** -22 * (np.sqrt(128) * score / np.sqrt(128) + score)
     extra = 0.875 * (2.0 ** -22 * (8 + np.sqrt(cap)) + 4 * e + cap * 2.0 ** -37)
     assert (np.abs(got - ref) <= U * (1 + 2.0 ** -10) * ref + extra).all(), (got.min(), got.max(), ref.min(), ref.max())
+
+
+@pytest.mark.parametrize("t,cap", [(1, 320), (1, 4096), (33, 320), (300, 320), (401, 448)])
+@pytest.mark.parametrize("size", [2.0, 600.0, 8000.0, 60000.0])
+def test_scores_of_any_size(gpu, t, cap, size):
+    """Keys of two sizes, so scores of two values: the larger ones' rows share the weight equally, also where f32 cannot tell
+    the scores' neighbours apart any more (2^36 at 60000) and where all of them are negative."""
+    lk, q4 = gpu, gpu.ops.q4_gpu
+    r = np.random.default_rng([38, t, cap])
+    n = cap - 7
+    k, v = np.full((n, 256), 0.5 * size, np.float16), r.standard_normal((n, 256)).astype(np.float16)
+    top = [3, 9]
+    k[top] = size
+    kv = q4.kv4_cache(1, 2, cap)
+    q4.kv4_write_f16_gpu(kv, G(lk, k), G(lk, v), I(lk, 0))
+    key, val = O.cache_values(k, v, 2)
+    for sign in (1, -1):
+        q = np.full((t, 4 * 128), sign * size, np.float16)
+        got = q4.attention_kv4_f16_gpu(G(lk, q), kv, I(lk, n - t)).numpy().astype(np.float64).reshape(t, 4, 128)
+        for i in (0, t // 2, t - 1):
+            for h in range(4):
+                seen = n - t + i + 1
+                s = key[:seen, h // 2] @ q[i, h * 128:(h + 1) * 128].astype(np.float64) / np.sqrt(128)
+                e = np.exp(s - s.max())
+                ref = (e / e.sum()) @ val[:seen, h // 2]
+                assert np.isfinite(got[i, h]).all(), (sign, i, h)
+                # a weight next to the largest: all or none, or (size 2) scores of 45 at 2^-22
+                assert (np.abs(got[i, h] - ref) <= U * (1 + 2.0 ** -10) * np.abs(ref) + np.abs(val).max() * 2.0 ** -22 *
+                        (8 + np.sqrt(cap) + 4 * 2 * 46) + SUB).all(), (sign, i, h)
