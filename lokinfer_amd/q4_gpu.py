@@ -121,26 +121,43 @@ def quantize_w4_f16_gpu(w, group: int = 64, nt: bool = False) -> PackedWeight4:
     return PackedWeight4(Tensor(q), Tensor(s), (k, n), group)
 
 
+_CODES, _SCALES = "codes must be 0 .. 15", "scales must be >= 0, at most 8128, of at most 8 significant bits"
+
+
+def _held(a, dtype, said):
+    """Host values as `dtype`, which must hold them as they are; an lk.Tensor as it is."""
+    if isinstance(a, Tensor):
+        return a
+    given = np.asarray(a)
+    with np.errstate(invalid="ignore", over="ignore"):
+        cast = np.ascontiguousarray(given, dtype)
+    check(cast.dtype == given.dtype or np.array_equal(cast, given), said)
+    return cast
+
+
+def _up(a, dtype) -> Tensor:
+    if isinstance(a, Tensor):
+        return a
+    return Tensor(torch.from_numpy(np.ascontiguousarray(a, dtype)).to(GpuContext.shared().device))
+
+
 def pack_w4(w, scales=None, group: int = 64, nt: bool = False) -> PackedWeight4:
     """A weight into the kernels' layout: w f16[K, N] (numpy array or lk.Tensor; nt: f16[N, K]), quantised here, or its
-    codes u8[K, N] (0 .. 15) with scales f16[ceil(K / group), N] (>= 0, at most 8 significant bits and 8128)."""
-    def up(a, dtype):
-        if isinstance(a, Tensor):
-            return a
-        return Tensor(torch.from_numpy(np.ascontiguousarray(a, dtype)).to(GpuContext.shared().device))
-
+    codes u8[K, N] (0 .. 15) with scales f16[ceil(K / group), N] (>= 0, at most 8 significant bits and 8128); codes and
+    scales in arrays of other types must be values that u8 and f16 hold."""
     if scales is None:
-        return quantize_w4_f16_gpu(up(w, np.float16), group, nt)
+        return quantize_w4_f16_gpu(_up(w, np.float16), group, nt)
     check(not nt, "codes are given as u8[K, N]")
-    codes, scales = _arg(up(w, np.uint8), _U8, 2, "codes"), _arg(up(scales, np.float16), _F16, 2, "scales")
+    codes, scales = _held(w, np.uint8, _CODES), _held(scales, np.float16, _SCALES)
+    codes, scales = _arg(_up(codes, np.uint8), _U8, 2, "codes"), _arg(_up(scales, np.float16), _F16, 2, "scales")
     k, n = codes.shape
     q, s = _w4_empty(k, n, group)
     check(tuple(scales.shape) == (-(-k // group), n), "scales must be f16[ceil(K / group), N]")
     flag = torch.zeros(1, dtype=_I32, device=codes.device)
     _call("pack_w4_u8_gpu", [codes, scales, flag, q, s], [group])
     bad = int(flag)  # waits for the layout: once per weight
-    check(not bad & 1, "codes must be 0 .. 15")
-    check(not bad, "scales must be >= 0, at most 8128, of at most 8 significant bits")
+    check(not bad & 1, _CODES)
+    check(not bad, _SCALES)
     return PackedWeight4(Tensor(q), Tensor(s), (k, n), group)
 
 

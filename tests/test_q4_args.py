@@ -1,0 +1,29 @@
+"""4-bit ops and the launch path without a GPU: what a call is refused for, and where a launch goes."""
+import numpy as np
+import pytest
+import torch
+
+import lokinfer_amd as lk
+from lokinfer_amd import ops
+from lokinfer_amd import q4_gpu as q4
+
+
+@pytest.mark.parametrize("bad", [np.full((64, 4), 257, np.int32), np.full((64, 4), -250),
+                                 np.full((64, 4), 1.7), np.full((64, 4), np.nan, np.float32), np.full((64, 4), 2 ** 40)],
+                         ids=["257", "-250", "1.7", "nan", "2^40"])
+def test_codes_are_checked_as_given(bad):
+    """Not after a cast to u8, which would turn 257 into 1."""
+    codes = np.full(bad.shape, 3, bad.dtype)
+    codes[63, 2] = bad[0, 0]
+    with pytest.raises(ops.OpError, match="codes must be 0 .. 15"):
+        q4.pack_w4(codes, np.ones((2, 4), np.float16), 32)
+
+
+@pytest.mark.parametrize("bad", [np.float32(1e-9), np.float64(1 + 2.0 ** -12), np.float32(1e6), np.float32(np.nan), 70000],
+                         ids=["1e-9", "1 + 2^-12", "1e6", "nan", "70000"])
+def test_scales_are_checked_as_given(bad):
+    """Not after a cast to f16, which would turn 1e-9 into 0."""
+    scales = np.ones((2, 4), np.asarray(bad).dtype)
+    scales[1, 3] = bad
+    with pytest.raises(ops.OpError, match="scales must be"):
+        q4.pack_w4(np.zeros((64, 4), np.uint8), scales, 32)

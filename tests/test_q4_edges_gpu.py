@@ -127,3 +127,14 @@ def test_scores_of_any_size(gpu, t, cap, size):
                 # a weight next to the largest: all or none, or (size 2) scores of 45 at 2^-22
                 assert (np.abs(got[i, h] - ref) <= U * (1 + 2.0 ** -10) * np.abs(ref) + np.abs(val).max() * 2.0 ** -22 *
                         (8 + np.sqrt(cap) + 4 * 2 * 46) + SUB).all(), (sign, i, h)
+
+
+def test_codes_and_scales_of_other_types(gpu):
+    """Values that u8 and f16 hold are taken whatever type they come in."""
+    lk, q4 = gpu, gpu.ops.q4_gpu
+    r = np.random.default_rng(35)
+    codes, scales = r.integers(0, 16, (100, 20)), r.integers(1, 256, (4, 20)) * 2.0 ** -12
+    want = ((codes - 8) * np.repeat(scales, 32, 0)[:100]).astype(np.float16)
+    for c, s in ((np.uint8, np.float16), (np.int64, np.float32), (np.float32, np.float64)):
+        assert np.array_equal(q4.unpack_w4_f16_gpu(q4.pack_w4(codes.astype(c), scales.astype(s), 32)).numpy(), want)
+    assert np.array_equal(q4.unpack_w4_f16_gpu(q4.pack_w4(codes.tolist(), scales.tolist(), 32)).numpy(), want)
