@@ -144,9 +144,12 @@ def _up(a, dtype) -> Tensor:
 def pack_w4(w, scales=None, group: int = 64, nt: bool = False) -> PackedWeight4:
     """A weight into the kernels' layout: w f16[K, N] (numpy array or lk.Tensor; nt: f16[N, K]), quantised here, or its
     codes u8[K, N] (0 .. 15) with scales f16[ceil(K / group), N] (>= 0, at most 8 significant bits and 8128); codes and
-    scales in arrays of other types must be values that u8 and f16 hold."""
+    scales in arrays of other types must be values that u8 and f16 hold. The weight is ready for every stream."""
     if scales is None:
-        return quantize_w4_f16_gpu(_up(w, np.float16), group, nt)
+        packed = quantize_w4_f16_gpu(_up(w, np.float16), group, nt)
+        if not torch.cuda.is_current_stream_capturing():  # like an uploaded weight: ready for every stream that may run first
+            torch.cuda.current_stream(packed._q.device).synchronize()
+        return packed
     check(not nt, "codes are given as u8[K, N]")
     codes, scales = _held(w, np.uint8, _CODES), _held(scales, np.float16, _SCALES)
     codes, scales = _arg(_up(codes, np.uint8), _U8, 2, "codes"), _arg(_up(scales, np.float16), _F16, 2, "scales")

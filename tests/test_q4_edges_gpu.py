@@ -138,3 +138,23 @@ def test_codes_and_scales_of_other_types(gpu):
     for c, s in ((np.uint8, np.float16), (np.int64, np.float32), (np.float32, np.float64)):
         assert np.array_equal(q4.unpack_w4_f16_gpu(q4.pack_w4(codes.astype(c), scales.astype(s), 32)).numpy(), want)
     assert np.array_equal(q4.unpack_w4_f16_gpu(q4.pack_w4(codes.tolist(), scales.tolist(), 32)).numpy(), want)
+
+
+def test_weights_are_ready_on_any_stream(gpu, monkeypatch):
+    """A weight laid out on one stream, where that takes long, is used at once on another."""
+    lk, q4 = gpu, gpu.ops.q4_gpu
+    w = np.random.default_rng(33).standard_normal((256, 96)).astype(np.float16)
+    want = q4.unpack_w4_f16_gpu(q4.pack_w4(w)).numpy()
+    quantize = q4.quantize_w4_f16_gpu
+
+    def late(*args):
+        torch.cuda._sleep(100_000_000)  # some 50 ms on the device
+        return quantize(*args)
+
+    monkeypatch.setattr(q4, "quantize_w4_f16_gpu", late)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        p = q4.pack_w4(w)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        got = q4.unpack_w4_f16_gpu(p)
+        torch.cuda.current_stream().synchronize()
+        assert np.array_equal(got.numpy(), want)
