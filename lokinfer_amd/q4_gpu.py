@@ -41,10 +41,10 @@ _index = None  # of the context's GPU
 def _arg(x, dtype, rank, what) -> torch.Tensor:
     """The torch tensor of an operand: of this type and rank, on the context's GPU."""
     global _index
-    t = getattr(x, "t", None)
-    if t is None or t.dtype is not dtype or t.dim() != rank or t.get_device() != _index or _index is None:
-        if not isinstance(x, Tensor):
-            raise OpError(f"{what}: expected lk.Tensor, got {type(x).__name__}")
+    if not isinstance(x, Tensor):
+        raise OpError(f"{what}: expected lk.Tensor, got {type(x).__name__}")
+    t = x.t
+    if t.dtype is not dtype or t.dim() != rank or t.get_device() != _index or _index is None:
         if t.dtype is not dtype or t.dim() != rank:
             raise OpError(f"{what} must be a rank {rank} {str(dtype)[6:]} tensor, got {str(t.dtype)[6:]}{list(t.shape)}")
         if not t.is_cuda:

@@ -27,3 +27,16 @@ def test_scales_are_checked_as_given(bad):
     scales[1, 3] = bad
     with pytest.raises(ops.OpError, match="scales must be"):
         q4.pack_w4(np.zeros((64, 4), np.uint8), scales, 32)
+
+
+def test_torch_tensors_are_no_operands():
+    """A torch.Tensor has a method `t`, as an lk.Tensor has the attribute: the refusal names the type."""
+    h, u8, i64 = (torch.zeros(*s, dtype=d) for s, d in (((1, 128), torch.float16), ((1, 2, 1, 72 * 32), torch.uint8),
+                                                        ((1,), torch.int64)))
+    w = q4.PackedWeight4.__new__(q4.PackedWeight4)
+    for call in (lambda: q4.quantize_w4_f16_gpu(h), lambda: q4.gemm_w4_f16_gpu(h, w), lambda: q4.rmsnorm_gemm_w4_f16_gpu(h, h, w),
+                 lambda: q4.kv4_write_f16_gpu(u8, h, h, i64), lambda: q4.attention_kv4_f16_gpu(h, u8, i64),
+                 lambda: q4.qknorm_rope_kv4_f16_gpu(h, h, h, i64, u8), lambda: q4.kv4_reorder_gpu(u8, i64, i64),
+                 lambda: q4.quantize_w4_f16_gpu(np.zeros((8, 8)))):
+        with pytest.raises(ops.OpError, match="expected lk.Tensor"):
+            call()
