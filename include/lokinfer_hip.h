@@ -382,7 +382,8 @@ int lk_hip_kv4_reorder(void* kv, const int64_t* parents, const int64_t* n, int64
                        void* stream);
 
 /* ---- beam search (MI355X backend): candidate (b, t) = scores[b] + logits[b, t] - log sum exp logits[b], a finished beam's
- *      (done[b] != 0) its score at eos[0] alone; the k best, ties to the lowest b V + t. B, k <= 32, V <= 262144, 1 to 4
+ *      (done[b] != 0) its score at eos[0] alone; the k best, a beam's own ordered by their logits; equal logits of a beam to
+ *      the lowest t, equal candidates (in 64 bits) of different beams to the lowest b. B, k <= 32, V <= 262144, 1 to 4
  *      eos ids. What has no value (NaN; a row or score that is not finite) counts as -inf. out_done: the parent's, or the
  *      token is an eos. Returns 3 when the workspace (16-byte aligned) is short. ---- */
 int64_t lk_hip_beam_select_workspace_bytes(int64_t b, int64_t v, int k);

@@ -2,7 +2,8 @@
 //
 //   candidate (b, t) of an unfinished beam: score[b] + logits[b, t] - log sum_j exp(logits[b, j]);
 //   of a finished one: score[b] at t = eos[0], nothing elsewhere.
-// The k best of all B V, ties to the lowest b V + t. What has no value (a NaN, a row without a finite log-sum, a beam whose
+// The k best of all B V: a beam's own by their logits, which candidates in 64 bits may not tell apart; equal logits to the lowest t,
+// equal candidates of different beams to the lowest b. What has no value (a NaN, a row without a finite log-sum, a beam whose
 // score is not finite) counts as -inf.
 //
 // Two launches. beamScanKernel passes once over the logits, 8192 of a row per workgroup, 32 per lane in registers, and leaves

@@ -76,7 +76,8 @@ def attention(q: np.ndarray, key: np.ndarray, val: np.ndarray, pos: int):
 
 
 def beam_select(logits, scores, done, k, eos):
-    """-> (scores f64[k], parents, tokens, done)."""
+    """-> (scores f64[k], parents, tokens, done). A beam's own candidates stand in the order of their logits, which 64 bits of a
+    candidate may not tell apart."""
     x = np.asarray(logits, np.float64)
     b, v = x.shape
     cand = np.full((b, v), -np.inf)
@@ -90,8 +91,10 @@ def beam_select(logits, scores, done, k, eos):
         if np.isfinite(m):
             cand[i] = float(scores[i]) + (x[i] - (m + np.log(np.exp(x[i] - m).sum())))
     cand = np.where(np.isnan(cand), -np.inf, cand).reshape(-1)
-    at = np.argsort(-cand, kind="stable")[:k]
-    parent, token = at // v, at % v
+    parent, token = np.divmod(np.arange(b * v), v)
+    logit = np.where(np.isfinite(cand) & (np.asarray(done)[parent] == 0), x.reshape(-1), 0.0)
+    at = np.lexsort((token, -logit, parent, -cand))[:k]
+    parent, token = parent[at], token[at]
     return cand[at], parent, token, np.array([int(bool(done[p]) or t in eos) for p, t in zip(parent, token)])
 
 

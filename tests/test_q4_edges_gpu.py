@@ -158,3 +158,18 @@ def test_weights_are_ready_on_any_stream(gpu, monkeypatch):
         got = q4.unpack_w4_f16_gpu(p)
         torch.cuda.current_stream().synchronize()
         assert np.array_equal(got.numpy(), want)
+
+
+def test_logits_that_give_equal_candidates_keep_their_order(gpu):
+    """Beside a log-sum of 8, 1e-20 and 0 are one candidate in 64 bits. Within a beam the larger logit still comes first;
+    between beams equal candidates go to the lower one."""
+    lk = gpu
+    row = np.full(9000, -1.0, np.float32)
+    row[[50, 100, 200, 8500, 8700]] = [-1e-20, 0.0, 1e-20, 3e-20, -0.0]
+    best = [8500, 200, 100, 8700, 50]
+    for b, k, parents, tokens in ((1, 3, [0] * 3, best[:3]), (1, 6, [0] * 6, best + [0]), (2, 7, [0] * 5 + [1] * 2, best + best[:2])):
+        logits, scores, done = np.stack([row] * b), np.full(b, -2.0, np.float32), np.zeros(b, np.int64)
+        got = [x.numpy() for x in lk.ops.beam_select_f32_gpu(G(lk, logits), G(lk, scores), G(lk, done), k, (7,))]
+        assert got[1].tolist() == parents and got[2].tolist() == tokens
+        ref = O.beam_select(logits, scores, done, k, [7])
+        assert ref[1].tolist() == parents and ref[2].tolist() == tokens
