@@ -54,13 +54,16 @@ def lib():
 
 
 def check_device_errors() -> None:
-    """Waits for the current GPU and raises LokinferError if a kernel recorded a data error since the last check
+    """Waits for the context's GPU (the current one before there is a context) and raises LokinferError if a kernel recorded a data error since the last check
     (a position outside a KV cache, an id out of range, a persistent kernel whose exchange timed out); clears it.
     The reference reports GPU failures the same way, at its next synchronisation (takeGpuError,
     src/runtime/executable.cpp:850-852 in lariaus/lokinfer)."""
+    from .runtime import context_device
+
     L = lib()
     detail = C.c_int64(0)
-    code = L.lk_take_device_error(C.byref(detail))
+    with context_device():
+        code = L.lk_take_device_error(C.byref(detail))
     if code < 0:
         raise LokinferError("could not read the device error record")
     if code:

@@ -7,6 +7,7 @@ as LokinferError, the binding-level exception the reference raises from Status (
 """
 from __future__ import annotations
 
+import contextlib
 from array import array
 
 import torch
@@ -16,6 +17,7 @@ from .graph import current_graph
 
 WORKSPACE_BYTES = 64 << 20
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 class GpuContext:
@@ -107,6 +109,9 @@ class GpuContext:
         return h
 
     def run(self, name: str, ptrs, ints, floats) -> None:
+        if _current_device() != self._index:  # the null stream is the current device's, whichever that is
+            with torch.cuda.device(self._index):
+                return self.run(name, ptrs, ints, floats)
         n = len(ptrs)
         words = array("q", (*ptrs, *ints))  # both arrays of lk_run_kernel: one buffer is cheaper to make than two
         at = words.buffer_info()[0]
@@ -119,6 +124,12 @@ class GpuContext:
                               _raw_stream(self._index))
         if rc != 0:
             raise LokinferError(self.lib.lk_last_error().decode())
+
+
+def context_device():
+    """Context manager: the shared context's GPU is the current one (before there is a context, the one that is)."""
+    ctx = GpuContext._shared
+    return contextlib.nullcontext() if ctx is None else torch.cuda.device(ctx.device)
 
 
 def synchronize() -> None:

@@ -1,4 +1,6 @@
 """4-bit ops and the launch path without a GPU: what a call is refused for, and where a launch goes."""
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -40,3 +42,41 @@ def test_torch_tensors_are_no_operands():
                  lambda: q4.quantize_w4_f16_gpu(np.zeros((8, 8)))):
         with pytest.raises(ops.OpError, match="expected lk.Tensor"):
             call()
+
+
+def test_launches_go_to_the_contexts_gpu(monkeypatch):
+    """The null stream is that of the current GPU, whichever that is: a launch makes the context's the current one."""
+    from lokinfer_amd import _lib, runtime
+
+    current, seen = [1], []
+
+    @contextlib.contextmanager
+    def device(of):
+        was, current[0] = current[0], getattr(of, "index", of)
+        yield
+        current[0] = was
+
+    ctx = runtime.GpuContext.__new__(runtime.GpuContext)
+    ctx._index, ctx._handles, ctx.slot = 0, {"op": 1}, 0
+    ctx.device = torch.device("cuda", 0)
+    ctx._ws_by_slot = {0: torch.zeros(1)}
+    ctx._run_kernel = lambda *args: seen.append(current[0]) or 0
+    monkeypatch.setattr(runtime, "_current_device", lambda: current[0])
+    monkeypatch.setattr(runtime, "_raw_stream", lambda index: 0)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    ctx.run("op", (1, 2), (3,), ())
+    current[0] = 0
+    ctx.run("op", (1, 2), (3,), (0.5,))
+    assert seen == [0, 0]
+    # and a data error is read from where the kernels ran
+    current[0] = 1
+    monkeypatch.setattr(runtime.GpuContext, "_shared", ctx)
+
+    class Lib:
+        def lk_take_device_error(self, detail):
+            seen.append(current[0])
+            return 0
+
+    monkeypatch.setattr(_lib, "lib", Lib)
+    _lib.check_device_errors()
+    assert seen == [0, 0, 0] and current == [1]
