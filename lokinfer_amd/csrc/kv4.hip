@@ -53,7 +53,7 @@ __device__ __forceinline__ Kv4Word kv4Quantise(half8 x) {
 }
 
 // grid: T / 16, kv heads, B. A wave takes 4 rows, two at a time; the scales go through LDS, since a plane's neighbours are
-// neighbouring rows'. 32768 rows of 8 heads 65 us (172 MB, 2.7 TB/s; one row per wave and single scales: 108); 409 rows 4.2 us,
+// neighbouring rows'. 32768 rows of 8 heads 62 us (172 MB, 2.8 TB/s; one row per wave and single scales: 108); 409 rows 4.2 us,
 // of which 2.5 are a launch's.
 constexpr int kWriteRows = 16;
 __global__ __launch_bounds__(256) void kv4WriteKernel(char* __restrict__ kv, const h16* __restrict__ k,
@@ -101,8 +101,8 @@ struct Kv4QkrParams {
 };
 
 // One wave per (row, q head) and (row, kv head), grid rows / 4, heads: a q head is normalized and rotated to q, a kv head's key
-// likewise and quantised with its value. Arithmetic and roundings of the norm and the rotation as qkRopeKvKernel's. 16 / 8 heads: 1 row 4.4
-// us, 409 8.5, 2048 27 (instructions: a rotation's sine and cosine, 4 values per lane).
+// likewise and quantised with its value. Arithmetic and roundings of the norm and the rotation as qkRopeKvKernel's. 16 / 8 heads: 1 row 3.8
+// us, 409 8.1, 2048 26 (bytes: 6): the sine and cosine of a row's angles in 64 bits, which each of its 24 waves takes for itself.
 __global__ __launch_bounds__(256) void kv4QkRopeKernel(Kv4QkrParams p) {
   __shared__ __attribute__((aligned(16))) h16 rows[4][2 * KHD];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -205,9 +205,9 @@ struct Kv4Params {
 // less time, m at one with room for 2^8 up to 2.3%, which loses weights under 2^-25 of the largest. A score is one fma away
 // from m, its product with the scale not rounded by itself; where f32's steps are too coarse for that, from 2^20 on (at 2^28 the
 // difference would leave f16), the product is rounded first, as the maximum's was, and m is the maximum: 1% of the time.
-// 16 / 8 heads: one query over 417 rows 6.6 us and over 32768 12.6 + 4.1 of the joining launch (38 MB, 2.3 TB/s): latency, of one
-// chunk in the first. 2048 queries over as many rows 46 us, 370 TFLOP/s: bound by VALU (some 70% of the cycles, MFMA 30%), half of it
-// the codes' conversion, which 32 rows share, half the softmax. Tiles of f16 made once per call and shared through LDS took
+// 16 / 8 heads: one query over 417 rows 6.7 us and over 32768 12.3 + 4.2 of the joining launch (38 MB, 2.3 TB/s): latency, of one
+// chunk in the first; its 128 registers (4 waves a SIMD) leave 4 values in scratch. 2048 queries over as many rows 46 us, 370
+// TFLOP/s: bound by VALU (some 70% of the cycles, MFMA 28%), half of it the codes' conversion, which 32 rows share, half the softmax. Tiles of f16 made once per call and shared through LDS took
 // 6 + 50; more rows a wave leave one wave a SIMD (61 us).
 constexpr float kTop = 15.0f, kStart = 12.0f, kCoarse = 0x1p20f;
 template <int RB, int KW>

@@ -26,7 +26,7 @@ struct W4Layout {
 
 // One thread per (column of a tile, group), from w f16[K, N] (neighbouring threads on neighbouring columns) or NT f16[N, K]
 // (on neighbouring groups). The group's values stay in registers between the search for its scale and the codes. Runs once per
-// weight: 2048 x 12288 39 us (1.7 TB/s), NT 151936 x 2048 0.25 ms (3.1 TB/s).
+// weight: 2048 x 12288 34 us (1.9 TB/s), NT 151936 x 2048 0.26 ms (3.0 TB/s).
 template <bool NT, int G>
 __global__ __launch_bounds__(256) void w4QuantizeKernel(const h16* __restrict__ w, unsigned* __restrict__ q,
                                                         h16* __restrict__ s, W4Layout p, bool wide) {
@@ -305,7 +305,8 @@ __global__ __launch_bounds__(64 * WAVES) void w4SplitKernel(W4Params p) {
 }
 
 // Many tiles: x (normalized with RMS) goes to LDS once per workgroup, then each wave streams tiles of its own, U k blocks
-// ahead, over the tiles' ends. 1 x 2048 x 151936 30.7 us: 166 MB at 5.4 TB/s, above what a large copy reaches (4.7).
+// ahead, over the tiles' ends. 1 x 2048 x 151936 30.7 us: 166 MB at 5.4 TB/s, above what a large copy reaches (4.7); 4 rows 33,
+// 16 rows 53, with two workgroups a CU beside their 67 KB of x.
 constexpr int kStreamPad = 32;  // halves between x's rows in LDS
 template <int RU, int G, int W, bool F32, bool RMS>
 __global__ __launch_bounds__(256) void w4StreamKernel(W4Params p) {
@@ -446,10 +447,10 @@ __global__ __launch_bounds__(512) void w4RowsKernel(W4Params p) {
 // block's words of one c are loaded while the other c's are used. Each step's operands are made during the MFMAs of the one
 // before.
 // 128 x 256 (4 waves side by side, no split): 2048 x 2048 x 6144 of two weights 107 us, 960 TFLOP/s (the library's f16 product of
-// the same sizes, without SwiGLU: 107 us); MFMA 51%, VALU 48% of the cycles, two waves a SIMD, the conversion of the codes
-// (13 instructions for 8) between them. 64 x 64 with 8 k groups, for grids that would leave CUs empty: 409 x 6144 x 2048 23.5
-// us, 440 TFLOP/s (library 43 us); half of a round goes to its start and to joining the sums, and x passes the L1 once per
-// 64 columns. 32 x 64: 32 x 2048 x 12288 8.7 us.
+// the same sizes, without SwiGLU: 102 us); MFMA 51%, VALU 48% of the cycles, two waves a SIMD, the conversion of the codes
+// (13 instructions for 8) between them; neither is full, and what keeps the two from overlapping further is not known. 64 x 64 with 8 k groups, for grids that would leave CUs empty: 409 x 6144 x 2048 23.5
+// us, 440 TFLOP/s (library 37 us); half of a round goes to its start and to joining the sums, x passes the L1 once per 64
+// columns, and a code is converted for 64 rows alone (325 VALU to 32 MFMA instructions per 128 k). 32 x 64: 32 x 2048 x 12288 8.7 us.
 template <int BM, int NW, int KG, int G, int W, bool F32>
 __global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
   const Q4Masks masks;
