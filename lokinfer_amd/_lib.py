@@ -54,8 +54,9 @@ def lib():
 
 
 def check_device_errors() -> None:
-    """Waits for the context's GPU (the current one before there is a context) and raises LokinferError if a kernel recorded a data error since the last check
-    (a position outside a KV cache, an id out of range, a persistent kernel whose exchange timed out); clears it.
+    """Waits for the context's GPU (the current one before there is a context) and raises LokinferError if a kernel
+    recorded a data error since the last check (a position outside a KV cache, an id out of range, a persistent kernel
+    whose exchange timed out); clears it.
     The reference reports GPU failures the same way, at its next synchronisation (takeGpuError,
     src/runtime/executable.cpp:850-852 in lariaus/lokinfer)."""
     from .runtime import context_device

@@ -207,8 +207,8 @@ struct Kv4Params {
 // difference would leave f16), the product is rounded first, as the maximum's was, and m is the maximum: 1% of the time.
 // 16 / 8 heads: one query over 417 rows 6.7 us and over 32768 12.3 + 4.2 of the joining launch (38 MB, 2.3 TB/s): latency, of one
 // chunk in the first; its 128 registers (4 waves a SIMD) leave 4 values in scratch. 2048 queries over as many rows 46 us, 370
-// TFLOP/s: bound by VALU (some 70% of the cycles, MFMA 28%), half of it the codes' conversion, which 32 rows share, half the softmax. Tiles of f16 made once per call and shared through LDS took
-// 6 + 50; more rows a wave leave one wave a SIMD (61 us).
+// TFLOP/s: bound by VALU (some 70% of the cycles, MFMA 28%), half of it the codes' conversion, which 32 rows share, half the
+// softmax. Tiles of f16 made once per call and shared through LDS took 6 + 50; more rows a wave leave one wave a SIMD (61 us).
 constexpr float kTop = 15.0f, kStart = 12.0f, kCoarse = 0x1p20f;
 template <int RB, int KW>
 __global__ __launch_bounds__(64 * KW) __attribute__((amdgpu_waves_per_eu(RB == 1 ? 4 : 2))) void kv4AttnKernel(Kv4Params p) {

@@ -448,9 +448,10 @@ __global__ __launch_bounds__(512) void w4RowsKernel(W4Params p) {
 // before.
 // 128 x 256 (4 waves side by side, no split): 2048 x 2048 x 6144 of two weights 107 us, 960 TFLOP/s (the library's f16 product of
 // the same sizes, without SwiGLU: 102 us); MFMA 51%, VALU 48% of the cycles, two waves a SIMD, the conversion of the codes
-// (13 instructions for 8) between them; neither is full, and what keeps the two from overlapping further is not known. 64 x 64 with 8 k groups, for grids that would leave CUs empty: 409 x 6144 x 2048 23.5
-// us, 440 TFLOP/s (library 37 us); half of a round goes to its start and to joining the sums, x passes the L1 once per 64
-// columns, and a code is converted for 64 rows alone (325 VALU to 32 MFMA instructions per 128 k). 32 x 64: 32 x 2048 x 12288 8.7 us.
+// (13 instructions for 8) between them; neither is full, and what keeps the two from overlapping further is not known. 64 x 64
+// with 8 k groups, for grids that would leave CUs empty: 409 x 6144 x 2048 23.5 us, 440 TFLOP/s (library 37 us); half of a
+// round goes to its start and to joining the sums, x passes the L1 once per 64 columns, and a code is converted for 64 rows
+// alone (325 VALU to 32 MFMA instructions per 128 k). 32 x 64: 32 x 2048 x 12288 8.7 us.
 template <int BM, int NW, int KG, int G, int W, bool F32>
 __global__ __launch_bounds__(64 * NW * KG, 2) void w4GemmKernel(W4Params p) {
   const Q4Masks masks;

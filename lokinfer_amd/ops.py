@@ -933,9 +933,10 @@ def _beam_work(b, v, k) -> int:
 def beam_select_f32_gpu(logits, scores, done, k, eos):
     """(MI355X backend) A beam search's step over logits f32[B, V], the beams' scores f32[B] and done i64[B]: the k best of
     the candidates scores[b] + logits[b, t] - log sum exp logits[b] (a beam with done[b] != 0 has one, its score at eos[0]),
-    a beam's own ordered by their logits; equal logits of a beam to the lowest t, equal candidates (in 64 bits) of different
-    beams to the lowest b -> (scores f32[k], parents i64[k], tokens i64[k], done i64[k]), best first; done: the parent's, or
-    the token is one of `eos` (1 to 4 ids). What has no value (a NaN, a row or a score that is not finite) counts as -inf.
+    a beam's own ordered by their logits; equal logits of a beam to the lowest t, equal candidates of different beams to the
+    lowest b (the log-sums come from f32 exponentials: beams' candidates within some 2^-20 may stand in either order) ->
+    (scores f32[k], parents i64[k], tokens i64[k], done i64[k]), best first; done: the parent's, or the token is one of `eos`
+    (1 to 4 ids). What has no value (a NaN, a row or a score that is not finite) counts as -inf.
     B, k <= 32, V <= 262144. Not traceable."""
     if current_graph() is not None:
         raise OpError("beam_select runs eagerly or in a stream-captured function, not in a traced one")
