@@ -385,7 +385,8 @@ int lk_hip_kv4_reorder(void* kv, const int64_t* parents, const int64_t* n, int64
  *      (done[b] != 0) its score at eos[0] alone; the k best, a beam's own ordered by their logits; equal logits of a beam to
  *      the lowest t, equal candidates of different beams to the lowest b (the log-sums come from f32 exponentials: beams'
  *      candidates within some 2^-20 may stand in either order). B, k <= 32, V <= 262144, 1 to 4 eos ids. What has no value
- *      (NaN; a row or score that is not finite) counts as -inf. out_done: the parent's, or the token is an eos. Returns 3 when the workspace (16-byte aligned) is short. ---- */
+ *      (NaN; a row or score that is not finite) counts as -inf. out_done: the parent's, or the token is an eos. Returns 3 when
+ *      the workspace (16-byte aligned) is short. ---- */
 int64_t lk_hip_beam_select_workspace_bytes(int64_t b, int64_t v, int k);
 int lk_hip_beam_select_f32(const float* logits, const float* scores, const int64_t* done, float* out_scores,
                            int64_t* out_parents, int64_t* out_tokens, int64_t* out_done, int64_t b, int64_t v, int k,
